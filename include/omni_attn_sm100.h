@@ -30,6 +30,7 @@ extern "C" {
 /* dtype argument */
 #define OMNI_DTYPE_F16 0
 #define OMNI_DTYPE_BF16 1
+#define OMNI_DTYPE_F32 2   /* the rotary entry points only */
 
 /* Block types, as stored in block_mask_types (omni-attn-mma/omni_attn_torch.py:30-41). */
 #define OMNI_BLOCK_MASKED 0
@@ -54,6 +55,8 @@ extern "C" {
 #define OMNI_ERR_SCRATCH (-12)         /* scratch buffer smaller than OMNI_ATTN_SCRATCH_BYTES */
 #define OMNI_ERR_SOFTCAP (-14)         /* softcap negative or NaN */
 #define OMNI_ERR_WORKSPACE (-15)       /* omni_attn_bwd_sm100: workspace smaller than omni_attn_bwd_workspace_bytes() */
+#define OMNI_ERR_ROTARY (-16)          /* rotary_dim odd, negative or above head_dim, or no inv_freq for one that is not 0 */
+#define OMNI_ERR_CACHE (-17)           /* paged cache: sizes not positive, page_size no power of two from 16 to 1024, or heads that do not divide the queries' */
 #define OMNI_ERR_NOALLOC_LIMIT (-13)   /* omni_attn_fwd_noalloc_sm100: byte mask pool larger than the built-in scratch holds */
 
 /* Values a kernel can leave in *device_status (0 = clean run). Low byte = kind, upper bits = the
@@ -314,6 +317,92 @@ int omni_attn_bwd_rows_sm100(const void* q, const void* k, const void* v, const 
                              int head_dim, int q_block, int kv_block, int max_blocks, int num_partial, int dtype,
                              float scale, void* cuda_stream, int32_t* device_status_or_null, void* workspace,
                              long long workspace_bytes, float softcap, int rows);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Rotary positions with norms of the heads, and the paged key/value cache of generation. The reference leaves both to
+ * the model around its operator (transfusion_pytorch/transfusion.py:941-942 rotary, :933-939 the concatenated cache).
+ * --------------------------------------------------------------------------------------------------------------- */
+
+/* [B, heads, N, head_dim] with the strides given, in elements; head_dim is contiguous. */
+typedef struct omni_attn_heads {
+  const void* data;
+  long long stride_b, stride_h, stride_n;
+  int heads;
+} omni_attn_heads;
+
+/* What is done to the queries and keys: y = x / sqrt(mean(x^2) + eps) * weight over head_dim (with a weight), then pair p
+ * of the first rotary_dim elements is turned by position * inv_freq[p] and multiplied by factor. */
+typedef struct omni_attn_rotary {
+  const double* inv_freq;     /* device, [rotary_dim / 2], radians per position; may be NULL with rotary_dim 0 */
+  int rotary_dim;             /* even, 0 .. head_dim; the elements behind it pass through */
+  int half_layout;            /* members of pair p: 0: 2p and 2p + 1; 1: p and p + rotary_dim / 2 */
+  float factor;               /* 1 unless the frequencies were scaled for long contexts */
+  const void* positions;      /* device, [B, N] with the strides below, or NULL: n, in an append lengths[b] + n */
+  int positions_64;           /* 1: int64, 0: int32 */
+  long long pos_stride_b, pos_stride_n;
+  const void* q_weight;       /* device, [head_dim] or [heads, head_dim], or NULL: no norm */
+  const void* k_weight;
+  int weight_f32;             /* 1: the weights are fp32, 0: in the data's type */
+  int weight_per_head;        /* 1: [heads, head_dim] */
+  float eps;
+} omni_attn_rotary;
+
+/* Keys and values of B sequences in pages: token i of sequence b is row i % page_size of page
+ * page_table[b, i / page_size]. A page id outside [0, num_pages) is a page that is not there: nothing is stored to it,
+ * its tokens are not attended to, and the status word gets OMNI_STATUS_BAD_INDEX when it is met. */
+typedef struct omni_attn_paged_cache {
+  void* k_pages;              /* device, [num_pages, heads, page_size, head_dim], 16-byte aligned */
+  void* v_pages;
+  const int32_t* page_table;  /* device, [B, max_pages], table_stride entries from one sequence to the next */
+  long long table_stride;
+  const int32_t* lengths;     /* device, [B]: tokens that were there before this step's */
+  int num_pages, max_pages, page_size, heads;
+} omni_attn_paged_cache;
+
+/* q_out, k_out (contiguous [B, heads, N, head_dim]) = q, k normed and rotated; dtype fp16, bf16 or fp32. q or k may be
+ * NULL, with its output. inverse = 1 turns the other way, which is the backward of a call without norms. One kernel. */
+int omni_attn_rotary_sm100(const omni_attn_heads* q, const omni_attn_heads* k, void* q_out, void* k_out,
+                           const omni_attn_rotary* rotary, int B, int N, int head_dim, int dtype, int inverse,
+                           void* cuda_stream);
+
+/* Backward of omni_attn_rotary_sm100 for those of q and k that have a weight (the other must be NULL: its backward is
+ * the inverse call): dq, dk (contiguous) and dq_weight, dk_weight (in the weights' type) for the gradients d_q_out,
+ * d_k_out of the results. q and k are the forward's inputs. Two kernels; deterministic. */
+long long omni_attn_rotary_bwd_workspace_bytes(int q_heads, int k_heads, int B, int N, int head_dim, int weight_per_head);
+int omni_attn_rotary_bwd_sm100(const omni_attn_heads* q, const omni_attn_heads* k, const omni_attn_heads* d_q_out,
+                               const omni_attn_heads* d_k_out, void* dq, void* dk, void* dq_weight, void* dk_weight,
+                               const omni_attn_rotary* rotary, int B, int N, int head_dim, int dtype, void* workspace,
+                               long long workspace_bytes, void* cuda_stream);
+
+/* Stores N new tokens of each sequence: k, normed and rotated, and v go to the slots lengths[b] .. lengths[b] + counts[b]
+ * - 1 of the cache (counts NULL: N of each; tokens behind a sequence's count are ignored), and q_out (contiguous) = q
+ * normed and rotated, zero behind a sequence's count. q may be NULL with q_out, rotary may be NULL: stored as it is.
+ * Tokens beyond the page table's end are not stored (OMNI_STATUS_BAD_INDEX). `lengths` is read, not written. fp16, bf16.
+ * One kernel. Two sequences must not have a page in common that this call writes to. */
+int omni_attn_cache_append_sm100(const omni_attn_heads* q, const omni_attn_heads* k, const omni_attn_heads* v,
+                                 void* q_out, const omni_attn_paged_cache* cache, const int32_t* counts_or_null,
+                                 const omni_attn_rotary* rotary_or_null, int B, int N, int head_dim, int dtype,
+                                 void* cuda_stream, int32_t* device_status_or_null);
+
+/* Attention of T new tokens of each sequence (they are in the cache already) over the cache: row (b, h, t) attends keys
+ * [0, limit) through key/value head h / (H / cache.heads), with limit = limits[b, t] if limits is given, else
+ * lengths[b] + t + 1 (causal) or lengths[b] + counts[b], and never beyond the latter. Rows behind a sequence's count, and
+ * rows whose limit is not positive, are zero with LSE -inf.
+ *  q              in  [B, H, T, head_dim] fp16 or bf16, rows 16-byte aligned
+ *  out            out [B, H, T, head_dim] contiguous; lse [B, H, T] fp32, natural log, or NULL
+ *  softcap        tanh soft-cap of the scaled scores, 0 = none; scale <= 0: head_dim ** -0.5
+ *  shared_prefix  the first that many tokens of all sequences are in the same pages (rounded down to whole pages): they
+ *                 are read once for the batch. 0 = nothing is known to be shared. With a status word, table entries that
+ *                 break the promise are reported as OMNI_STATUS_BAD_INDEX.
+ *  workspace      omni_attn_cache_attention_workspace_bytes(...) bytes, 16-byte aligned; no state between calls, calls
+ *                 that overlap in time need two
+ * What a page holds behind a sequence's last token is never used. */
+long long omni_attn_cache_attention_workspace_bytes(int B, int H, int kv_heads, int T, int head_dim, int shared_prefix);
+int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* lse_or_null,
+                                    const omni_attn_paged_cache* cache, const int32_t* counts_or_null,
+                                    const int32_t* limits_or_null, int causal, int B, int T, int head_dim, int dtype,
+                                    float scale, float softcap, int shared_prefix, void* workspace,
+                                    long long workspace_bytes, void* cuda_stream, int32_t* device_status_or_null);
 
 /* Text for an OMNI_ERR_* code; the pointer is static storage. */
 const char* omni_attn_error_string(int code);

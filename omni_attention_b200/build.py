@@ -12,9 +12,11 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
+OBJ_DIR = os.path.join(PKG_DIR, "_obj")
 LIB_NAME = "libomni_attn_sm100.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 PYBIND_PATH = os.path.join(PKG_DIR, "omni_attn" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
@@ -23,8 +25,9 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",
 ]
-CUDA_SOURCES = ["omni_abi.cu", "omni_fwd_simple.cu", "omni_fwd_ws.cu", "omni_mask_build.cu", "omni_bwd.cu"]
-CUDA_HEADERS = ["ptx_sm100.cuh", "omni_common.cuh", "omni_launch.h", os.path.join("..", "..", "include", "omni_attn_sm100.h")]
+CUDA_SOURCES = ["omni_abi.cu", "omni_fwd_simple.cu", "omni_fwd_ws.cu", "omni_mask_build.cu", "omni_bwd.cu",
+                "omni_rotary.cu", "omni_cache_attn.cu", "omni_cache_abi.cu"]
+CUDA_HEADERS = ["ptx_sm100.cuh", "omni_common.cuh", "omni_launch.h", "omni_rotary.cuh", "omni_cache_attn.cuh", os.path.join("..", "..", "include", "omni_attn_sm100.h")]
 
 
 def _newer(target: str, deps) -> bool:
@@ -46,11 +49,20 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     deps = srcs + [os.path.join(CSRC, h) for h in CUDA_HEADERS]
     if not force and _newer(LIB_PATH, deps):
         return LIB_PATH
-    cmd = [_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *srcs]
-    if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    subprocess.run(cmd, check=True, cwd=CSRC)
+    # one object per source, several at a time; an object that is newer than its source and all headers stays
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    headers = [os.path.join(CSRC, h) for h in CUDA_HEADERS]
+    objs = [os.path.join(OBJ_DIR, os.path.basename(s)[:-3] + ".o") for s in srcs]
+    flags = [*NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else [])]
+
+    def compile_one(pair):
+        src, obj = pair
+        if force or not _newer(obj, [src, *headers]):
+            subprocess.run([_nvcc(), *flags, "-c", "-o", obj, src], check=True, cwd=CSRC)
+
+    with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 1)) as pool:
+        list(pool.map(compile_one, zip(srcs, objs)))
+    subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *objs], check=True, cwd=CSRC)
     return LIB_PATH
 
 
@@ -59,7 +71,7 @@ def build_pybind(force: bool = False) -> str:
     from torch.utils import cpp_extension
 
     src = os.path.join(CSRC, "omni_attn_pybind.cc")
-    if not force and _newer(PYBIND_PATH, [src, LIB_PATH, os.path.join(PKG_DIR, "..", "include", "omni_attn_sm100.h")]):
+    if not force and _newer(PYBIND_PATH, [src, os.path.join(CSRC, "omni_cache_pybind.h"), LIB_PATH, os.path.join(PKG_DIR, "..", "include", "omni_attn_sm100.h")]):
         return PYBIND_PATH
     inc = []
     for p in cpp_extension.include_paths() + [sysconfig.get_paths()["include"], "/usr/local/cuda/include"]:

@@ -312,6 +312,10 @@ __global__ void pack_partial_kernel(const uint8_t* __restrict__ src, uint32_t* _
 }  // namespace
 }  // namespace omni
 
+namespace omni {
+void set_last_cuda_error(int code) { g_last_cuda_error = code; }
+}  // namespace omni
+
 extern "C" {
 
 int omni_attn_fwd_sm100(const void* q, const void* k, const void* v, void* o, float* lse_or_null,
@@ -584,6 +588,9 @@ const char* omni_attn_error_string(int code) {
     case OMNI_ERR_SCRATCH: return "scratch buffer smaller than OMNI_ATTN_SCRATCH_BYTES";
     case OMNI_ERR_SOFTCAP: return "softcap must be >= 0 (0 = none); the plain kernel has no soft-cap";
     case OMNI_ERR_WORKSPACE: return "workspace smaller than omni_attn_bwd_workspace_bytes()";
+    case OMNI_ERR_ROTARY: return "rotary_dim must be even, 0 <= rotary_dim <= head_dim, with inv_freq unless it is 0";
+    case OMNI_ERR_CACHE:
+      return "paged cache: sizes must be positive, page_size a power of two from 16 to 1024, and its heads must divide the queries' heads";
     case OMNI_ERR_NOALLOC_LIMIT:
       return "byte-per-element partial pool has more than OMNI_ATTN_NOALLOC_MAX_PARTIAL (1024) tiles: too large for "
              "the built-in scratch; pass a bit-packed pool or use omni_attn_fwd_scratch_sm100";

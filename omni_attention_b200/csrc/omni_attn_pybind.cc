@@ -14,12 +14,15 @@
 #include <dlfcn.h>
 #include <torch/extension.h>
 
+#include <climits>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <optional>
 #include <sstream>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <utility>
 
 #include "../../include/omni_attn_sm100.h"
@@ -37,6 +40,12 @@ struct Library {
   decltype(&::omni_attn_bwd_rows_sm100) bwd_rows = &::omni_attn_bwd_rows_sm100;
   decltype(&::omni_attn_build_mask_sm100) build_mask = &::omni_attn_build_mask_sm100;
   decltype(&::omni_attn_bwd_workspace_bytes) bwd_workspace_bytes = &::omni_attn_bwd_workspace_bytes;
+  decltype(&::omni_attn_rotary_sm100) rotary = &::omni_attn_rotary_sm100;
+  decltype(&::omni_attn_rotary_bwd_workspace_bytes) rotary_bwd_workspace = &::omni_attn_rotary_bwd_workspace_bytes;
+  decltype(&::omni_attn_rotary_bwd_sm100) rotary_bwd = &::omni_attn_rotary_bwd_sm100;
+  decltype(&::omni_attn_cache_append_sm100) cache_append = &::omni_attn_cache_append_sm100;
+  decltype(&::omni_attn_cache_attention_workspace_bytes) cache_attention_workspace = &::omni_attn_cache_attention_workspace_bytes;
+  decltype(&::omni_attn_cache_attention_sm100) cache_attention = &::omni_attn_cache_attention_sm100;
   decltype(&::omni_attn_error_string) error_string = &::omni_attn_error_string;
   decltype(&::omni_attn_last_cuda_error) last_cuda_error = &::omni_attn_last_cuda_error;
 };
@@ -61,6 +70,12 @@ void use_library(const std::string& path) {
   look_up(handle, "omni_attn_bwd_rows_sm100", found.bwd_rows);
   look_up(handle, "omni_attn_build_mask_sm100", found.build_mask);
   look_up(handle, "omni_attn_bwd_workspace_bytes", found.bwd_workspace_bytes);
+  look_up(handle, "omni_attn_rotary_sm100", found.rotary);
+  look_up(handle, "omni_attn_rotary_bwd_workspace_bytes", found.rotary_bwd_workspace);
+  look_up(handle, "omni_attn_rotary_bwd_sm100", found.rotary_bwd);
+  look_up(handle, "omni_attn_cache_append_sm100", found.cache_append);
+  look_up(handle, "omni_attn_cache_attention_workspace_bytes", found.cache_attention_workspace);
+  look_up(handle, "omni_attn_cache_attention_sm100", found.cache_attention);
   look_up(handle, "omni_attn_error_string", found.error_string);
   look_up(handle, "omni_attn_last_cuda_error", found.last_cuda_error);
   library = found;
@@ -569,9 +584,12 @@ pybind11::object build_mask(torch::Tensor modality_positions, int B, int H, int 
   return pybind11::make_tuple(mask, nb, idx, types, pidx, bits, count);
 }
 
+#include "omni_cache_pybind.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  define_cache(m);
   m.def("omni_attn_mma_stages_split_q_shared_kv", &omni_attn_mma_stages_split_q_shared_kv,
         "omni_attn_mma_stages_split_q_shared_kv");
   m.def("omni_attn_simple_kernel", &omni_attn_simple_kernel, "omni_attn_simple_kernel");

@@ -1,0 +1,34 @@
+// Launch parameters of the attention over a paged key/value cache (omni_cache_attn.cu).
+#pragma once
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace omni {
+
+struct CacheAttnParams {
+  const void* q;                // [B, H, T, D], strides in elements, every row 16-byte aligned
+  long long qs_b, qs_h, qs_t;
+  void* out;                    // [B, H, T, D] contiguous
+  float* lse;                   // [B, H, T] or null
+  const void* k_pages;          // [num_pages, Hkv, page_size, D]
+  const void* v_pages;
+  const int32_t* page_table;    // [B, max_pages]
+  long long table_stride;
+  const int32_t* lengths;       // [B] tokens before this call's T
+  const int32_t* counts;        // [B] or null (= T)
+  const int32_t* limits;        // [B, T] keys a row sees, or null
+  int32_t* status;
+  float* partial;               // workspace, see omni_cache_attn.cu
+  long long capacity;           // max_pages * page_size
+  int B, H, Hkv, G, T;
+  int max_pages, num_pages, page_shift;
+  int prefix;                   // tokens that all sequences have in the same pages (multiple of the page size), or 0
+  int causal;
+  float scale;                  // softmax scale
+  float softcap;                // 0 = none
+};
+
+cudaError_t launch_cache_attn(int head_dim, bool bf16, const CacheAttnParams& p, cudaStream_t stream);
+long long cache_attn_workspace_bytes(int B, int H, int Hkv, int T, int head_dim, bool prefix);
+
+}  // namespace omni

@@ -32,6 +32,9 @@ cudaError_t launch_ws(int head_dim, bool bf16, const CUtensorMap& tmQ, const CUt
 cudaError_t launch_bwd(int head_dim, bool bf16, const CUtensorMap& tmQ, const CUtensorMap& tmK,
                        const CUtensorMap& tmV, const CUtensorMap& tmdO, const BwdParams& p, cudaStream_t stream);
 
+// What omni_attn_last_cuda_error returns on this thread.
+void set_last_cuda_error(int code);
+
 // Sets a kernel's dynamic shared memory limit once per device (any host thread may be the first).
 struct SmemAttrOnce {
   std::once_flag once;

@@ -48,6 +48,12 @@ ABI_SYMBOLS = (
     "omni_attn_bwd_sm100",
     "omni_attn_bwd_ex_sm100",
     "omni_attn_bwd_rows_sm100",
+    "omni_attn_rotary_sm100",
+    "omni_attn_rotary_bwd_workspace_bytes",
+    "omni_attn_rotary_bwd_sm100",
+    "omni_attn_cache_append_sm100",
+    "omni_attn_cache_attention_workspace_bytes",
+    "omni_attn_cache_attention_sm100",
     "omni_attn_error_string",
     "omni_attn_last_cuda_error",
     "omni_attn_abi_version",
