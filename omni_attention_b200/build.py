@@ -26,8 +26,9 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC",
 ]
 CUDA_SOURCES = ["omni_abi.cu", "omni_fwd_simple.cu", "omni_fwd_ws.cu", "omni_mask_build.cu", "omni_bwd.cu",
-                "omni_rotary.cu", "omni_cache_attn.cu", "omni_cache_abi.cu"]
-CUDA_HEADERS = ["ptx_sm100.cuh", "omni_common.cuh", "omni_launch.h", "omni_rotary.cuh", "omni_cache_attn.cuh", os.path.join("..", "..", "include", "omni_attn_sm100.h")]
+                "omni_rotary.cu", "omni_cache_attn.cu", "omni_cache_wide.cu", "omni_cache_abi.cu"]
+CUDA_HEADERS = ["ptx_sm100.cuh", "omni_common.cuh", "omni_launch.h", "omni_rotary.cuh", "omni_cache_attn.cuh", "omni_cache_line.cuh",
+                os.path.join("..", "..", "include", "omni_attn_sm100.h")]
 
 
 def _newer(target: str, deps) -> bool:

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "../../include/omni_attn_sm100.h"
+#include "omni_cache_attn.cuh"
 #include "omni_launch.h"
 
 namespace omni {
@@ -314,6 +315,31 @@ __global__ void pack_partial_kernel(const uint8_t* __restrict__ src, uint32_t* _
 
 namespace omni {
 void set_last_cuda_error(int code) { g_last_cuda_error = code; }
+
+long long wait_cycle_budget() { return g_wait_cycles.load(std::memory_order_relaxed); }
+
+// The pages of a cache as a matrix [num_pages * heads * page_size, head_dim]; box = up to 128 tokens of one page and head x
+// 64 columns, 128-byte swizzle. Columns beyond head_dim (head_dim 32) read as zeros.
+cudaError_t make_page_maps(const CacheAttnParams& p, int head_dim, bool bf16, CUtensorMap* tmK, CUtensorMap* tmV) {
+  if (bind_context() != OMNI_OK) return static_cast<cudaError_t>(g_last_cuda_error);
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return cudaErrorNotSupported;
+  const int page = 1 << p.page_shift;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(p.num_pages) * p.Hkv * page};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(head_dim) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(page < 128 ? page : 128)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap* maps[2] = {tmK, tmV};
+  const void* pages[2] = {p.k_pages, p.v_pages};
+  for (int i = 0; i < 2; ++i) {
+    if (fn(maps[i], type, 2, const_cast<void*>(pages[i]), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+      return cudaErrorInvalidValue;
+    }
+  }
+  return cudaSuccess;
+}
 }  // namespace omni
 
 extern "C" {

@@ -35,6 +35,7 @@ int check_cache(const omni_attn_paged_cache* c) {
     return OMNI_ERR_CACHE;
   }
   if (static_cast<long long>(c->max_pages) * c->page_size > 0x7FFF0000LL) return OMNI_ERR_TOO_LONG;   // token numbers are int32
+  if (static_cast<long long>(c->num_pages) * c->heads * c->page_size >= (1LL << 31)) return OMNI_ERR_TOO_LONG;   // and so are rows of the pages
   if (misaligned(c->k_pages) || misaligned(c->v_pages)) return OMNI_ERR_ALIGNMENT;
   return OMNI_OK;
 }
@@ -267,6 +268,7 @@ int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* 
   p.causal = causal;
   p.scale = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(head_dim));
   p.softcap = softcap;
+  p.wait_cycles = wait_cycle_budget();
   return ended(launch_cache_attn(head_dim, dtype == OMNI_DTYPE_BF16, p, static_cast<cudaStream_t>(cuda_stream)));
 }
 

@@ -17,8 +17,7 @@
 // The maximum moves only when it would grow by more than 2^8 (scores are in the log2 domain), P goes into the product as
 // a 16-bit value plus the 16-bit rest (two products; the tensor cores have the room), so the only rounding that shows
 // is that of the result.
-#include "omni_cache_attn.cuh"
-#include "omni_common.cuh"
+#include "omni_cache_line.cuh"
 #include "omni_launch.h"
 
 namespace omni {
@@ -38,91 +37,6 @@ struct CacheCfg {
   static constexpr int kJoin = kWarps * kRows * (D + 4) * 4;               // O shares, over the ring
   static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
 };
-
-// ---------------------------------------------------------------------------------------------------------------------
-// what a sequence holds, and the line of units
-// ---------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ int count_of(const CacheAttnParams& p, int b) {
-  return p.counts == nullptr ? p.T : min(max(__ldg(p.counts + b), 0), p.T);
-}
-// tokens of sequence b that exist once this call's are in: [0, capacity]
-__device__ __forceinline__ int total_of(const CacheAttnParams& p, int b) {
-  const long long n = static_cast<long long>(max(__ldg(p.lengths + b), 0)) + count_of(p, b);
-  return static_cast<int>(n < p.capacity ? n : p.capacity);
-}
-// keys row (b, t) sees
-__device__ __forceinline__ int limit_of(const CacheAttnParams& p, int b, int t) {
-  if (t >= count_of(p, b)) return 0;
-  const int total = total_of(p, b);
-  if (p.limits != nullptr) return min(__ldg(p.limits + static_cast<long long>(b) * p.T + t), total);
-  if (!p.causal) return total;
-  const long long n = static_cast<long long>(max(__ldg(p.lengths + b), 0)) + t + 1;
-  return static_cast<int>(n < total ? n : total);
-}
-__device__ __forceinline__ int tiles_between(int from, int to) {
-  return to > from ? (to - from + kTileKeys - 1) / kTileKeys : 1;   // a triple without keys still has rows to write
-}
-
-// A segment is a set of keys with the rows that read it: the shared prefix with the rows of all sequences (first, if
-// there is one), then each sequence's own keys with its own rows.
-struct Line {
-  long long units;    // all of them
-  long long span;     // of one CTA
-  long long prefix_units;
-  int prefix_seq;     // the sequence whose page table the prefix is read through: the longest
-  int prefix_end;
-  int tiles_prefix, rt_prefix, rt_own;
-};
-
-__device__ __forceinline__ long long own_units(const CacheAttnParams& p, const Line& ln, int b) {
-  return static_cast<long long>(p.Hkv) * ln.rt_own * tiles_between(p.prefix, total_of(p, b));
-}
-
-// All lanes of a warp; every CTA of both kernels comes to the same line.
-__device__ __forceinline__ Line make_line(const CacheAttnParams& p, int ctas) {
-  Line ln;
-  ln.rt_own = (p.G * p.T + kRows - 1) / kRows;
-  const int lane = threadIdx.x & 31;
-  long long sum = 0;
-  int most = -1, seq = 0;
-  for (int b = lane; b < p.B; b += 32) {
-    sum += own_units(p, ln, b);
-    const int total = total_of(p, b);
-    if (total > most) {
-      most = total;
-      seq = b;
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    const int m2 = __shfl_xor_sync(0xFFFFFFFFu, most, o), s2 = __shfl_xor_sync(0xFFFFFFFFu, seq, o);
-    if (m2 > most || (m2 == most && s2 < seq)) {
-      most = m2;
-      seq = s2;
-    }
-  }
-  ln.prefix_units = 0;
-  ln.prefix_seq = seq;
-  ln.prefix_end = min(p.prefix, most);
-  ln.tiles_prefix = 0;
-  ln.rt_prefix = 0;
-  if (p.prefix > 0) {
-    ln.rt_prefix = static_cast<int>((static_cast<long long>(p.B) * p.G * p.T + kRows - 1) / kRows);
-    ln.tiles_prefix = tiles_between(0, ln.prefix_end);
-    ln.prefix_units = static_cast<long long>(p.Hkv) * ln.rt_prefix * ln.tiles_prefix;
-  }
-  ln.units = sum + ln.prefix_units;
-  ln.span = (ln.units + ctas - 1) / ctas;
-  return ln;
-}
-
-// One share in the workspace: O [16][D], then the rows' maxima [16] (log2 domain) and sums [16]. CTA i has share 2 i
-// (of a triple that began before its span) and 2 i + 1 (of one that begins in it and goes on after it); with a prefix, triples
-// inside one span have a share of their own behind those: prefix triples first, then the sequences'.
-__device__ __forceinline__ float* share_at(const CacheAttnParams& p, long long index, int d) {
-  return p.partial + index * (kRows * (d + 2));
-}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // instructions
@@ -191,25 +105,11 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
   }
 }
 
-// Which (batch element, token, query head of the group) row r of a segment is.
-struct RowId {
-  int b, t, g;
-};
-__device__ __forceinline__ RowId row_of(const CacheAttnParams& p, bool prefix, int b, int r) {
-  RowId id;
-  const int per = p.G * p.T;
-  id.b = prefix ? r / per : b;
-  const int in = prefix ? r - id.b * per : r;
-  id.t = in / p.G;
-  id.g = in - id.t * p.G;
-  return id;
-}
-
 // ---------------------------------------------------------------------------------------------------------------------
 // the kernel
 // ---------------------------------------------------------------------------------------------------------------------
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads) omni_cache_attn_kernel(const __grid_constant__ CacheAttnParams p) {
+__global__ void __launch_bounds__(kThreads) omni_cache_attn_kernel(const __grid_constant__ CacheAttnParams p, const __grid_constant__ CacheLaunch how) {
   using Cfg = CacheCfg<D>;
   constexpr int KS = D / 16;        // steps of Q K^T
   constexpr int CH = D / 8;         // 16-byte chunks of a row
@@ -220,60 +120,23 @@ __global__ void __launch_bounds__(kThreads) omni_cache_attn_kernel(const __grid_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int quad = lane >> 2, pos = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * (Cfg::kStages * Cfg::kStageBytes);
-  const Line ln = make_line(p, gridDim.x);
-  long long u = ln.span * blockIdx.x;
-  const long long u_end = min(u + ln.span, ln.units);
-  if (u >= u_end) return;
-
-  // the segment the span begins in: -1 the prefix, else a sequence; `base` = its first unit
-  int seg = -1;
-  long long base = 0;
-  if (u >= ln.prefix_units) {
-    base = ln.prefix_units;
-    for (int b0 = 0;; b0 += 32) {
-      const int b = b0 + lane;
-      long long mine = b < p.B ? own_units(p, ln, b) : 0, upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        if (lane >= o) upto += v;
-      }
-      const unsigned past = __ballot_sync(0xFFFFFFFFu, base + upto > u);
-      if (past != 0) {
-        const int l = __ffs(past) - 1;
-        seg = b0 + l;
-        base += __shfl_sync(0xFFFFFFFFu, upto - mine, l);
-        break;
-      }
-      base += __shfl_sync(0xFFFFFFFFu, upto, 31);
-    }
-  }
-
   const float scale_log2 = p.scale * 1.4426950408889634f;
-  while (u < u_end) {
-    const bool prefix = seg < 0;
-    const int rts = prefix ? ln.rt_prefix : ln.rt_own;
-    const int table_of = prefix ? ln.prefix_seq : seg;
-    const int key0 = prefix ? 0 : p.prefix;
-    const int total = prefix ? ln.prefix_end : total_of(p, seg);
-    const int tiles = prefix ? ln.tiles_prefix : tiles_between(key0, total);
-    const long long triple = (u - base) / tiles;
-    const int tile0 = static_cast<int>(u - base - triple * tiles);
-    const int tile1 = static_cast<int>(min(static_cast<long long>(tiles), tile0 + (u_end - u)));
-    const int hk = static_cast<int>(triple / rts), rt = static_cast<int>(triple - static_cast<long long>(hk) * rts);
-    const int rows = prefix ? p.B * p.G * p.T : p.G * p.T;
+  Walk walk(p, how);
+  Piece pc;
+  while (walk.next(p, pc)) {
+    const int hk = pc.hk, rows = pc.rows, tile0 = pc.tile0, tile1 = pc.tile1;
 
     // this thread's two rows: their queries as mma operands, their numbers of visible keys
     uint32_t qf[KS][4];
     int lim[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = rt * kRows + quad + 8 * i;
+      const int r = pc.rt * kRows + quad + 8 * i;
       lim[i] = 0;
       const uint32_t* src = nullptr;
       if (r < rows) {
-        const RowId id = row_of(p, prefix, seg, r);
-        lim[i] = min(limit_of(p, id.b, id.t), total);
+        const RowId id = row_of(p, pc.prefix, pc.seg, r);
+        lim[i] = min(limit_of(p, id.b, id.t), pc.total);
         src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + id.b * p.qs_b +
                                                 (static_cast<long long>(hk) * p.G + id.g) * p.qs_h + id.t * p.qs_t);
       }
@@ -296,10 +159,10 @@ __global__ void __launch_bounds__(kThreads) omni_cache_attn_kernel(const __grid_
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     // this warp's 16 keys of tile t begin at key_at(t)
-    auto key_at = [&](int t) { return key0 + t * kTileKeys + warp * 16; };
+    auto key_at = [&](int t) { return pc.key0 + t * kTileKeys + warp * 16; };
     auto page_at = [&](int t) -> int {
       const int key = key_at(t);
-      return t < tile1 && key < lim_max ? __ldg(p.page_table + table_of * p.table_stride + (key >> p.page_shift)) : -1;
+      return t < tile1 && key < lim_max ? __ldg(p.page_table + pc.table_of * p.table_stride + (key >> p.page_shift)) : -1;
     };
     uint32_t there = 0;   // bit (tile & 31): the tile's page exists
     auto issue = [&](int t, int page) {
@@ -436,21 +299,9 @@ __global__ void __launch_bounds__(kThreads) omni_cache_attn_kernel(const __grid_
       }
     }
     __syncthreads();
-    const bool whole = tile0 == 0 && tile1 == tiles;
-    long long share = -1;
-    if (!whole) {
-      share = 2LL * blockIdx.x + (tile0 == 0 ? 1 : 0);
-    } else if (p.prefix > 0) {
-      share = 2LL * gridDim.x;
-      if (prefix) {
-        share += triple;
-      } else {
-        share += static_cast<long long>(p.Hkv) * ln.rt_prefix + (static_cast<long long>(seg) * p.Hkv * ln.rt_own + triple);
-      }
-    }
     constexpr int LPR = D / 4;    // threads of a row, 4 columns each
     for (int r = threadIdx.x / LPR; r < kRows; r += kThreads / LPR) {
-      const int row = rt * kRows + r, col = (threadIdx.x % LPR) * 4;
+      const int row = pc.rt * kRows + r, col = (threadIdx.x % LPR) * 4;
       if (row >= rows) break;
       float top = -INFINITY;
 #pragma unroll
@@ -468,16 +319,15 @@ __global__ void __launch_bounds__(kThreads) omni_cache_attn_kernel(const __grid_
         acc.z += f * v.z;
         acc.w += f * v.w;
       }
-      if (share >= 0) {
-        float* to = share_at(p, share, D);
+      if (pc.share >= 0) {
+        float* to = share_at(p, how, pc.share, D);
         *reinterpret_cast<float4*>(to + r * D + col) = acc;
         if (col == 0) {
           to[kRows * D + r] = top;
           to[kRows * D + kRows + r] = sum;
         }
       } else {
-        const RowId id = row_of(p, prefix, seg, row);
-        const long long at_row = (static_cast<long long>(id.b) * p.H + static_cast<long long>(hk) * p.G + id.g) * p.T + id.t;
+        const long long at_row = out_row(p, row_of(p, pc.prefix, pc.seg, row), hk);
         const bool any = !(sum == 0.f);   // NaN shows
         const float inv = 1.f / sum;
         uint2 out = make_uint2(0u, 0u);
@@ -490,56 +340,55 @@ __global__ void __launch_bounds__(kThreads) omni_cache_attn_kernel(const __grid_
       }
     }
     __syncthreads();   // the shares are read: the next triple's stages may go over them
-
-    u += tile1 - tile0;
-    if (u < u_end && u - base >= static_cast<long long>(p.Hkv) * rts * tiles) {
-      base += static_cast<long long>(p.Hkv) * rts * tiles;
-      ++seg;
-    }
   }
 }
 
-// Joins the shares of the rows that no single span covered. One CTA per (sequence, key/value head, 16-row tile), a warp
-// per row.
+// Joins the shares of the rows that no single span covered. One CTA per (sequence, key/value head, 16 rows), a warp per
+// row. `pre` is the launch that had the prefix (if there is one), `own` the one that had the sequences' own keys; they may
+// be the same launch.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128) omni_cache_join_kernel(const __grid_constant__ CacheAttnParams p, int ctas) {
+__global__ void __launch_bounds__(128) omni_cache_join_kernel(const __grid_constant__ CacheAttnParams p, const __grid_constant__ CacheLaunch pre,
+                                                              const __grid_constant__ CacheLaunch own) {
   constexpr int V = D / 32;   // columns of a lane
-  const Line ln = make_line(p, ctas);
+  const int rows = p.G * p.T;
+  const int groups = (rows + kRows - 1) / kRows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long triples = static_cast<long long>(p.Hkv) * ln.rt_own;
-  const int seq = static_cast<int>(blockIdx.x / triples);
-  const long long triple = blockIdx.x - seq * triples;
-  const int hk = static_cast<int>(triple / ln.rt_own), rt = static_cast<int>(triple % ln.rt_own);
+  const int seq = static_cast<int>(blockIdx.x / (static_cast<long long>(p.Hkv) * groups));
+  const int in_seq = static_cast<int>(blockIdx.x - static_cast<long long>(seq) * p.Hkv * groups);
+  const int hk = in_seq / groups, group = in_seq % groups;
 
-  if (p.prefix > 0 && p.status != nullptr && triple == 0) {   // is the prefix in the same pages?
-    const int pages = (min(p.prefix, total_of(p, seq)) + (1 << p.page_shift) - 1) >> p.page_shift;
-    bool same = true;
-    for (int i = threadIdx.x; i < pages; i += blockDim.x) {
-      same &= __ldg(p.page_table + seq * p.table_stride + i) == __ldg(p.page_table + ln.prefix_seq * p.table_stride + i);
-    }
-    if (!same) atomicCAS(p.status, 0, kStatusBadIndex);
-  }
-
+  const Line lo = make_line(p, own);
   long long before = 0;
-  for (int b = lane; b < seq; b += 32) before += own_units(p, ln, b);
+  for (int b = lane; b < seq; b += 32) before += lo.own_units(p, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
-  const long long tiles = tiles_between(p.prefix, total_of(p, seq));
-  const long long first = ln.prefix_units + before + triple * tiles;
-  const long long c0 = first / ln.span, c1 = (first + tiles - 1) / ln.span;
+  const long long tiles = lo.tiles_between(p.prefix, total_of(p, seq));
+  const long long triple = static_cast<long long>(hk) * lo.rt_own + group * kRows / own.rows;
+  const long long first = lo.prefix_units + before + triple * tiles;
+  const long long c0 = first / lo.span, c1 = (first + tiles - 1) / lo.span;
   if (p.prefix == 0 && c0 == c1) return;   // written by the one CTA that had it
-  const long long whole = 2LL * ctas;
+  Line lp = lo;
+  if (p.prefix > 0) {
+    lp = make_line(p, pre);
+    if (p.status != nullptr && in_seq == 0) {   // is the prefix in the same pages?
+      const int pages = (min(p.prefix, total_of(p, seq)) + (1 << p.page_shift) - 1) >> p.page_shift;
+      bool same = true;
+      for (int i = threadIdx.x; i < pages; i += blockDim.x) {
+        same &= __ldg(p.page_table + seq * p.table_stride + i) == __ldg(p.page_table + lp.prefix_seq * p.table_stride + i);
+      }
+      if (!same) atomicCAS(p.status, 0, kStatusBadIndex);
+    }
+  }
 
-  const int rows = p.G * p.T;
   for (int r = warp; r < kRows; r += 4) {
-    const int row = rt * kRows + r;
+    const int row = group * kRows + r;
     if (row >= rows) break;
     float top = -INFINITY, sum = 0.f, acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    auto add = [&](long long share, int in) {
-      const float* from = share_at(p, share, D);
-      const float m2 = __ldcg(from + kRows * D + in), l2 = __ldcg(from + kRows * D + kRows + in);
+    auto add = [&](const CacheLaunch& how, long long share, int in) {
+      const float* from = share_at(p, how, share, D);
+      const float m2 = __ldcg(from + how.rows * D + in), l2 = __ldcg(from + how.rows * D + how.rows + in);
       float v[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = __ldcg(from + in * D + lane + 32 * i);
@@ -550,25 +399,22 @@ __global__ void __launch_bounds__(128) omni_cache_join_kernel(const __grid_const
       for (int i = 0; i < V; ++i) acc[i] = acc[i] * f1 + v[i] * f2;
       top = to;
     };
+    auto add_triple = [&](const CacheLaunch& how, long long from, long long n, long long span, long long whole, int in) {
+      const long long i0 = from / span, i1 = (from + n - 1) / span;
+      if (i0 == i1) {
+        add(how, whole, in);
+      } else {
+        for (long long i = i0; i <= i1; ++i) add(how, 2 * i + (i == i0 ? 1 : 0), in);
+      }
+    };
     if (p.prefix > 0) {
       const long long gr = static_cast<long long>(seq) * rows + row;   // the row in the prefix segment
-      const long long pt = static_cast<long long>(hk) * ln.rt_prefix + gr / kRows;
-      const int in = static_cast<int>(gr % kRows);
-      const long long f = pt * ln.tiles_prefix;
-      const long long d0 = f / ln.span, d1 = (f + ln.tiles_prefix - 1) / ln.span;
-      if (d0 == d1) {
-        add(whole + pt, in);
-      } else {
-        for (long long i = d0; i <= d1; ++i) add(2 * i + (i == d0 ? 1 : 0), in);
-      }
+      const long long pt = static_cast<long long>(hk) * lp.rt_prefix + gr / pre.rows;
+      add_triple(pre, pt * lp.tiles_prefix, lp.tiles_prefix, lp.span, 2LL * pre.ctas + pt, static_cast<int>(gr % pre.rows));
     }
-    if (c0 == c1) {
-      add(whole + static_cast<long long>(p.Hkv) * ln.rt_prefix + static_cast<long long>(blockIdx.x), r);
-    } else {
-      for (long long i = c0; i <= c1; ++i) add(2 * i + (i == c0 ? 1 : 0), r);
-    }
-    const RowId id = row_of(p, false, seq, row);
-    const long long at_row = (static_cast<long long>(id.b) * p.H + static_cast<long long>(hk) * p.G + id.g) * p.T + id.t;
+    add_triple(own, first, tiles, lo.span, 2LL * own.ctas + static_cast<long long>(p.Hkv) * (lo.rt_prefix + static_cast<long long>(seq) * lo.rt_own) + triple,
+               row % own.rows);
+    const long long at_row = out_row(p, row_of(p, false, seq, row), hk);
     const bool any = !(sum == 0.f);   // NaN shows
     const float inv = 1.f / sum;
 #pragma unroll
@@ -585,32 +431,79 @@ __global__ void __launch_bounds__(128) omni_cache_join_kernel(const __grid_const
   }
 }
 
-constexpr int kMaxCtas = 148 * 2;   // two CTAs on each SM at head_dim 128
+constexpr int kNarrowCtas = 148 * 2;   // two CTAs on each SM at head_dim 128
+
+// The launches of a call: one over everything, or one over the prefix and one over the sequences' own keys where only one
+// of the two has more than 16 rows to a key/value head (the 16-row tile would read its keys once for every 16 rows).
+struct Plan {
+  CacheLaunch of[2];   // the prefix's, the sequences'; equal if one launch has both
+  bool wide[2];
+  long long floats;
+};
+
+Plan make_plan(int B, int Hkv, long long per, int head_dim, bool prefix, long long capacity) {
+  Plan pl;
+  pl.floats = 0;
+  const long long rows[2] = {B * per, per};
+  for (int i = 0; i < 2; ++i) pl.wide[i] = rows[i] > kRows;
+  if (!prefix) pl.wide[0] = pl.wide[1];
+  const bool one = !prefix || pl.wide[0] == pl.wide[1];
+  for (int i = 0; i < 2; ++i) {
+    CacheLaunch& how = pl.of[i];
+    how.rows = pl.wide[i] ? kWideRows : kRows;
+    how.keys = pl.wide[i] ? kWideKeys : kTileKeys;
+    how.prefix = prefix && (one || i == 0);
+    how.own = one || i == 1;
+    if (i == 1 && one) {
+      how = pl.of[0];
+      break;
+    }
+    long long triples = 0;
+    if (how.prefix) triples += Hkv * ((rows[0] + how.rows - 1) / how.rows);
+    if (how.own) triples += static_cast<long long>(B) * Hkv * ((rows[1] + how.rows - 1) / how.rows);
+    const long long most = triples * ((capacity + how.keys - 1) / how.keys);
+    const int limit = pl.wide[i] ? kWideCtas : kNarrowCtas;
+    how.ctas = static_cast<int>(most < limit ? most : limit);
+    how.share0 = pl.floats;
+    pl.floats += (2LL * limit + (prefix ? triples : 0)) * how.rows * (head_dim + 2);
+  }
+  return pl;
+}
 
 template <int D, bool BF16>
-cudaError_t launch_t(const CacheAttnParams& p, cudaStream_t stream) {
+cudaError_t launch_narrow(const CacheAttnParams& p, const CacheLaunch& how, cudaStream_t stream) {
   using Cfg = CacheCfg<D>;
   auto kern = omni_cache_attn_kernel<D, BF16>;
   static SmemAttrOnce attr_once[kMaxDevices];
   cudaError_t e = ensure_smem_attr(kern, Cfg::kSmem, attr_once);
   if (e != cudaSuccess) return e;
-  const long long rt = (p.G * static_cast<long long>(p.T) + kRows - 1) / kRows;
-  const long long most = static_cast<long long>(p.B) * p.Hkv * rt * ((p.capacity + kTileKeys - 1) / kTileKeys);
-  const int ctas = static_cast<int>(most < kMaxCtas ? most : kMaxCtas);
-  kern<<<ctas, kThreads, Cfg::kSmem, stream>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  omni_cache_join_kernel<D, BF16><<<static_cast<unsigned>(p.B * static_cast<long long>(p.Hkv) * rt), 128, 0, stream>>>(p, ctas);
+  kern<<<how.ctas, kThreads, Cfg::kSmem, stream>>>(p, how);
+  return cudaGetLastError();
+}
+
+template <int D, bool BF16>
+cudaError_t launch_t(const CacheAttnParams& p, cudaStream_t stream) {
+  const long long per = p.G * static_cast<long long>(p.T);
+  const Plan pl = make_plan(p.B, p.Hkv, per, D, p.prefix > 0, p.capacity);
+  CUtensorMap tmK, tmV;
+  if (pl.wide[0] || pl.wide[1]) {
+    cudaError_t e = make_page_maps(p, D, BF16, &tmK, &tmV);
+    if (e != cudaSuccess) return e;
+  }
+  for (int i = 0; i < 2; ++i) {
+    if (i == 1 && pl.of[0].own) break;
+    const cudaError_t e = pl.wide[i] ? launch_cache_wide(D, BF16, tmK, tmV, p, pl.of[i], stream) : launch_narrow<D, BF16>(p, pl.of[i], stream);
+    if (e != cudaSuccess) return e;
+  }
+  omni_cache_join_kernel<D, BF16><<<static_cast<unsigned>(p.B * static_cast<long long>(p.Hkv) * ((per + kRows - 1) / kRows)), 128, 0, stream>>>(
+      p, pl.of[0], pl.of[1]);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 long long cache_attn_workspace_bytes(int B, int H, int Hkv, int T, int head_dim, bool prefix) {
-  const long long per = static_cast<long long>(H / Hkv) * T;
-  long long shares = 2 * kMaxCtas;
-  if (prefix) shares += Hkv * ((B * per + kRows - 1) / kRows + B * ((per + kRows - 1) / kRows));
-  return shares * kRows * (head_dim + 2) * 4;
+  return make_plan(B, Hkv, static_cast<long long>(H / Hkv) * T, head_dim, prefix, 1 << 30).floats * 4;
 }
 
 cudaError_t launch_cache_attn(int head_dim, bool bf16, const CacheAttnParams& p, cudaStream_t stream) {

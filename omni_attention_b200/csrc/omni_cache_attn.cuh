@@ -1,5 +1,7 @@
 // Launch parameters of the attention over a paged key/value cache (omni_cache_attn.cu).
 #pragma once
+#include <cuda.h>
+
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -26,9 +28,27 @@ struct CacheAttnParams {
   int causal;
   float scale;                  // softmax scale
   float softcap;                // 0 = none
+  long long wait_cycles;        // cycle budget of one bounded wait
+};
+
+// One launch over some of the segments (omni_cache_line.cuh).
+struct CacheLaunch {
+  int rows, keys;               // of a tile
+  int ctas;
+  int prefix, own;              // which segments
+  long long share0;             // its shares in the workspace, in floats
 };
 
 cudaError_t launch_cache_attn(int head_dim, bool bf16, const CacheAttnParams& p, cudaStream_t stream);
 long long cache_attn_workspace_bytes(int B, int H, int Hkv, int T, int head_dim, bool prefix);
+
+// Tensor maps of k_pages and v_pages for it (omni_abi.cu).
+cudaError_t make_page_maps(const CacheAttnParams& p, int head_dim, bool bf16, CUtensorMap* tmK, CUtensorMap* tmV);
+
+// Tiles of 128 rows on the tcgen05 tensor cores (omni_cache_wide.cu). tmK, tmV: the pages as a matrix of rows, one box =
+// 64 columns of min(page_size, 128) tokens of one page and head.
+constexpr int kWideRows = 128, kWideKeys = 128, kWideCtas = 148;
+cudaError_t launch_cache_wide(int head_dim, bool bf16, const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p,
+                              const CacheLaunch& how, cudaStream_t stream);
 
 }  // namespace omni

@@ -1,0 +1,468 @@
+// Attention over a paged key/value cache for many query rows to a key/value head: an image's tokens, a draft, or all
+// sequences' rows on the prefix they share. The mathematics, the cut of the work and the shares are those of
+// omni_cache_attn.cu; a tile is 128 rows by 128 keys, on the tcgen05 tensor cores.
+//
+// Bound: at 128 rows the read of a tile (64 KB at head_dim 128) takes an SM about as long as the card's HBM rate gives it
+// (2 800 cycles), its two products 1 024; from 256 rows on the second row tile finds the keys in L2 and the chain scores ->
+// softmax -> P -> product bounds it. So the tiles of keys go to two softmax groups in turn, each with its own scores,
+// maximum, sum and O, and one group's chain runs under the other's products; at the end of a piece the groups' halves are
+// joined through shared memory.
+//
+// Roles of a CTA (one per SM, 320 threads):
+//   warps 0-3, 4-7  softmax groups: thread = query row = TMEM lane. They also gather the rows' queries into shared memory
+//                   (any strides, rows of one tile may belong to different sequences) and write the result.
+//   warp 8          TMA: K and V of each tile of keys page by page into a ring (lane = page of the tile)
+//   warp 9          one elected thread issues every tcgen05.mma
+// Hand-overs go through mbarriers; every wait is bounded as in the forward kernels. TMEM: S of the two groups (P, 16 bit,
+// over the first half of S), O of the two groups.
+//
+// Keys that are not there - behind the last token, in a page that does not exist - are never loaded; what the ring holds in
+// their places is zeroed in V (0 * NaN) and masked in S.
+#include "omni_cache_line.cuh"
+#include "omni_launch.h"
+
+namespace omni {
+
+namespace {
+
+constexpr int kWideThreads = 320;
+constexpr float kLazyLog2 = 8.f;
+constexpr long long kDrain = 4000000000LL;
+
+template <int D>
+struct WideCfg {
+  static constexpr int kTile = 128 * D * 2;
+  static constexpr int kChunks = D / 64;
+  static constexpr int kChunk = 128 * 128;
+  static constexpr int kSlots = D == 128 ? 6 : 10;   // K and V tiles in flight
+  static constexpr int kBars = (1 + kSlots) * kTile;
+  static constexpr int kSmem = kBars + 2560;         // barriers, row states
+};
+
+// Named barrier of the eight softmax warps.
+__device__ __forceinline__ void softmax_sync() { named_barrier_sync(1, 256); }
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y)
+               : "memory");
+}
+
+// The first n (may be below 0 or above 32) bits set.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+template <int COLS>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t addr, float (&f)[COLS]) {
+  if constexpr (COLS == 32) {
+    uint32_t r[32];
+    tmem_ld32(addr, r);
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(r[j]);
+  } else {
+    uint32_t r[16];
+    tmem_ld16(addr, r);
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(r[j]);
+  }
+}
+
+template <int D, bool BF16, bool SOFTCAP>
+__global__ void __launch_bounds__(kWideThreads, 1)
+omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                       const __grid_constant__ CacheAttnParams p, const __grid_constant__ CacheLaunch how, int d_real) {
+  using Cfg = WideCfg<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];   // what the 128-byte swizzle wants; there is no room to align by hand
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (p.status != nullptr && threadIdx.x == 0) atomicExch(p.status, kStatusWaitTimeout | (49 << 8));
+    return;
+  }
+  const uint32_t sQ = smem_u32(smem), sRing = sQ + Cfg::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBars);
+  const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * Cfg::kSlots;
+  const uint32_t bar_q = bar_empty + 8 * Cfg::kSlots;   // the rows' queries are in shared memory
+  const uint32_t bar_s = bar_q + 8;                     // [2] scores done
+  const uint32_t bar_p = bar_s + 16;                    // [2] P stored
+  const uint32_t bar_o = bar_p + 16;                    // [2] the group's last product of the piece done
+  const uint32_t bar_end = bar_o + 16;                  // drain of a launch that gives up
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kBars + 256);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_lim = reinterpret_cast<int*>(tmem_slot + 2);                                    // [8] largest limit of a warp's rows
+  uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + Cfg::kBars + 320);      // [kSlots] keys that are there
+  float* s_m = reinterpret_cast<float*>(smem + Cfg::kBars + 512);                         // [2][128]
+  float* s_l = s_m + 256;                                                                 // [2][128]
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < Cfg::kSlots; ++i) {
+      mbar_init(bar_full + 8 * i, 1);
+      mbar_init(bar_empty + 8 * i, 1);
+    }
+    mbar_init(bar_q, 256);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(bar_s + 8 * g, 1);
+      mbar_init(bar_p + 8 * g, 128);
+      mbar_init(bar_o + 8 * g, 1);
+    }
+    mbar_init(bar_end, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const long long limit = p.wait_cycles;
+  Walk walk(p, how);
+  Piece pc;
+
+  if (warp < 8) {
+    // =========================== softmax groups ===================================================
+    const int g = warp >> 2, r = tid & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + 128 * g + lanes, tO = tmem + 256 + D * g + lanes;
+    const float scale_log2 = p.scale * 1.4426950408889634f, inv_scale_log2 = 1.f / scale_log2;
+    const float cap_in = SOFTCAP ? p.scale / p.softcap : 0.f, cap_out = SOFTCAP ? p.softcap / p.scale : 0.f;
+    uint32_t n_vis = 0, n_pieces = 0;   // this group's visits and pieces with visits so far = phases of its barriers
+    uint32_t fill = 0;                  // ring entries of the pieces before this one
+    while (walk.next(p, pc)) {
+      const int n = pc.tile1 - pc.tile0;
+      // ---- the rows' queries: thread (row tid / 2, half of its chunks) ----
+      {
+        const int row = pc.rt * kWideRows + (tid >> 1);
+        const uint4* src = nullptr;
+        if (row < pc.rows) {
+          const RowId id = row_of(p, pc.prefix, pc.seg, row);
+          src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + id.b * p.qs_b +
+                                               (static_cast<long long>(pc.hk) * p.G + id.g) * p.qs_h + id.t * p.qs_t);
+        }
+        const int c0 = (tid & 1) * (D / 16);
+        uint4 v[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          v[i] = src != nullptr && (c0 + i) * 8 < d_real ? __ldg(src + c0 + i) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int c = c0 + i, rr = tid >> 1;
+          *reinterpret_cast<uint4*>(smem + (c >> 3) * Cfg::kChunk + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
+        }
+        fence_async_smem();
+        mbar_arrive(bar_q);
+      }
+      const int my_row = pc.rt * kWideRows + r;
+      RowId id{0, 0, 0};
+      int lim = 0;
+      if (my_row < pc.rows) {
+        id = row_of(p, pc.prefix, pc.seg, my_row);
+        lim = min(limit_of(p, id.b, id.t), pc.total);
+      }
+      const int warp_max = __reduce_max_sync(0xFFFFFFFFu, lim);
+      if (lane == 0) s_lim[warp] = warp_max;
+      named_barrier_sync(2 + g, 128);
+      int lim_max = s_lim[4 * g];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) lim_max = max(lim_max, s_lim[4 * g + w]);
+
+      RowState st{-INFINITY, 0.f};
+      int mine = 0;   // visits of this group in this piece
+      for (int i = g; i < n; i += 2, ++mine, ++n_vis) {
+        const uint32_t vs = (fill + 2 * i + 1) % Cfg::kSlots;   // V's place in the ring
+        const int key = pc.key0 + (pc.tile0 + i) * kWideKeys;
+        if (lane == 0) {
+          mbar_wait_lim(bar_s + 8 * g, n_vis & 1, abort_flag, p.status, 40 + g, limit);
+          mbar_wait_lim(bar_full + 8 * vs, ((fill + 2 * i + 1) / Cfg::kSlots) & 1, abort_flag, p.status, 42, limit);
+        }
+        __syncwarp();
+        tc_fence_after();
+        uint32_t valid[4], allow[4];
+        bool all = true, holes = false;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          valid[w] = *const_cast<volatile uint32_t*>(&s_valid[vs][w]) & low_bits(lim_max - key - 32 * w);
+          holes |= valid[w] != 0xFFFFFFFFu;
+          allow[w] = valid[w] & low_bits(lim - key - 32 * w);
+          all &= allow[w] == 0xFFFFFFFFu;
+        }
+        if (holes && !(valid[r >> 5] >> (r & 31) & 1u)) {   // key r of the tile: zero its V
+#pragma unroll
+          for (int c = 0; c < Cfg::kChunks; ++c) {
+            uint4* at = reinterpret_cast<uint4*>(smem + Cfg::kTile * (1 + vs) + c * Cfg::kChunk + r * 128);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) at[j] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+        }
+        const bool masked = !__all_sync(0xFFFFFFFFu, all);
+
+        float mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float s[64];
+          load_scores64(tS + 64 * h, s);
+          if constexpr (SOFTCAP) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) s[j] = cap_out * tanhf(s[j] * cap_in);
+          }
+          if (masked) apply_allow64(allow[2 * h], allow[2 * h + 1], s);
+          if constexpr (SOFTCAP) {
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(s[32 * c + j]);
+              tmem_st32(tS + 64 * h + 32 * c, w);
+            }
+          }
+          mx = fmaxf(mx, row_max64(s));
+        }
+        if constexpr (SOFTCAP) tc_wait_st();
+        const float alpha = softmax_update(st, mx, scale_log2, kLazyLog2);
+        if (mine > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.f)) rescale_o<D>(tO, alpha);
+        float sum = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float s[64];
+          uint32_t pk[32];
+          load_scores64(tS + 64 * h, s);
+          if (!SOFTCAP && masked) apply_allow64(allow[2 * h], allow[2 * h + 1], s);
+          sum += exp_and_pack_n<BF16, 0, 1, 64>(s, st.M, scale_log2, inv_scale_log2, pk);
+          tmem_st32(tS + 32 * h, pk);
+        }
+        st.l = st.l * alpha + sum;
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar_p + 8 * g);
+      }
+      fill += 2 * n;
+
+      // ---- the groups' halves of the piece: each takes half of the columns and gets the other's share of them ----
+      if (mine > 0) {
+        if (lane == 0) mbar_wait_lim(bar_o + 8 * g, n_pieces & 1, abort_flag, p.status, 44 + g, limit);
+        __syncwarp();
+        tc_fence_after();
+        ++n_pieces;
+      }
+      s_m[128 * g + r] = st.M;
+      s_l[128 * g + r] = st.l;
+      softmax_sync();   // (also: every score of the piece is read, its queries are not needed any more)
+      const float mo = s_m[128 * (1 - g) + r], lo = s_l[128 * (1 - g) + r];
+      const float top = fmaxf(st.M, mo), at = top == -INFINITY ? 0.f : top;
+      const float f = ex2_approx(st.M - at), fo = ex2_approx(mo - at);
+      const float sum = st.l * f + lo * fo;
+      constexpr int C = D / 4;   // columns of a round
+      float* xchg = reinterpret_cast<float*>(smem) + g * (C * 128);
+      const float* theirs = reinterpret_cast<const float*>(smem) + (1 - g) * (C * 128);
+      const bool any = !(sum == 0.f);   // NaN shows
+      const float inv = 1.f / sum;
+      const bool have_row = my_row < pc.rows;
+      const long long at_row = have_row ? out_row(p, id, pc.hk) : 0;
+      float* share = pc.share >= 0 ? share_at(p, how, pc.share, d_real) : nullptr;
+#pragma unroll
+      for (int round = 0; round < 2; ++round) {
+        float o[C];
+        const int give = (1 - g) * (D / 2) + round * C, keep = g * (D / 2) + round * C;
+        if (mine > 0) tmem_ld_cols<C>(tO + give, o);
+#pragma unroll
+        for (int j = 0; j < C; ++j) xchg[j * 128 + r] = mine > 0 ? o[j] * f : 0.f;
+        softmax_sync();
+        if (mine > 0) tmem_ld_cols<C>(tO + keep, o);
+#pragma unroll
+        for (int j = 0; j < C; ++j) o[j] = (mine > 0 ? o[j] * f : 0.f) + theirs[j * 128 + r];
+        softmax_sync();   // the next round, or the next piece's queries, go over what was read
+        if (have_row && keep < d_real) {
+          if (share != nullptr) {
+#pragma unroll
+            for (int j = 0; j < C; j += 4) {
+              *reinterpret_cast<float4*>(share + r * d_real + keep + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            }
+          } else {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at_row * d_real + keep);
+#pragma unroll
+            for (int j = 0; j < C / 8; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = any ? pack2<BF16>(o[8 * j + 2 * k] * inv, o[8 * j + 2 * k + 1] * inv) : 0u;
+              dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+      if (have_row && g == 0) {
+        if (share != nullptr) {
+          share[kWideRows * d_real + r] = top;
+          share[kWideRows * d_real + kWideRows + r] = sum;
+        } else if (p.lse != nullptr) {
+          p.lse[at_row] = any ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        }
+      }
+    }
+  } else if (warp == 8) {
+    // =========================== TMA ==============================================================
+    const int page_rows = 1 << p.page_shift;
+    const int box = page_rows < 128 ? page_rows : 128;   // tokens of a copy
+    const int pages = 128 / box;                         // copies of a tile and chunk
+    uint32_t fill = 0;
+    bool alive = true;
+    while (alive && walk.next(p, pc)) {
+      const int* table = p.page_table + pc.table_of * p.table_stride;
+      auto page_at = [&](int t) -> int {   // of this lane's part of tile t
+        const int key = pc.key0 + t * kWideKeys + lane * box;
+        return t < pc.tile1 && lane < pages && key < pc.total ? __ldg(table + (key >> p.page_shift)) : -1;
+      };
+      int next = page_at(pc.tile0);
+      for (int t = pc.tile0; alive && t < pc.tile1; ++t) {
+        const int page = next, key = pc.key0 + t * kWideKeys + lane * box;
+        next = page_at(t + 1);
+        const bool ok = page >= 0 && page < p.num_pages;
+        if (!ok && lane < pages && key < pc.total && p.status != nullptr) atomicCAS(p.status, 0, kStatusBadIndex);
+        const unsigned there = __ballot_sync(0xFFFFFFFFu, ok);
+        uint32_t word = 0;   // keys 32 * lane .. of the tile that are there (lanes 0-3)
+        if (lane < 4) {
+          if (box >= 32) {
+            word = there >> (32 * lane / box) & 1u ? 0xFFFFFFFFu : 0u;
+          } else {
+            word = (there >> (2 * lane) & 1u ? 0x0000FFFFu : 0u) | (there >> (2 * lane + 1) & 1u ? 0xFFFF0000u : 0u);
+          }
+        }
+        const int y = ok ? ((page * p.Hkv + pc.hk) << p.page_shift) + (key & (page_rows - 1)) : 0;
+        const uint32_t bytes = __popc(there) * box * 128 * Cfg::kChunks;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++fill) {
+          const uint32_t s = fill % Cfg::kSlots;
+          if (lane == 0 && fill >= Cfg::kSlots) {
+            alive = mbar_wait_lim(bar_empty + 8 * s, ((fill / Cfg::kSlots) - 1) & 1, abort_flag, p.status, 46, limit);
+          }
+          alive = __shfl_sync(0xFFFFFFFFu, alive, 0) && !*abort_flag;
+          alive = __all_sync(0xFFFFFFFFu, alive);
+          if (!alive) break;
+          if (kv == 1 && lane < 4) s_valid[s][lane] = word;
+          __syncwarp();
+          if (lane == 0) {
+            if (bytes > 0) {
+              mbar_expect_tx(bar_full + 8 * s, bytes);
+            } else {
+              mbar_arrive(bar_full + 8 * s);
+            }
+          }
+          __syncwarp();
+          if (ok) {
+#pragma unroll
+            for (int c = 0; c < Cfg::kChunks; ++c) {
+              tma_load_2d(sRing + s * Cfg::kTile + c * Cfg::kChunk + lane * box * 128, kv == 0 ? &tmK : &tmV, bar_full + 8 * s, c * 64, y);
+            }
+          }
+        }
+      }
+    }
+    if (*abort_flag && lane == 0) {   // giving up: nothing may still be on its way into shared memory at the end
+      for (uint32_t s = 0; s < Cfg::kSlots && s < fill; ++s) {
+        const uint32_t last = ((fill - 1 - s) / Cfg::kSlots) * Cfg::kSlots + s;
+        mbar_wait_drain(bar_full + 8 * s, (last / Cfg::kSlots) & 1, kDrain);
+      }
+    }
+    __syncwarp();
+  } else {
+    // =========================== MMA issuer =======================================================
+    if (elect_one()) {
+      constexpr int fmt = BF16 ? 1 : 0;
+      constexpr uint32_t idesc_qk = umma_idesc_f16(128, 128, fmt, 0), idesc_pv = umma_idesc_f16(128, D, fmt, 1);
+      constexpr uint32_t hi = umma_desc_hi_sw128(1024);
+      constexpr uint32_t kSlot = Cfg::kTile >> 4, kChunk = Cfg::kChunk >> 4;
+      const uint32_t q0 = umma_desc_lo(sQ, 16), k0 = umma_desc_lo(sRing, 16), v0 = umma_desc_lo(sRing, Cfg::kChunk);
+      uint32_t fill = 0, n_piece = 0, n_p[2] = {0, 0};
+      bool alive = true, issued = false;
+      while (alive && walk.next(p, pc)) {
+        const int n = pc.tile1 - pc.tile0;
+        alive = mbar_wait_lim(bar_q, n_piece & 1, abort_flag, p.status, 50, limit);
+        ++n_piece;
+        tc_fence_after();
+        auto scores = [&](int i) {   // S_g = Q K^T of visit i
+          const uint32_t f = fill + 2 * i, s = f % Cfg::kSlots;
+          alive = alive && mbar_wait_lim(bar_full + 8 * s, (f / Cfg::kSlots) & 1, abort_flag, p.status, 51, limit);
+          if (!alive) return;
+          tc_fence_after();
+          const uint32_t d = tmem + 128 * (i & 1), kd = k0 + s * kSlot;
+          umma_ss_lo<false>(d, q0, kd, hi, idesc_qk);
+#pragma unroll
+          for (int k = 1; k < D / 16; ++k) {
+            const uint32_t off = (k / 4) * kChunk + (k % 4) * 2;
+            umma_ss_lo<true>(d, q0 + off, kd + off, hi, idesc_qk);
+          }
+          tc_commit(bar_empty + 8 * s);
+          tc_commit(bar_s + 8 * (i & 1));
+          issued = true;
+        };
+        if (alive) scores(0);
+        if (alive && n > 1) scores(1);
+        for (int i = 0; alive && i < n; ++i) {
+          const int g = i & 1;
+          const uint32_t f = fill + 2 * i + 1, s = f % Cfg::kSlots;
+          alive = mbar_wait_lim(bar_p + 8 * g, (g == 0 ? n_p[0] : n_p[1]) & 1, abort_flag, p.status, 52 + g, limit) &&
+                  mbar_wait_lim(bar_full + 8 * s, (f / Cfg::kSlots) & 1, abort_flag, p.status, 54, limit);
+          if (!alive) break;
+          if (g == 0) {
+            ++n_p[0];
+          } else {
+            ++n_p[1];
+          }
+          tc_fence_after();
+          const uint32_t d = tmem + 256 + D * g, a = tmem + 128 * g, vd = v0 + s * kSlot;
+          umma_ts_lo(d, a, vd, hi, idesc_pv, i >= 2 ? 1u : 0u);
+#pragma unroll
+          for (int k = 1; k < 8; ++k) umma_ts_lo_acc(d, a + 8 * k, vd + k * 128, hi, idesc_pv);   // 16 keys = 2048 bytes
+          tc_commit(bar_empty + 8 * s);
+          if (i + 2 >= n) tc_commit(bar_o + 8 * g);
+          if (i + 2 < n) scores(i + 2);
+        }
+        fill += 2 * n;
+      }
+      if (*abort_flag && issued) {   // giving up: wait for the MMAs in flight
+        tc_commit(bar_end);
+        mbar_wait_drain(bar_end, 0, kDrain);
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+template <int D, bool BF16, bool SOFTCAP>
+cudaError_t launch_wide_t(const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p, const CacheLaunch& how, int d_real,
+                          cudaStream_t stream) {
+  auto kern = omni_cache_wide_kernel<D, BF16, SOFTCAP>;
+  static SmemAttrOnce attr_once[kMaxDevices];
+  const cudaError_t e = ensure_smem_attr(kern, WideCfg<D>::kSmem, attr_once);
+  if (e != cudaSuccess) return e;
+  kern<<<how.ctas, kWideThreads, WideCfg<D>::kSmem, stream>>>(tmK, tmV, p, how, d_real);
+  return cudaGetLastError();
+}
+
+template <int D, bool BF16>
+cudaError_t launch_wide_c(const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p, const CacheLaunch& how, int d_real,
+                          cudaStream_t stream) {
+  return p.softcap > 0.f ? launch_wide_t<D, BF16, true>(tmK, tmV, p, how, d_real, stream)
+                         : launch_wide_t<D, BF16, false>(tmK, tmV, p, how, d_real, stream);
+}
+
+}  // namespace
+
+// head_dim 32 is computed as 64: the TMA unit fills the missing columns with zeros.
+cudaError_t launch_cache_wide(int head_dim, bool bf16, const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p,
+                              const CacheLaunch& how, cudaStream_t stream) {
+  if (head_dim == 128) {
+    return bf16 ? launch_wide_c<128, true>(tmK, tmV, p, how, head_dim, stream) : launch_wide_c<128, false>(tmK, tmV, p, how, head_dim, stream);
+  }
+  return bf16 ? launch_wide_c<64, true>(tmK, tmV, p, how, head_dim, stream) : launch_wide_c<64, false>(tmK, tmV, p, how, head_dim, stream);
+}
+
+}  // namespace omni

@@ -34,6 +34,8 @@ cudaError_t launch_bwd(int head_dim, bool bf16, const CUtensorMap& tmQ, const CU
 
 // What omni_attn_last_cuda_error returns on this thread.
 void set_last_cuda_error(int code);
+// Cycle budget of a bounded wait (omni_attn_set_wait_cycles).
+long long wait_cycle_budget();
 
 // Sets a kernel's dynamic shared memory limit once per device (any host thread may be the first).
 struct SmemAttrOnce {

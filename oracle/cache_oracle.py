@@ -38,11 +38,12 @@ def slots(page_table, lengths, counts, T, page_size, num_pages):
 
 
 def attention(q, k_pages, v_pages, page_table, lengths, counts=None, causal=True, limits=None, scale=None, softcap=0.0):
-    """(out [B, H, T, D], lse [B, H, T]) in float64."""
+    """(out [B, H, T, D], lse [B, H, T], the same mean of |v| as out is of v) in float64."""
     B, H, T, D = q.shape
     P, Hkv, page, _ = k_pages.shape
     G, cap = H // Hkv, page_table.shape[1] * page
     out = torch.zeros(B, H, T, D, dtype=torch.float64)
+    size = torch.zeros(B, H, T, D, dtype=torch.float64)
     lse = torch.full((B, H, T), -math.inf, dtype=torch.float64)
     scale = D ** -0.5 if scale is None else scale
     for b in range(B):
@@ -68,5 +69,6 @@ def attention(q, k_pages, v_pages, page_table, lengths, counts=None, causal=True
                 if softcap > 0:
                     x = softcap * torch.tanh(x / softcap)
                 lse[b, h, t] = torch.logsumexp(x, 0)
-                out[b, h, t] = torch.softmax(x, 0) @ v
-    return out, lse
+                w = torch.softmax(x, 0)
+                out[b, h, t], size[b, h, t] = w @ v, w @ v.abs()
+    return out, lse, size
