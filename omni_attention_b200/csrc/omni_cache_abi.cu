@@ -269,6 +269,7 @@ int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* 
   p.scale = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(head_dim));
   p.softcap = softcap;
   p.wait_cycles = wait_cycle_budget();
+  if (!cache_attn_fits(p)) return OMNI_ERR_TOO_LONG;
   return ended(launch_cache_attn(head_dim, dtype == OMNI_DTYPE_BF16, p, static_cast<cudaStream_t>(cuda_stream)));
 }
 

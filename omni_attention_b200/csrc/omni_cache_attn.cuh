@@ -42,13 +42,36 @@ struct CacheLaunch {
 cudaError_t launch_cache_attn(int head_dim, bool bf16, const CacheAttnParams& p, cudaStream_t stream);
 long long cache_attn_workspace_bytes(int B, int H, int Hkv, int T, int head_dim, bool prefix);
 
-// Tensor maps of k_pages and v_pages for it (omni_abi.cu).
+// Tensor maps of k_pages and v_pages (omni_abi.cu): the pages as a matrix of rows, one box = 64 columns of
+// min(page_size, 128) tokens of one page and head.
 cudaError_t make_page_maps(const CacheAttnParams& p, int head_dim, bool bf16, CUtensorMap* tmK, CUtensorMap* tmV);
 
-// Tiles of 128 rows on the tcgen05 tensor cores (omni_cache_wide.cu). tmK, tmV: the pages as a matrix of rows, one box =
-// 64 columns of min(page_size, 128) tokens of one page and head.
-constexpr int kWideRows = 128, kWideKeys = 128, kWideCtas = 148;
+constexpr int kTileKeys = 128;     // of both kernels
+constexpr int kNarrowRows = 16, kWideRows = 128;
+constexpr int kCacheCtas = 148;    // one CTA per SM
+// Longest triples, in tiles of keys, that are left uncut. Cutting costs a second kernel over the shares.
+constexpr int kUncutTiles = 8;
+// Tiles of 128 rows on the tcgen05 tensor cores (omni_cache_wide.cu). `chained`: the launch may start before its
+// predecessor ends, and ends after it.
 cudaError_t launch_cache_wide(int head_dim, bool bf16, const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p,
-                              const CacheLaunch& how, cudaStream_t stream);
+                              const CacheLaunch& how, bool chained, cudaStream_t stream);
+// Whether the call's line of units can be counted in 31 bits.
+bool cache_attn_fits(const CacheAttnParams& p);
+
+// A launch with or without the attribute of a programmatic dependent launch.
+template <typename... P, typename... A>
+inline cudaError_t launch_chained(void (*kern)(P...), unsigned grid, int threads, int smem, bool chained, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = chained ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
 
 }  // namespace omni

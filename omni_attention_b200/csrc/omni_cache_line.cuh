@@ -30,32 +30,35 @@ __device__ __forceinline__ int limit_of(const CacheAttnParams& p, int b, int t) 
 
 struct Line {
   CacheLaunch how;
-  long long units;          // all of them
-  long long span;           // of one CTA
-  long long prefix_units;   // those of the prefix, which come first
+  unsigned units;           // all of them
+  unsigned span;            // of one CTA
+  unsigned prefix_units;    // those of the prefix, which come first
   int prefix_seq;           // the sequence whose page table the prefix is read through: the longest
   int prefix_end;
-  int tiles_prefix, rt_prefix, rt_own;
+  int rt_prefix, rt_own;
+  // Every triple is short (kUncutTiles tiles of keys at most): a triple is one unit, none is cut and nothing is joined.
+  bool uncut;
 
   __device__ __forceinline__ int tiles_between(int from, int to) const {
     return to > from ? (to - from + how.keys - 1) / how.keys : 1;   // a triple without keys still has rows to write
   }
-  __device__ __forceinline__ long long own_units(const CacheAttnParams& p, int b) const {
-    return how.own ? static_cast<long long>(p.Hkv) * rt_own * tiles_between(p.prefix, total_of(p, b)) : 0;
+  __device__ __forceinline__ unsigned units_between(int from, int to) const { return uncut ? 1u : tiles_between(from, to); }
+  __device__ __forceinline__ unsigned own_units(const CacheAttnParams& p, int b) const {
+    return how.own ? static_cast<unsigned>(p.Hkv) * rt_own * units_between(p.prefix, total_of(p, b)) : 0u;
   }
 };
 
-// All lanes of a warp; every CTA of every kernel comes to the same line.
+// All lanes of a warp; every CTA of every kernel comes to the same line. (The host refuses what would have 2^31 units.)
 __device__ __forceinline__ Line make_line(const CacheAttnParams& p, const CacheLaunch& how) {
   Line ln;
   ln.how = how;
   ln.rt_own = (p.G * p.T + how.rows - 1) / how.rows;
   const int lane = threadIdx.x & 31;
-  long long sum = 0;
+  unsigned sum = 0;
   int most = -1, seq = 0;
   for (int b = lane; b < p.B; b += 32) {
-    sum += ln.own_units(p, b);
     const int total = total_of(p, b);
+    sum += ln.tiles_between(p.prefix, total);
     if (total > most) {
       most = total;
       seq = b;
@@ -70,16 +73,16 @@ __device__ __forceinline__ Line make_line(const CacheAttnParams& p, const CacheL
       seq = s2;
     }
   }
-  ln.prefix_units = 0;
   ln.prefix_seq = seq;
   ln.prefix_end = min(p.prefix, most);
-  ln.tiles_prefix = ln.tiles_between(0, ln.prefix_end);
+  ln.uncut = (!how.own || most - p.prefix <= kUncutTiles * how.keys) && (!how.prefix || ln.prefix_end <= kUncutTiles * how.keys);
+  ln.prefix_units = 0;
   ln.rt_prefix = 0;
   if (how.prefix) {
-    ln.rt_prefix = static_cast<int>((static_cast<long long>(p.B) * p.G * p.T + how.rows - 1) / how.rows);
-    ln.prefix_units = static_cast<long long>(p.Hkv) * ln.rt_prefix * ln.tiles_prefix;
+    ln.rt_prefix = (p.B * p.G * p.T + how.rows - 1) / how.rows;
+    ln.prefix_units = static_cast<unsigned>(p.Hkv) * ln.rt_prefix * ln.units_between(0, ln.prefix_end);
   }
-  ln.units = sum + ln.prefix_units;
+  ln.units = ln.prefix_units + (how.own ? static_cast<unsigned>(p.Hkv) * ln.rt_own * (ln.uncut ? static_cast<unsigned>(p.B) : sum) : 0u);
   ln.span = (ln.units + how.ctas - 1) / how.ctas;
   return ln;
 }
@@ -96,7 +99,7 @@ struct Piece {
 // Walks over the pieces of one CTA. The constructor is for all lanes of a warp, next() for any thread by itself.
 struct Walk {
   Line ln;
-  long long u, u_end, base;
+  unsigned u, u_end, base;
   int seg;
 
   __device__ __forceinline__ Walk(const CacheAttnParams& p, const CacheLaunch& how) : ln(make_line(p, how)), base(0), seg(-1) {
@@ -107,11 +110,11 @@ struct Walk {
     const int lane = threadIdx.x & 31;
     for (int b0 = 0;; b0 += 32) {   // ends: u lies in some sequence's units
       const int b = b0 + lane;
-      const long long mine = b < p.B ? ln.own_units(p, b) : 0;
-      long long upto = mine;
+      const unsigned mine = b < p.B ? ln.own_units(p, b) : 0;
+      unsigned upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        const unsigned v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
         if (lane >= o) upto += v;
       }
       const unsigned past = __ballot_sync(0xFFFFFFFFu, base + upto > u);
@@ -129,30 +132,30 @@ struct Walk {
     if (u >= u_end) return false;
     pc.prefix = seg < 0;
     pc.seg = seg;
-    const int rts = pc.prefix ? ln.rt_prefix : ln.rt_own;
+    const unsigned rts = pc.prefix ? ln.rt_prefix : ln.rt_own;
     pc.table_of = pc.prefix ? ln.prefix_seq : seg;
     pc.key0 = pc.prefix ? 0 : p.prefix;
     pc.total = pc.prefix ? ln.prefix_end : total_of(p, seg);
     pc.rows = pc.prefix ? p.B * p.G * p.T : p.G * p.T;
-    const int tiles = pc.prefix ? ln.tiles_prefix : ln.tiles_between(pc.key0, pc.total);
-    const long long triple = (u - base) / tiles;
-    pc.tile0 = static_cast<int>(u - base - triple * tiles);
-    pc.tile1 = static_cast<int>(min(static_cast<long long>(tiles), pc.tile0 + (u_end - u)));
+    const unsigned units = ln.units_between(pc.key0, pc.total);
+    const unsigned triple = (u - base) / units, first = u - base - triple * units, n = min(units - first, u_end - u);
+    pc.whole = n == units;
+    pc.tile0 = static_cast<int>(first);
+    pc.tile1 = ln.uncut ? ln.tiles_between(pc.key0, pc.total) : static_cast<int>(first + n);
     pc.hk = static_cast<int>(triple / rts);
-    pc.rt = static_cast<int>(triple - static_cast<long long>(pc.hk) * rts);
-    pc.whole = pc.tile0 == 0 && pc.tile1 == tiles;
+    pc.rt = static_cast<int>(triple - pc.hk * rts);
     // CTA i has share 2 i (of a triple that began before its span) and 2 i + 1 (of one that begins in it and goes on after
     // it); with a prefix, triples inside one span have a share of their own behind those: the prefix's, then the sequences'.
     pc.share = -1;
     if (!pc.whole) {
-      pc.share = 2LL * blockIdx.x + (pc.tile0 == 0 ? 1 : 0);
+      pc.share = 2LL * blockIdx.x + (first == 0 ? 1 : 0);
     } else if (p.prefix > 0) {
       pc.share = 2LL * ln.how.ctas + triple;
       if (!pc.prefix) pc.share += static_cast<long long>(p.Hkv) * (ln.rt_prefix + static_cast<long long>(seg) * ln.rt_own);
     }
-    u += pc.tile1 - pc.tile0;
-    if (u - base >= static_cast<long long>(p.Hkv) * rts * tiles) {
-      base += static_cast<long long>(p.Hkv) * rts * tiles;
+    u += n;
+    if (u - base >= p.Hkv * rts * units) {
+      base += p.Hkv * rts * units;
       ++seg;
     }
     return true;
@@ -180,5 +183,103 @@ __device__ __forceinline__ RowId row_of(const CacheAttnParams& p, bool prefix, i
 __device__ __forceinline__ long long out_row(const CacheAttnParams& p, const RowId& id, int hk) {
   return (static_cast<long long>(id.b) * p.H + static_cast<long long>(hk) * p.G + id.g) * p.T + id.t;
 }
+
+// ---------------------------------------------------------------------------------------------------------------------
+// pieces of the two kernels
+// ---------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// x: element along head_dim (a multiple of 64), y: row of the matrix of pages.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y)
+               : "memory");
+}
+
+// Programmatic dependent launch: a kernel so launched may start before its predecessor has ended; what that one wrote is
+// there behind grid_wait. grid_go lets a successor start. Both are no-ops without such launches.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// The ring of K and V tiles (128 keys, [64 columns][128 rows][128 bytes], 128-byte swizzle) that a warp fills page by page.
+struct RingState {
+  uint32_t fill = 0;
+  bool alive = true;
+};
+template <int TILE, int CHUNKS, int SLOTS>
+struct Ring {
+  uint32_t data, full, empty;       // shared addresses
+  uint32_t (*valid)[4];             // [SLOTS]: of a V tile, which keys are there
+  volatile int* abort_flag;
+
+  // All lanes of the producing warp: tiles tile0 .. tile1 of a piece, K then V of each.
+  __device__ __forceinline__ void stream(const CacheAttnParams& p, const CUtensorMap* tmK, const CUtensorMap* tmV, const Piece& pc, int tile1,
+                                         RingState& st, int where) const {
+    const int lane = threadIdx.x & 31;
+    const int page_rows = 1 << p.page_shift;
+    const int box = page_rows < 128 ? page_rows : 128;   // tokens of a copy
+    const int pages = 128 / box;                         // copies of a tile and chunk: lane = copy
+    const int* table = p.page_table + pc.table_of * p.table_stride;
+    auto page_at = [&](int t) -> int {
+      const int key = pc.key0 + t * 128 + lane * box;
+      return t < tile1 && lane < pages && key < pc.total ? __ldg(table + (key >> p.page_shift)) : -1;
+    };
+    int next = page_at(pc.tile0);
+    for (int t = pc.tile0; st.alive && t < tile1; ++t) {
+      const int page = next, key = pc.key0 + t * 128 + lane * box;
+      next = page_at(t + 1);
+      const bool ok = page >= 0 && page < p.num_pages;
+      if (!ok && lane < pages && key < pc.total && p.status != nullptr) atomicCAS(p.status, 0, kStatusBadIndex);
+      const unsigned there = __ballot_sync(0xFFFFFFFFu, ok);
+      uint32_t word = 0;   // keys 32 * lane .. of the tile that are there (lanes 0-3)
+      if (lane < 4) {
+        if (box >= 32) {
+          word = there >> (32 * lane / box) & 1u ? 0xFFFFFFFFu : 0u;
+        } else {
+          word = (there >> (2 * lane) & 1u ? 0x0000FFFFu : 0u) | (there >> (2 * lane + 1) & 1u ? 0xFFFF0000u : 0u);
+        }
+      }
+      const int y = ok ? ((page * p.Hkv + pc.hk) << p.page_shift) + (key & (page_rows - 1)) : 0;
+      const uint32_t bytes = __popc(there) * box * 128 * CHUNKS;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv, ++st.fill) {
+        const uint32_t s = st.fill % SLOTS;
+        if (lane == 0 && st.fill >= SLOTS) {
+          st.alive = mbar_wait_lim(empty + 8 * s, ((st.fill / SLOTS) - 1) & 1, abort_flag, p.status, where, p.wait_cycles);
+        }
+        st.alive = __shfl_sync(0xFFFFFFFFu, st.alive, 0) && !*abort_flag;
+        st.alive = __all_sync(0xFFFFFFFFu, st.alive);
+        if (!st.alive) break;
+        if (kv == 1 && lane < 4) valid[s][lane] = word;
+        __syncwarp();
+        if (lane == 0) {
+          if (bytes > 0) {
+            mbar_expect_tx(full + 8 * s, bytes);
+          } else {
+            mbar_arrive(full + 8 * s);
+          }
+        }
+        __syncwarp();
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c) {
+            tma_load_2d(data + s * TILE + c * (128 * 128) + lane * box * 128, kv == 0 ? tmK : tmV, full + 8 * s, c * 64, y);
+          }
+        }
+      }
+    }
+  }
+
+  // A launch that gives up: nothing may still be on its way into shared memory when the CTA ends.
+  __device__ __forceinline__ void drain(const RingState& st) const {
+    if (*abort_flag && (threadIdx.x & 31) == 0) {
+      for (uint32_t s = 0; s < SLOTS && s < st.fill; ++s) {
+        const uint32_t last = ((st.fill - 1 - s) / SLOTS) * SLOTS + s;
+        mbar_wait_drain(full + 8 * s, (last / SLOTS) & 1, 4000000000LL);
+      }
+    }
+    __syncwarp();
+  }
+};
 
 }  // namespace omni

@@ -42,14 +42,6 @@ struct WideCfg {
 // Named barrier of the eight softmax warps.
 __device__ __forceinline__ void softmax_sync() { named_barrier_sync(1, 256); }
 
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y)
-               : "memory");
-}
-
 // The first n (may be below 0 or above 32) bits set.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
 
@@ -119,7 +111,9 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
   const long long limit = p.wait_cycles;
+  grid_go();
   Walk walk(p, how);
   Piece pc;
 
@@ -175,7 +169,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       int mine = 0;   // visits of this group in this piece
       for (int i = g; i < n; i += 2, ++mine, ++n_vis) {
         const uint32_t vs = (fill + 2 * i + 1) % Cfg::kSlots;   // V's place in the ring
-        const int key = pc.key0 + (pc.tile0 + i) * kWideKeys;
+        const int key = pc.key0 + (pc.tile0 + i) * kTileKeys;
         if (lane == 0) {
           mbar_wait_lim(bar_s + 8 * g, n_vis & 1, abort_flag, p.status, 40 + g, limit);
           mbar_wait_lim(bar_full + 8 * vs, ((fill + 2 * i + 1) / Cfg::kSlots) & 1, abort_flag, p.status, 42, limit);
@@ -306,69 +300,9 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     }
   } else if (warp == 8) {
     // =========================== TMA ==============================================================
-    const int page_rows = 1 << p.page_shift;
-    const int box = page_rows < 128 ? page_rows : 128;   // tokens of a copy
-    const int pages = 128 / box;                         // copies of a tile and chunk
-    uint32_t fill = 0;
-    bool alive = true;
-    while (alive && walk.next(p, pc)) {
-      const int* table = p.page_table + pc.table_of * p.table_stride;
-      auto page_at = [&](int t) -> int {   // of this lane's part of tile t
-        const int key = pc.key0 + t * kWideKeys + lane * box;
-        return t < pc.tile1 && lane < pages && key < pc.total ? __ldg(table + (key >> p.page_shift)) : -1;
-      };
-      int next = page_at(pc.tile0);
-      for (int t = pc.tile0; alive && t < pc.tile1; ++t) {
-        const int page = next, key = pc.key0 + t * kWideKeys + lane * box;
-        next = page_at(t + 1);
-        const bool ok = page >= 0 && page < p.num_pages;
-        if (!ok && lane < pages && key < pc.total && p.status != nullptr) atomicCAS(p.status, 0, kStatusBadIndex);
-        const unsigned there = __ballot_sync(0xFFFFFFFFu, ok);
-        uint32_t word = 0;   // keys 32 * lane .. of the tile that are there (lanes 0-3)
-        if (lane < 4) {
-          if (box >= 32) {
-            word = there >> (32 * lane / box) & 1u ? 0xFFFFFFFFu : 0u;
-          } else {
-            word = (there >> (2 * lane) & 1u ? 0x0000FFFFu : 0u) | (there >> (2 * lane + 1) & 1u ? 0xFFFF0000u : 0u);
-          }
-        }
-        const int y = ok ? ((page * p.Hkv + pc.hk) << p.page_shift) + (key & (page_rows - 1)) : 0;
-        const uint32_t bytes = __popc(there) * box * 128 * Cfg::kChunks;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++fill) {
-          const uint32_t s = fill % Cfg::kSlots;
-          if (lane == 0 && fill >= Cfg::kSlots) {
-            alive = mbar_wait_lim(bar_empty + 8 * s, ((fill / Cfg::kSlots) - 1) & 1, abort_flag, p.status, 46, limit);
-          }
-          alive = __shfl_sync(0xFFFFFFFFu, alive, 0) && !*abort_flag;
-          alive = __all_sync(0xFFFFFFFFu, alive);
-          if (!alive) break;
-          if (kv == 1 && lane < 4) s_valid[s][lane] = word;
-          __syncwarp();
-          if (lane == 0) {
-            if (bytes > 0) {
-              mbar_expect_tx(bar_full + 8 * s, bytes);
-            } else {
-              mbar_arrive(bar_full + 8 * s);
-            }
-          }
-          __syncwarp();
-          if (ok) {
-#pragma unroll
-            for (int c = 0; c < Cfg::kChunks; ++c) {
-              tma_load_2d(sRing + s * Cfg::kTile + c * Cfg::kChunk + lane * box * 128, kv == 0 ? &tmK : &tmV, bar_full + 8 * s, c * 64, y);
-            }
-          }
-        }
-      }
-    }
-    if (*abort_flag && lane == 0) {   // giving up: nothing may still be on its way into shared memory at the end
-      for (uint32_t s = 0; s < Cfg::kSlots && s < fill; ++s) {
-        const uint32_t last = ((fill - 1 - s) / Cfg::kSlots) * Cfg::kSlots + s;
-        mbar_wait_drain(bar_full + 8 * s, (last / Cfg::kSlots) & 1, kDrain);
-      }
-    }
-    __syncwarp();
+    RingState st;
+    while (st.alive && walk.next(p, pc)) ring.stream(p, &tmK, &tmV, pc, pc.tile1, st, 46);
+    ring.drain(st);
   } else {
     // =========================== MMA issuer =======================================================
     if (elect_one()) {
@@ -434,35 +368,35 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   tc_fence_before();
   __syncthreads();
   if (warp == 8) tmem_dealloc(tmem, 512);
+  grid_wait();   // a launch that was allowed to start early ends after its predecessor
 }
 
 template <int D, bool BF16, bool SOFTCAP>
 cudaError_t launch_wide_t(const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p, const CacheLaunch& how, int d_real,
-                          cudaStream_t stream) {
+                          bool chained, cudaStream_t stream) {
   auto kern = omni_cache_wide_kernel<D, BF16, SOFTCAP>;
   static SmemAttrOnce attr_once[kMaxDevices];
   const cudaError_t e = ensure_smem_attr(kern, WideCfg<D>::kSmem, attr_once);
   if (e != cudaSuccess) return e;
-  kern<<<how.ctas, kWideThreads, WideCfg<D>::kSmem, stream>>>(tmK, tmV, p, how, d_real);
-  return cudaGetLastError();
+  return launch_chained(kern, how.ctas, kWideThreads, WideCfg<D>::kSmem, chained, stream, tmK, tmV, p, how, d_real);
 }
 
 template <int D, bool BF16>
 cudaError_t launch_wide_c(const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p, const CacheLaunch& how, int d_real,
-                          cudaStream_t stream) {
-  return p.softcap > 0.f ? launch_wide_t<D, BF16, true>(tmK, tmV, p, how, d_real, stream)
-                         : launch_wide_t<D, BF16, false>(tmK, tmV, p, how, d_real, stream);
+                          bool chained, cudaStream_t stream) {
+  return p.softcap > 0.f ? launch_wide_t<D, BF16, true>(tmK, tmV, p, how, d_real, chained, stream)
+                         : launch_wide_t<D, BF16, false>(tmK, tmV, p, how, d_real, chained, stream);
 }
 
 }  // namespace
 
 // head_dim 32 is computed as 64: the TMA unit fills the missing columns with zeros.
 cudaError_t launch_cache_wide(int head_dim, bool bf16, const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p,
-                              const CacheLaunch& how, cudaStream_t stream) {
+                              const CacheLaunch& how, bool chained, cudaStream_t stream) {
   if (head_dim == 128) {
-    return bf16 ? launch_wide_c<128, true>(tmK, tmV, p, how, head_dim, stream) : launch_wide_c<128, false>(tmK, tmV, p, how, head_dim, stream);
+    return bf16 ? launch_wide_c<128, true>(tmK, tmV, p, how, head_dim, chained, stream) : launch_wide_c<128, false>(tmK, tmV, p, how, head_dim, chained, stream);
   }
-  return bf16 ? launch_wide_c<64, true>(tmK, tmV, p, how, head_dim, stream) : launch_wide_c<64, false>(tmK, tmV, p, how, head_dim, stream);
+  return bf16 ? launch_wide_c<64, true>(tmK, tmV, p, how, head_dim, chained, stream) : launch_wide_c<64, false>(tmK, tmV, p, how, head_dim, chained, stream);
 }
 
 }  // namespace omni
