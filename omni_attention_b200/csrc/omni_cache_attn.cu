@@ -27,27 +27,25 @@ namespace omni {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32 + 32;
-constexpr int kRows = kNarrowRows;
+constexpr int kThreads = kWarps * 32 + 64;
 
 template <int D>
 struct CacheCfg {
   static constexpr int kTile = 128 * D * 2;
   static constexpr int kChunks = D / 64;
   static constexpr int kSlots = D == 128 ? 6 : 10;
-  static constexpr int kRound = D / 4;                                       // columns of a round of the join
-  static constexpr int kJoin = kWarps * kRows * (kRound + 4) * 4;
-  static constexpr int kQ = kRows * D * 2;                                   // queries of a triple
+  static constexpr int kRound = D / 2;                                       // columns of a round of the join, 8 rows
+  static constexpr int kJoin = kWarps * 8 * (kRound + 8) * 4;                // (16 rows: half of the columns)
+  static constexpr int kQ = kNarrowRows * D * 2;                             // queries of a triple
   static constexpr int kSmem = kSlots * kTile + kJoin + 2 * kQ + 2560;       // + barriers, descriptions
 };
 
-// What the loading warp tells the others of a piece.
+// What the computing warps are told of a piece.
 struct PieceInfo {
-  int n, key0, rows, hk;      // tiles of keys, first key, rows of the tile, -1 in n: no more pieces
-  int lim_max, pad;
+  int n, key0, rows, lim_max;   // tiles of keys (-1: no more pieces), first key, rows, most keys that a row sees
   long long share;
-  int lim[kRows];             // keys that a row sees
-  long long out[kRows];       // where it is written
+  int lim[kNarrowRows];         // keys that a row sees
+  int out[kNarrowRows];         // where it is written
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
@@ -93,6 +91,12 @@ __device__ __forceinline__ float2 unpack16(uint32_t u) {
   }
 }
 
+// Transposes an 8 x 8 matrix of 16-bit values, two of a row to a thread.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
   const int bytes = ok ? 16 : 0;   // 0: the 16 bytes are filled with zeros, nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -126,12 +130,13 @@ __device__ __forceinline__ bool compute_vote(bool ok) {
   return all != 0;
 }
 
-template <int D, bool BF16>
+template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CacheAttnParams p,
                        const __grid_constant__ CacheLaunch how, int d_real) {
   using Cfg = CacheCfg<D>;
-  constexpr int KS = D / 16;        // steps of Q K^T
+  constexpr int KS = D / 16;        // steps of K Q^T, and 16-column tiles of O
+  constexpr int ROWS = 8 * NT;
   extern __shared__ __align__(1024) uint8_t smem[];   // what the 128-byte swizzle wants
   if ((smem_u32(smem) & 1023u) != 0) {
     if (p.status != nullptr && threadIdx.x == 0) atomicExch(p.status, kStatusWaitTimeout | (69 << 8));
@@ -148,7 +153,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(rest + 256);   // [kSlots]
   PieceInfo* info = reinterpret_cast<PieceInfo*>(rest + 512);             // [2]
   float* s_m = reinterpret_cast<float*>(rest + 1024);                     // [8][16]
-  float* s_l = s_m + kWarps * kRows;                                      // [8][16]
+  float* s_l = s_m + kWarps * kNarrowRows;                                // [8][16]
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
@@ -162,17 +167,26 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     }
     *abort_flag = 0;
     mbar_fence_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
   }
-  __syncthreads();
+  if (!how.late_wait) grid_wait();   // lengths, queries and pages may be the predecessor's work
   grid_go();
+  __syncthreads();
   const long long limit = p.wait_cycles;
 
   if (warp == kWarps) {
-    // =========================== loads ============================================================
+    // =========================== K and V ==========================================================
     const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
     Walk walk(p, how);
     Piece pc;
     RingState st;
+    while (st.alive && walk.next(p, pc)) ring.stream(p, &tmK, &tmV, pc, pc.tile1, st, 61);
+    ring.drain(st);
+  } else if (warp > kWarps) {
+    // =========================== queries and what is known of the rows ============================
+    Walk walk(p, how);
+    Piece pc;
     for (int piece = 0;; ++piece) {
       const int buf = piece & 1;
       if (piece >= 2) {
@@ -187,52 +201,46 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         mbar_arrive(bar_q + 8 * buf);
         break;
       }
-      // rows: lane = row
-      const int row = pc.rt * kRows + lane;
+      // lane = row
+      const int row = pc.rt * ROWS + lane;
       int lim = 0;
       const uint16_t* src = nullptr;
-      long long out = 0;
-      if (lane < kRows && row < pc.rows) {
+      if (lane < ROWS && row < pc.rows) {
         const RowId id = row_of(p, pc.prefix, pc.seg, row);
-        lim = min(limit_of(p, id.b, id.t), pc.total);
-        out = out_row(p, id, pc.hk);
         src = static_cast<const uint16_t*>(p.q) + id.b * p.qs_b + (static_cast<long long>(pc.hk) * p.G + id.g) * p.qs_h + id.t * p.qs_t;
+        lim = min(limit_of(p, id.b, id.t), pc.total);
+        to.out[lane] = static_cast<int>(out_row(p, id, pc.hk));
       }
-      const int lim_max = __reduce_max_sync(0xFFFFFFFFu, lim);
       constexpr int CH = D / 8;
 #pragma unroll
-      for (int i = 0; i < kRows * CH / 32; ++i) {
+      for (int i = 0; i < ROWS * CH / 32; ++i) {
         const int item = lane + 32 * i, r = item / CH, c = item % CH;
         const uint16_t* from = reinterpret_cast<const uint16_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(src), r));
         const bool ok = from != nullptr && c * 8 < d_real;
-        cp_async16(sQ + buf * Cfg::kQ + swizzled(r, c, kRows * 128), ok ? from + c * 8 : p.q, ok);
+        cp_async16(sQ + buf * Cfg::kQ + swizzled(r, c, ROWS * 128), ok ? static_cast<const void*>(from + c * 8) : p.q, ok);
       }
       cp_async_arrive(bar_q + 8 * buf);
-      // tiles of keys that no row sees are not read
-      const int first = pc.key0 + pc.tile0 * kTileKeys;
-      const int seen = lim_max > first ? (lim_max - first + kTileKeys - 1) / kTileKeys : 0;
-      const int n = min(pc.tile1 - pc.tile0, seen);
-      if (lane < kRows) {
-        to.lim[lane] = lim;
-        to.out[lane] = out;
-      }
+      const int lim_max = __reduce_max_sync(0xFFFFFFFFu, lim);
+      if (lane < ROWS) to.lim[lane] = lim;
       if (lane == 0) {
-        to.n = n;
-        to.key0 = first;
-        to.rows = min(kRows, pc.rows - pc.rt * kRows);
+        to.n = pc.tile1 - pc.tile0;
+        to.key0 = pc.key0 + pc.tile0 * kTileKeys;
+        to.rows = min(ROWS, pc.rows - pc.rt * ROWS);
         to.lim_max = lim_max;
         to.share = pc.share;
       }
       mbar_arrive(bar_q + 8 * buf);
-      ring.stream(p, &tmK, &tmV, pc, pc.tile0 + n, st, 61);
-      if (!st.alive) break;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    ring.drain(st);
   } else {
     // =========================== computation ======================================================
+    // S^T = K Q^T (16 keys x 8 rows a warp and product), O^T += V^T P^T (16 columns x 8 rows): the keys and columns fill the
+    // products' 16 rows, the query rows, which are few, their 8 columns. On this card a product of this kind takes about 16
+    // cycles of a quarter of an SM, and with the query rows as the 16 there were twice as many: 1 550 cycles a tile
+    // against 2 750 that the card's memory needs for it.
     const int quad = lane >> 2, pos = lane & 3;
     const float scale_log2 = p.scale * 1.4426950408889634f;
+    const float cap_in = p.softcap > 0.f ? p.scale / p.softcap : 0.f, cap_out = p.softcap * 1.4426950408889634f;
     uint32_t fill = 0;
     for (int piece = 0;; ++piece) {
       const int buf = piece & 1;
@@ -244,35 +252,68 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       const int n = in.n;
       if (n < 0) break;
       const int key0 = in.key0 + warp * 16, rows = in.rows, lim_max = in.lim_max;
-      const int lim[2] = {in.lim[quad], in.lim[quad + 8]};
-      int lim_min = min(quad < rows ? lim[0] : lim_max, quad + 8 < rows ? lim[1] : lim_max);
-      lim_min = __reduce_min_sync(0xFFFFFFFFu, lim_min);
-      uint32_t qf[KS][4];
+      // this thread's rows: 8 j + 2 pos + {0, 1}
+      int lim[2 * NT], lim_min = 0x7FFFFFFF;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        ldmatrix4(sQ + buf * Cfg::kQ + swizzled((lane & 7) + (((lane >> 3) & 1) << 3), 2 * k + (lane >> 4), kRows * 128), qf[k]);
+      for (int j = 0; j < 2 * NT; ++j) {
+        const int r = 8 * (j >> 1) + 2 * pos + (j & 1);
+        lim[j] = in.lim[r];
+        if (r < rows) lim_min = min(lim_min, lim[j]);
       }
-      float o_acc[D / 8][4];
+      lim_min = __reduce_min_sync(0xFFFFFFFFu, lim_min);
+      uint32_t qf[KS][2 * NT];   // Q^T, two steps to an ldmatrix for 8 rows, one for 16
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) o_acc[i][0] = o_acc[i][1] = o_acc[i][2] = o_acc[i][3] = 0.f;
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int k = 0; k < KS; k += 2 / NT) {
+        uint32_t b[4];
+        if constexpr (NT == 1) {
+          ldmatrix4(sQ + buf * Cfg::kQ + swizzled(lane & 7, 2 * k + (lane >> 3), ROWS * 128), b);
+          qf[k][0] = b[0];
+          qf[k][1] = b[1];
+          qf[k + 1][0] = b[2];
+          qf[k + 1][1] = b[3];
+        } else {
+          ldmatrix4(sQ + buf * Cfg::kQ + swizzled((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1), ROWS * 128), b);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qf[k][i] = b[i];
+        }
+      }
+      float o_acc[KS][NT][4];
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) o_acc[i][j][0] = o_acc[i][j][1] = o_acc[i][j][2] = o_acc[i][j][3] = 0.f;
+      }
+      float m[2 * NT], l[2 * NT];
+#pragma unroll
+      for (int j = 0; j < 2 * NT; ++j) {
+        m[j] = -INFINITY;
+        l[j] = 0.f;
+      }
 
       for (int t = 0; t < n; ++t, fill += 2) {
         const uint32_t ks = fill % Cfg::kSlots, vs = (fill + 1) % Cfg::kSlots;
         const int key = key0 + t * kTileKeys;
         if (lane == 0) mbar_wait_lim(bar_full + 8 * ks, (fill / Cfg::kSlots) & 1, abort_flag, p.status, 63, limit);
         __syncwarp();
-        float s[2][4];
+        float s[NT][4];   // [rows 8 j ..]: keys quad (0, 1) and quad + 8 (2, 3), rows 2 pos and 2 pos + 1
         if (key < lim_max) {   // else: nothing for this warp in the tile
           const uint32_t sk = sRing + ks * Cfg::kTile;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+          for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+          float s2[NT][4];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) s2[j][0] = s2[j][1] = s2[j][2] = s2[j][3] = 0.f;
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
-            uint32_t b[4];
-            ldmatrix4(sk + swizzled(warp * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1), 128 * 128), b);
-            mma16816<BF16>(s[0], qf[k], b[0], b[1]);
-            mma16816<BF16>(s[1], qf[k], b[2], b[3]);
+            uint32_t a[4];
+            ldmatrix4(sk + swizzled(warp * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), 2 * k + (lane >> 4), 128 * 128), a);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma16816<BF16>(k & 1 ? s2[j] : s[j], a, qf[k][2 * j], qf[k][2 * j + 1]);
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][e] += s2[j][e];
           }
         }
         __syncwarp();
@@ -295,112 +336,142 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             fence_async_smem();   // the ring's next copy goes over it
             __syncwarp();
           }
-          const bool masked = key + 16 > lim_min;
+          if (p.softcap > 0.f) {
+            float big = 0.f;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float x = s[j][e];
-              if (p.softcap > 0.f) {
-                x = tanhf(x * (p.scale / p.softcap)) * (p.softcap * 1.4426950408889634f);
-              } else {
-                x *= scale_log2;
+              for (int e = 0; e < 4; ++e) {
+                s[j][e] *= cap_in;
+                big = fmaxf(big, fabsf(s[j][e]));
               }
-              if (masked && key + 8 * j + 2 * pos + (e & 1) >= lim[e >> 1]) x = -INFINITY;
-              s[j][e] = x;
+            }
+            const bool small = !__any_sync(0xFFFFFFFFu, big > kTanhPolyLimit);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                float2 y = make_float2(s[j][e], s[j][e + 1]);
+                y = small ? tanh_small2(y) : make_float2(tanh_exact(y.x), tanh_exact(y.y));
+                s[j][e] = y.x * cap_out;
+                s[j][e + 1] = y.y * cap_out;
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[j][e] *= scale_log2;
+            }
+          }
+          if (key + 16 > lim_min) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (key + quad + 4 * (e & 2) >= lim[2 * j + (e & 1)]) s[j][e] = -INFINITY;
+              }
             }
           }
           // running maximum: moved only when it would grow by more than 8 (p <= 2^8 in 32 bits and in either 16-bit type)
           bool move = false;
-          float top[2];
+          float top[2 * NT];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float v = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
-            v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
-            v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
-            top[i] = v;
-            move |= v > m[i] + 8.f;
+          for (int j = 0; j < 2 * NT; ++j) top[j] = fmaxf(s[j >> 1][j & 1], s[j >> 1][2 + (j & 1)]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+#pragma unroll
+            for (int j = 0; j < 2 * NT; ++j) top[j] = fmaxf(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], o));
           }
+#pragma unroll
+          for (int j = 0; j < 2 * NT; ++j) move |= top[j] > m[j] + 8.f;
           if (__any_sync(0xFFFFFFFFu, move)) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float to = fmaxf(m[i], top[i]);
-              const float f = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - to);
-              m[i] = to;
-              l[i] *= f;
+            for (int j = 0; j < 2 * NT; ++j) {
+              const float to = fmaxf(m[j], top[j]);
+              const float f = m[j] == -INFINITY ? 0.f : ex2_approx(m[j] - to);
+              m[j] = to;
+              l[j] *= f;
 #pragma unroll
-              for (int d = 0; d < D / 8; ++d) {
-                o_acc[d][2 * i] *= f;
-                o_acc[d][2 * i + 1] *= f;
+              for (int d = 0; d < KS; ++d) {
+                o_acc[d][j >> 1][j & 1] *= f;
+                o_acc[d][j >> 1][2 + (j & 1)] *= f;
               }
             }
           }
-          uint32_t hi[4], lo[4];
+          uint32_t hi[NT][2], lo[NT][2];   // P^T: keys 0-7 and 8-15 of the warp's, turned so that a thread has two keys of a row
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float at = m[i] == -INFINITY ? 0.f : m[i];
+          for (int j = 0; j < NT; ++j) {
+            const float at0 = m[2 * j] == -INFINITY ? 0.f : m[2 * j], at1 = m[2 * j + 1] == -INFINITY ? 0.f : m[2 * j + 1];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float a = ex2_approx(s[j][2 * i] - at), b = ex2_approx(s[j][2 * i + 1] - at);
-              l[i] += a + b;
-              hi[2 * j + i] = pack16<BF16>(a, b);
-              const float2 h = unpack16<BF16>(hi[2 * j + i]);
-              lo[2 * j + i] = pack16<BF16>(a - h.x, b - h.y);
+            for (int h = 0; h < 2; ++h) {
+              const float a = ex2_approx(s[j][2 * h] - at0), b = ex2_approx(s[j][2 * h + 1] - at1);
+              l[2 * j] += a;
+              l[2 * j + 1] += b;
+              const uint32_t w = pack16<BF16>(a, b);
+              const float2 v = unpack16<BF16>(w);
+              hi[j][h] = movmatrix(w);
+              lo[j][h] = movmatrix(pack16<BF16>(a - v.x, b - v.y));
             }
           }
 #pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            uint32_t b[4];
-            ldmatrix4_trans(sv + swizzled(warp * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), 2 * d + (lane >> 4), 128 * 128), b);
-            mma16816<BF16>(o_acc[2 * d], hi, b[0], b[1]);
-            mma16816<BF16>(o_acc[2 * d + 1], hi, b[2], b[3]);
-            mma16816<BF16>(o_acc[2 * d], lo, b[0], b[1]);
-            mma16816<BF16>(o_acc[2 * d + 1], lo, b[2], b[3]);
+          for (int d = 0; d < KS; ++d) {
+            uint32_t a[4];   // V^T: 16 columns x 16 keys
+            ldmatrix4_trans(sv + swizzled(warp * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * d + ((lane >> 3) & 1), 128 * 128), a);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              mma16816<BF16>(o_acc[d][j], a, hi[j][0], hi[j][1]);
+              mma16816<BF16>(o_acc[d][j], a, lo[j][0], lo[j][1]);
+            }
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_empty + 8 * vs);
       }
 
-      // ---- the warps' shares of the piece, joined ----
+      // ---- the warps' shares of the piece, joined: kRound columns at a time ----
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
-        if (pos == 0) {
-          s_m[warp * kRows + quad + 8 * i] = m[i];
-          s_l[warp * kRows + quad + 8 * i] = l[i];
+      for (int j = 0; j < 2 * NT; ++j) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[j] += __shfl_xor_sync(0xFFFFFFFFu, l[j], o);
+        if (quad == 0) {
+          const int r = 8 * (j >> 1) + 2 * pos + (j & 1);
+          s_m[warp * kNarrowRows + r] = m[j];
+          s_l[warp * kNarrowRows + r] = l[j];
         }
       }
       const long long share = in.share;
-      const int r = threadIdx.x >> 4;                // the row this thread finishes, and which columns of a round
+      constexpr int C = Cfg::kRound / NT, TR = 256 / ROWS, V = C / TR;   // columns of a round, threads of a row, columns of a thread
+      constexpr int P = C + 4;                                           // pitch of a row
+      const int r = threadIdx.x / TR;                                    // the row this thread finishes
       const long long at_row = in.out[r];
       float f[kWarps], top = -INFINITY, sum = 0.f;
-      constexpr int C = Cfg::kRound, V = C / 16;     // columns of a round, of a thread
 #pragma unroll
-      for (int round = 0; round < 4; ++round) {
+      for (int round = 0; round < D / C; ++round) {
+        if (round * C >= d_real) break;
 #pragma unroll
-        for (int d = 0; d < C / 8; ++d) {
+        for (int d = 0; d < C / 16; ++d) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (quad + 8 * i < rows) {
-              *reinterpret_cast<float2*>(s_join + (warp * kRows + quad + 8 * i) * (C + 4) + 8 * d + 2 * pos) =
-                  make_float2(o_acc[round * (C / 8) + d][2 * i], o_acc[round * (C / 8) + d][2 * i + 1]);
+          for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int rr = 8 * j + 2 * pos + (e & 1);
+              if (rr < rows) s_join[(warp * ROWS + rr) * P + 16 * d + quad + 4 * (e & 2)] = o_acc[round * (C / 16) + d][j][e];
             }
           }
         }
         compute_sync();
         if (round == 0) {
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w * kRows + r]);
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w * kNarrowRows + r]);
           const float at = top == -INFINITY ? 0.f : top;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
-            f[w] = ex2_approx(s_m[w * kRows + r] - at);
-            sum += f[w] * s_l[w * kRows + r];
+            f[w] = ex2_approx(s_m[w * kNarrowRows + r] - at);
+            sum += f[w] * s_l[w * kNarrowRows + r];
           }
         }
-        const int col = round * C + (threadIdx.x & 15) * V;
+        const int in_round = (threadIdx.x % TR) * V, col = round * C + in_round;
         if (r < rows && col < d_real) {
           float acc[V];
 #pragma unroll
@@ -408,7 +479,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] += f[w] * s_join[(w * kRows + r) * (C + 4) + (threadIdx.x & 15) * V + i];
+            for (int i = 0; i < V; ++i) acc[i] += f[w] * s_join[(w * ROWS + r) * P + in_round + i];
           }
           if (share >= 0) {
             float* to = share_at(p, how, share, d_real) + r * d_real + col;
@@ -427,11 +498,11 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         }
         compute_sync();   // the next round goes over what was read
       }
-      if (r < rows && (threadIdx.x & 15) == 0) {
+      if (r < rows && threadIdx.x % TR == 0) {
         if (share >= 0) {
-          float* to = share_at(p, how, share, d_real) + kRows * d_real;
+          float* to = share_at(p, how, share, d_real) + how.rows * d_real;
           to[r] = top;
-          to[kRows + r] = sum;
+          to[how.rows + r] = sum;
         } else if (p.lse != nullptr) {
           p.lse[at_row] = !(sum == 0.f) ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
         }
@@ -441,40 +512,25 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     }
   }
   __syncthreads();
-  grid_wait();   // a launch that was allowed to start early ends after its predecessor
+  if (how.late_wait) grid_wait();
 }
 
-// Joins the shares of the rows that no single span covered. One CTA of 16 warps per (sequence, key/value head, 16 rows):
-// with fewer rows several warps take a row's shares in turn. `pre` is the launch that had the prefix (if there is one),
-// `own` the one that had the sequences' own keys; they may be the same launch.
+// Joins the shares of the rows that no single span covered, a warp per row. `pre` is the launch that had the prefix (if
+// there is one), `own` the one that had the sequences' own keys; they may be the same launch.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(512) omni_cache_join_kernel(const __grid_constant__ CacheAttnParams p, const __grid_constant__ CacheLaunch pre,
+__global__ void __launch_bounds__(256) omni_cache_join_kernel(const __grid_constant__ CacheAttnParams p, const __grid_constant__ CacheLaunch pre,
                                                               const __grid_constant__ CacheLaunch own) {
   constexpr int V = D / 32;   // columns of a lane
-  __shared__ float s_acc[16][D], s_top[16], s_sum[16];
-  const int rows = p.G * p.T;
-  const int groups = (rows + kRows - 1) / kRows;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int seq = static_cast<int>(blockIdx.x / (static_cast<unsigned>(p.Hkv) * groups));
-  const int in_seq = static_cast<int>(blockIdx.x - static_cast<unsigned>(seq) * p.Hkv * groups);
-  const int hk = in_seq / groups, group = in_seq % groups;
-
+  constexpr int AHEAD = 4;    // shares whose O is read before their maxima are known
+  const int lane = threadIdx.x & 31;
   const Line lo = make_line(p, own);
-  unsigned before = 0;
-  for (int b = lane; b < seq; b += 32) before += lo.own_units(p, b);
-  before = __reduce_add_sync(0xFFFFFFFFu, before);
-  const unsigned units = lo.units_between(p.prefix, total_of(p, seq));
-  const unsigned triple = static_cast<unsigned>(hk) * lo.rt_own + group * kRows / own.rows;
-  const unsigned first = lo.prefix_units + before + triple * units;
-  const unsigned c0 = first / lo.span, c1 = (first + units - 1) / lo.span;
-  if (p.prefix == 0 && c0 == c1) {   // written by the one CTA that had it
+  if (p.prefix == 0 && lo.uncut) {   // everything was written by the one CTA that had it
     grid_wait();
     return;
   }
-  Line lp = lo;
-  if (p.prefix > 0) {
-    lp = make_line(p, pre);
-    if (p.status != nullptr && in_seq == 0) {   // is the prefix in the same pages?
+  const Line lp = p.prefix > 0 ? make_line(p, pre) : lo;
+  if (p.prefix > 0 && p.status != nullptr) {   // is the prefix in the same pages?
+    for (int seq = blockIdx.x; seq < p.B; seq += gridDim.x) {
       const int pages = (min(p.prefix, total_of(p, seq)) + (1 << p.page_shift) - 1) >> p.page_shift;
       bool same = true;
       for (int i = threadIdx.x; i < pages; i += blockDim.x) {
@@ -483,126 +539,122 @@ __global__ void __launch_bounds__(512) omni_cache_join_kernel(const __grid_const
       if (!same) atomicCAS(p.status, 0, kStatusBadIndex);
     }
   }
-  // warps of a row, this warp's row and turn
-  const int here = min(kRows, rows - group * kRows);
-  const int shift = here > 8 ? 0 : here > 4 ? 1 : here > 2 ? 2 : here > 1 ? 3 : 4;
-  const int r = warp >> shift, part = warp & ((1 << shift) - 1);
-  const bool mine = r < here;
-  const int row = group * kRows + r;
+  const int rows = p.G * p.T;
+  const unsigned per_seq = static_cast<unsigned>(p.Hkv) * rows, all = per_seq * p.B;   // below 2^31
+  bool waited = false;
+  for (unsigned item = blockIdx.x * 8 + (threadIdx.x >> 5); item < all; item += gridDim.x * 8) {
+    const int seq = p.B == 1 ? 0 : static_cast<int>(item / per_seq);
+    const int in_seq = static_cast<int>(item - seq * per_seq), hk = in_seq / rows, row = in_seq - hk * rows;
+    unsigned before = 0;
+    for (int b = lane; b < seq; b += 32) before += lo.own_units(p, b);
+    before = __reduce_add_sync(0xFFFFFFFFu, before);
+    const unsigned units = lo.units_between(p.prefix, total_of(p, seq));
+    const unsigned triple = static_cast<unsigned>(hk) * lo.rt_own + row / own.rows;
+    const unsigned first = lo.prefix_units + before + triple * units;
+    const unsigned c0 = first / lo.span, n1 = (first + units - 1) / lo.span - c0 + 1;
+    if (p.prefix == 0 && n1 == 1) continue;   // written already
+    // the row's shares: n0 of the prefix, then n1 of its own keys
+    unsigned d0 = 0, n0 = 0, pt = 0;
+    int in0 = 0;
+    if (p.prefix > 0) {
+      const unsigned gr = static_cast<unsigned>(seq) * rows + row;   // the row in the prefix segment
+      pt = static_cast<unsigned>(hk) * lp.rt_prefix + gr / pre.rows;
+      in0 = static_cast<int>(gr % pre.rows);
+      const unsigned pu = lp.units_between(0, lp.prefix_end), f = pt * pu;
+      d0 = f / lp.span;
+      n0 = (f + pu - 1) / lp.span - d0 + 1;
+    }
+    const long long whole0 = 2LL * pre.ctas + pt;
+    const long long whole1 = 2LL * own.ctas + static_cast<long long>(p.Hkv) * (lo.rt_prefix + static_cast<long long>(seq) * lo.rt_own) + triple;
+    if (!waited) grid_wait();
+    waited = true;
 
-  // the row's shares: n0 of the prefix, then n1 of its own keys
-  unsigned d0 = 0, n0 = 0, pt = 0;
-  int in0 = 0;
-  if (p.prefix > 0) {
-    const unsigned gr = static_cast<unsigned>(seq) * rows + row;   // the row in the prefix segment
-    pt = static_cast<unsigned>(hk) * lp.rt_prefix + gr / pre.rows;
-    in0 = static_cast<int>(gr % pre.rows);
-    const unsigned pu = lp.units_between(0, lp.prefix_end), f = pt * pu;
-    d0 = f / lp.span;
-    n0 = (f + pu - 1) / lp.span - d0 + 1;
-  }
-  const unsigned n1 = c1 - c0 + 1;
-  const long long whole0 = 2LL * pre.ctas + pt;
-  const long long whole1 = 2LL * own.ctas + static_cast<long long>(p.Hkv) * (lo.rt_prefix + static_cast<long long>(seq) * lo.rt_own) + triple;
-  grid_wait();
-
-  float top = -INFINITY, sum = 0.f, acc[V];
+    float top = -INFINITY, sum = 0.f, acc[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  if (mine) {
-    for (unsigned j0 = part; j0 < n0 + n1; j0 += 32u << shift) {
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (unsigned j0 = 0; j0 < n0 + n1; j0 += 32) {
       // lane = share: maximum, sum and place of up to 32 of them at once
-      const unsigned j = j0 + (static_cast<unsigned>(lane) << shift);
+      const unsigned j = j0 + lane;
+      const int n = min(32, static_cast<int>(n0 + n1 - j0));
       float m2 = -INFINITY, l2 = 0.f;
       unsigned long long at = 0;
       if (j < n0 + n1) {
         const bool first_part = j < n0;
         const unsigned i = first_part ? j : j - n0;
-        const CacheLaunch& how = first_part ? pre : own;
+        const int tile_rows = first_part ? pre.rows : own.rows;
         const long long share = (first_part ? n0 : n1) == 1 ? (first_part ? whole0 : whole1) : 2LL * ((first_part ? d0 : c0) + i) + (i == 0 ? 1 : 0);
         const int in = first_part ? in0 : row % own.rows;
-        const float* from = share_at(p, how, share, D);
-        m2 = __ldcg(from + how.rows * D + in);
-        l2 = __ldcg(from + how.rows * D + how.rows + in);
+        const float* from = p.partial + (first_part ? pre.share0 : own.share0) + share * (tile_rows * (D + 2));
+        m2 = __ldcg(from + tile_rows * D + in);
+        l2 = __ldcg(from + tile_rows * D + tile_rows + in);
         at = reinterpret_cast<unsigned long long>(from + in * D);
+      }
+      auto read = [&](int i, float (&v)[V]) {
+        const float* from = reinterpret_cast<const float*>(__shfl_sync(0xFFFFFFFFu, at, i)) + lane * V;
+        if constexpr (V == 4) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(from));
+          v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        } else if constexpr (V == 2) {
+          const float2 x = __ldcg(reinterpret_cast<const float2*>(from));
+          v[0] = x.x, v[1] = x.y;
+        } else {
+          v[0] = __ldcg(from);
+        }
+      };
+      float early[AHEAD][V];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if (i < n) read(i, early[i]);
       }
       float to = fmaxf(top, m2);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xFFFFFFFFu, to, o));
       const float ref = to == -INFINITY ? 0.f : to;
       const float f1 = ex2_approx(top - ref), f2 = ex2_approx(m2 - ref);
-      float part_sum = l2 * f2;
+      float part = l2 * f2;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) part_sum += __shfl_xor_sync(0xFFFFFFFFu, part_sum, o);
-      sum = sum * f1 + part_sum;
+      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xFFFFFFFFu, part, o);
+      sum = sum * f1 + part;
       top = to;
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] *= f1;
-      const int n = min(32, static_cast<int>((n0 + n1 - j0 + (1u << shift) - 1) >> shift));
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float* from = reinterpret_cast<const float*>(__shfl_sync(0xFFFFFFFFu, at, i)) + lane * V;
-        const float f = __shfl_sync(0xFFFFFFFFu, f2, i);
-        if constexpr (V == 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(from));
-          acc[0] += f * v.x;
-          acc[1] += f * v.y;
-          acc[2] += f * v.z;
-          acc[3] += f * v.w;
-        } else if constexpr (V == 2) {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(from));
-          acc[0] += f * v.x;
-          acc[1] += f * v.y;
-        } else {
-          acc[0] += f * __ldcg(from);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if (i < n) {
+          const float f = __shfl_sync(0xFFFFFFFFu, f2, i);
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[k] += f * early[i][k];
         }
       }
-    }
-  }
-  if (shift > 0) {   // the warps of a row, in order
+#pragma unroll 4
+      for (int i = AHEAD; i < n; ++i) {
+        float v[V];
+        read(i, v);
+        const float f = __shfl_sync(0xFFFFFFFFu, f2, i);
 #pragma unroll
-    for (int i = 0; i < V; ++i) s_acc[warp][lane * V + i] = acc[i];
-    if (lane == 0) {
-      s_top[warp] = top;
-      s_sum[warp] = sum;
+        for (int k = 0; k < V; ++k) acc[k] += f * v[k];
+      }
     }
-    __syncthreads();
-    if (part != 0) return;
-    float to = top;
-    for (int w = 1; w < 1 << shift; ++w) to = fmaxf(to, s_top[warp + w]);
-    const float ref = to == -INFINITY ? 0.f : to;
-    const float f0 = ex2_approx(top - ref);
-    sum *= f0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] *= f0;
-    for (int w = 1; w < 1 << shift; ++w) {
-      const float f = ex2_approx(s_top[warp + w] - ref);
-      sum += f * s_sum[warp + w];
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] += f * s_acc[warp + w][lane * V + i];
+    const long long at_row = out_row(p, row_of(p, false, seq, row), hk);
+    const bool any = !(sum == 0.f);   // NaN shows
+    const float inv = 1.f / sum;
+    uint16_t* to = static_cast<uint16_t*>(p.out) + at_row * D + lane * V;
+    if constexpr (V == 4) {
+      *reinterpret_cast<uint2*>(to) = any ? make_uint2(pack16<BF16>(acc[0] * inv, acc[1] * inv), pack16<BF16>(acc[2] * inv, acc[3] * inv)) : make_uint2(0u, 0u);
+    } else if constexpr (V == 2) {
+      *reinterpret_cast<uint32_t*>(to) = any ? pack16<BF16>(acc[0] * inv, acc[1] * inv) : 0u;
+    } else {
+      *to = any ? static_cast<uint16_t>(pack16<BF16>(acc[0] * inv, 0.f)) : static_cast<uint16_t>(0);
     }
-    top = to;
+    if (p.lse != nullptr && lane == 0) p.lse[at_row] = any ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
   }
-  if (!mine) return;
-  const long long at_row = out_row(p, row_of(p, false, seq, row), hk);
-  const bool any = !(sum == 0.f);   // NaN shows
-  const float inv = 1.f / sum;
-  uint16_t* to = static_cast<uint16_t*>(p.out) + at_row * D + lane * V;
-  if constexpr (V == 4) {
-    *reinterpret_cast<uint2*>(to) = any ? make_uint2(pack16<BF16>(acc[0] * inv, acc[1] * inv), pack16<BF16>(acc[2] * inv, acc[3] * inv)) : make_uint2(0u, 0u);
-  } else if constexpr (V == 2) {
-    *reinterpret_cast<uint32_t*>(to) = any ? pack16<BF16>(acc[0] * inv, acc[1] * inv) : 0u;
-  } else {
-    *to = any ? static_cast<uint16_t>(pack16<BF16>(acc[0] * inv, 0.f)) : static_cast<uint16_t>(0);
-  }
-  if (p.lse != nullptr && lane == 0) p.lse[at_row] = any ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+  if (!waited) grid_wait();
 }
 
 // The launches of a call: one over everything, or one over the prefix and one over the sequences' own keys where only one
-// of the two has more than 16 rows to a key/value head (the 16-row tile would read its keys once for every 16 rows).
+// of the two has more than 16 rows to a key/value head (the narrow kernel would read its keys once for every 16 rows).
 struct Plan {
   CacheLaunch of[2];   // the prefix's, the sequences'; equal if one launch has both
-  bool wide[2];
   bool join;
   long long floats, units;
 };
@@ -610,57 +662,60 @@ struct Plan {
 Plan make_plan(int B, int Hkv, long long per, int head_dim, int prefix, long long capacity) {
   Plan pl{};
   const long long rows[2] = {B * per, per};
-  for (int i = 0; i < 2; ++i) pl.wide[i] = rows[i] > kRows;
-  if (prefix == 0) pl.wide[0] = pl.wide[1];
-  const bool one = prefix == 0 || pl.wide[0] == pl.wide[1];
+  auto tile = [](long long n) { return n > kNarrowRows ? kWideRows : n > 8 ? 16 : 8; };
+  const bool one = prefix == 0 || tile(rows[0]) == tile(rows[1]);
+  const long long tiles = (capacity + kTileKeys - 1) / kTileKeys;
   for (int i = 0; i < 2; ++i) {
     CacheLaunch& how = pl.of[i];
-    how.rows = pl.wide[i] ? kWideRows : kRows;
-    how.keys = kTileKeys;
-    how.prefix = prefix > 0 && (one || i == 0);
-    how.own = one || i == 1;
     if (i == 1 && one) {
       how = pl.of[0];
       break;
     }
-    long long triples = 0;
-    if (how.prefix) triples += Hkv * ((rows[0] + how.rows - 1) / how.rows);
-    if (how.own) triples += static_cast<long long>(B) * Hkv * ((rows[1] + how.rows - 1) / how.rows);
-    const long long most = triples * ((capacity + how.keys - 1) / how.keys);
+    how.prefix = prefix > 0 && (one || i == 0);
+    how.own = one || i == 1;
+    how.rows = tile(rows[how.own ? 1 : 0]);
+    how.uncut = prefix > 0 ? kUncutTilesPrefix : kUncutTiles;
+    how.late_wait = i;
+    how.rt_prefix = how.prefix ? static_cast<int>((rows[0] + how.rows - 1) / how.rows) : 0;
+    how.rt_own = static_cast<int>((rows[1] + how.rows - 1) / how.rows);
+    const long long triples = Hkv * (how.rt_prefix + (how.own ? static_cast<long long>(B) * how.rt_own : 0)), most = triples * tiles;
     pl.units += most;
     how.ctas = static_cast<int>(most < kCacheCtas ? most : kCacheCtas);
+    how.per_cta = static_cast<unsigned>((triples + how.ctas - 1) / how.ctas);
     how.share0 = pl.floats;
     pl.floats += (2LL * kCacheCtas + (prefix > 0 ? triples : 0)) * how.rows * (head_dim + 2);
+    pl.join = prefix > 0 || how.per_cta * tiles > 1 + kUncutTiles;   // else it is never cut
   }
-  pl.join = prefix > 0 || capacity > kUncutTiles * kTileKeys;
   return pl;
 }
 
-template <int D, bool BF16>
-cudaError_t launch_narrow(const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p, const CacheLaunch& how, int d_real, bool chained,
+template <int D, int NT, bool BF16>
+cudaError_t launch_narrow(const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p, const CacheLaunch& how, int d_real,
                           cudaStream_t stream) {
   using Cfg = CacheCfg<D>;
-  auto kern = omni_cache_attn_kernel<D, BF16>;
+  auto kern = omni_cache_attn_kernel<D, NT, BF16>;
   static SmemAttrOnce attr_once[kMaxDevices];
   const cudaError_t e = ensure_smem_attr(kern, Cfg::kSmem, attr_once);
   if (e != cudaSuccess) return e;
-  return launch_chained(kern, how.ctas, kThreads, Cfg::kSmem, chained, stream, tmK, tmV, p, how, d_real);
+  return launch_chained(kern, how.ctas, kThreads, Cfg::kSmem, stream, tmK, tmV, p, how, d_real);
 }
 
 template <int D, bool BF16>
 cudaError_t launch_t(const CacheAttnParams& p, cudaStream_t stream) {
-  const long long per = p.G * static_cast<long long>(p.T);
-  const Plan pl = make_plan(p.B, p.Hkv, per, D, p.prefix, p.capacity);
+  constexpr int C = D == 128 ? 128 : 64;   // head_dim 32 is computed as 64: the TMA unit fills the missing columns with zeros
+  const Plan pl = make_plan(p.B, p.Hkv, p.G * static_cast<long long>(p.T), D, p.prefix, p.capacity);
   CUtensorMap tmK, tmV;
   cudaError_t e = make_page_maps(p, D, BF16, &tmK, &tmV);
   for (int i = 0; e == cudaSuccess && i < 2; ++i) {
+    const CacheLaunch& how = pl.of[i];
     if (i == 1 && pl.of[0].own) break;
-    e = pl.wide[i] ? launch_cache_wide(D, BF16, tmK, tmV, p, pl.of[i], i == 1, stream)
-                   : launch_narrow<D == 128 ? 128 : 64, BF16>(tmK, tmV, p, pl.of[i], D, i == 1, stream);   // head_dim 32 as 64
+    e = how.rows == kWideRows ? launch_cache_wide(D, BF16, tmK, tmV, p, how, stream)
+        : how.rows == 16      ? launch_narrow<C, 2, BF16>(tmK, tmV, p, how, D, stream)
+                              : launch_narrow<C, 1, BF16>(tmK, tmV, p, how, D, stream);
   }
   if (e != cudaSuccess || !pl.join) return e;
-  const unsigned grid = static_cast<unsigned>(p.B * static_cast<long long>(p.Hkv) * ((per + kRows - 1) / kRows));
-  return launch_chained(omni_cache_join_kernel<D, BF16>, grid, 512, 0, true, stream, p, pl.of[0], pl.of[1]);
+  const long long ctas = (static_cast<long long>(p.B) * p.H * p.T + 7) / 8;
+  return launch_chained(omni_cache_join_kernel<D, BF16>, static_cast<unsigned>(ctas < 4 * kCacheCtas ? ctas : 4 * kCacheCtas), 256, 0, stream, p, pl.of[0], pl.of[1]);
 }
 
 }  // namespace

@@ -33,9 +33,13 @@ struct CacheAttnParams {
 
 // One launch over some of the segments (omni_cache_line.cuh).
 struct CacheLaunch {
-  int rows, keys;               // of a tile
+  int rows;                     // of a row tile
   int ctas;
   int prefix, own;              // which segments
+  int rt_prefix, rt_own;        // row tiles of the prefix (0 without it), of a sequence
+  unsigned per_cta;             // triples / ctas, rounded up
+  unsigned uncut;               // see Line::uncut
+  int late_wait;                // 0: waits for its predecessor before it reads anything; 1: only before it ends
   long long share0;             // its shares in the workspace, in floats
 };
 
@@ -47,20 +51,19 @@ long long cache_attn_workspace_bytes(int B, int H, int Hkv, int T, int head_dim,
 cudaError_t make_page_maps(const CacheAttnParams& p, int head_dim, bool bf16, CUtensorMap* tmK, CUtensorMap* tmV);
 
 constexpr int kTileKeys = 128;     // of both kernels
-constexpr int kNarrowRows = 16, kWideRows = 128;
+constexpr int kNarrowRows = 16, kWideRows = 128;   // most rows of the narrow kernel's tile: 8 or 16
 constexpr int kCacheCtas = 148;    // one CTA per SM
-// Longest triples, in tiles of keys, that are left uncut. Cutting costs a second kernel over the shares.
-constexpr int kUncutTiles = 8;
-// Tiles of 128 rows on the tcgen05 tensor cores (omni_cache_wide.cu). `chained`: the launch may start before its
-// predecessor ends, and ends after it.
+// What cutting costs, in tiles of keys: the shares' way through memory and the kernel that joins them.
+constexpr int kUncutTiles = 6, kUncutTilesPrefix = 1;   // with a prefix they are joined in any case
+// Tiles of 128 rows on the tcgen05 tensor cores (omni_cache_wide.cu).
 cudaError_t launch_cache_wide(int head_dim, bool bf16, const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p,
-                              const CacheLaunch& how, bool chained, cudaStream_t stream);
+                              const CacheLaunch& how, cudaStream_t stream);
 // Whether the call's line of units can be counted in 31 bits.
 bool cache_attn_fits(const CacheAttnParams& p);
 
-// A launch with or without the attribute of a programmatic dependent launch.
+// A programmatic dependent launch: may start before its predecessor on the stream has ended (omni_cache_line.cuh: grid_wait).
 template <typename... P, typename... A>
-inline cudaError_t launch_chained(void (*kern)(P...), unsigned grid, int threads, int smem, bool chained, cudaStream_t stream, A&&... args) {
+inline cudaError_t launch_chained(void (*kern)(P...), unsigned grid, int threads, int smem, cudaStream_t stream, A&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
@@ -70,7 +73,7 @@ inline cudaError_t launch_chained(void (*kern)(P...), unsigned grid, int threads
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = chained ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 

@@ -13,10 +13,11 @@ namespace omni {
 __device__ __forceinline__ int count_of(const CacheAttnParams& p, int b) {
   return p.counts == nullptr ? p.T : min(max(__ldg(p.counts + b), 0), p.T);
 }
-// tokens of sequence b that exist once this call's are in: [0, capacity]
+// tokens of sequence b that exist once this call's are in: [0, capacity]; 0 for a sequence without new tokens (nobody asks)
 __device__ __forceinline__ int total_of(const CacheAttnParams& p, int b) {
-  const long long n = static_cast<long long>(max(__ldg(p.lengths + b), 0)) + count_of(p, b);
-  return static_cast<int>(n < p.capacity ? n : p.capacity);
+  const int c = count_of(p, b);
+  const unsigned n = static_cast<unsigned>(max(__ldg(p.lengths + b), 0)) + c;
+  return c == 0 ? 0 : static_cast<int>(min(n, static_cast<unsigned>(p.capacity)));
 }
 // keys row (b, t) sees
 __device__ __forceinline__ int limit_of(const CacheAttnParams& p, int b, int t) {
@@ -24,8 +25,7 @@ __device__ __forceinline__ int limit_of(const CacheAttnParams& p, int b, int t) 
   const int total = total_of(p, b);
   if (p.limits != nullptr) return min(max(__ldg(p.limits + static_cast<long long>(b) * p.T + t), 0), total);
   if (!p.causal) return total;
-  const long long n = static_cast<long long>(max(__ldg(p.lengths + b), 0)) + t + 1;
-  return static_cast<int>(n < total ? n : total);
+  return static_cast<int>(min(static_cast<unsigned>(max(__ldg(p.lengths + b), 0)) + t + 1, static_cast<unsigned>(total)));
 }
 
 struct Line {
@@ -36,11 +36,12 @@ struct Line {
   int prefix_seq;           // the sequence whose page table the prefix is read through: the longest
   int prefix_end;
   int rt_prefix, rt_own;
-  // Every triple is short (kUncutTiles tiles of keys at most): a triple is one unit, none is cut and nothing is joined.
+  // A triple is one unit, none is cut and nothing has to be joined: where the CTA with most to do then has at most how.uncut
+  // tiles of keys more than an even cut would give it.
   bool uncut;
 
   __device__ __forceinline__ int tiles_between(int from, int to) const {
-    return to > from ? (to - from + how.keys - 1) / how.keys : 1;   // a triple without keys still has rows to write
+    return to > from ? (to - from + kTileKeys - 1) / kTileKeys : 1;   // a triple without keys still has rows to write
   }
   __device__ __forceinline__ unsigned units_between(int from, int to) const { return uncut ? 1u : tiles_between(from, to); }
   __device__ __forceinline__ unsigned own_units(const CacheAttnParams& p, int b) const {
@@ -52,7 +53,7 @@ struct Line {
 __device__ __forceinline__ Line make_line(const CacheAttnParams& p, const CacheLaunch& how) {
   Line ln;
   ln.how = how;
-  ln.rt_own = (p.G * p.T + how.rows - 1) / how.rows;
+  ln.rt_own = how.rt_own;
   const int lane = threadIdx.x & 31;
   unsigned sum = 0;
   int most = -1, seq = 0;
@@ -64,26 +65,21 @@ __device__ __forceinline__ Line make_line(const CacheAttnParams& p, const CacheL
       seq = b;
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    const int m2 = __shfl_xor_sync(0xFFFFFFFFu, most, o), s2 = __shfl_xor_sync(0xFFFFFFFFu, seq, o);
-    if (m2 > most || (m2 == most && s2 < seq)) {
-      most = m2;
-      seq = s2;
-    }
-  }
+  sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+  const int most_of_all = __reduce_max_sync(0xFFFFFFFFu, most);
+  seq = __reduce_min_sync(0xFFFFFFFFu, most == most_of_all ? seq : 0x7FFFFFFF);
+  most = most_of_all;
   ln.prefix_seq = seq;
   ln.prefix_end = min(p.prefix, most);
-  ln.uncut = (!how.own || most - p.prefix <= kUncutTiles * how.keys) && (!how.prefix || ln.prefix_end <= kUncutTiles * how.keys);
-  ln.prefix_units = 0;
-  ln.rt_prefix = 0;
-  if (how.prefix) {
-    ln.rt_prefix = (p.B * p.G * p.T + how.rows - 1) / how.rows;
-    ln.prefix_units = static_cast<unsigned>(p.Hkv) * ln.rt_prefix * ln.units_between(0, ln.prefix_end);
-  }
-  ln.units = ln.prefix_units + (how.own ? static_cast<unsigned>(p.Hkv) * ln.rt_own * (ln.uncut ? static_cast<unsigned>(p.B) : sum) : 0u);
-  ln.span = (ln.units + how.ctas - 1) / how.ctas;
+  ln.rt_prefix = how.rt_prefix;
+  const unsigned tiles_prefix = how.prefix ? ln.tiles_between(0, ln.prefix_end) : 0u, tiles_own = how.own ? ln.tiles_between(p.prefix, most) : 0u;
+  const unsigned heads = p.Hkv, rt_own = how.own ? ln.rt_own : 0;
+  const unsigned cut_units = heads * (ln.rt_prefix * tiles_prefix + rt_own * sum), cut_span = (cut_units + how.ctas - 1) / how.ctas;
+  const unsigned triples = heads * (ln.rt_prefix + rt_own * p.B), per_cta = how.per_cta;
+  ln.uncut = static_cast<unsigned long long>(per_cta) * max(tiles_prefix, tiles_own) <= cut_span + how.uncut;
+  ln.prefix_units = how.prefix ? heads * ln.rt_prefix * ln.units_between(0, ln.prefix_end) : 0u;
+  ln.units = ln.uncut ? triples : cut_units;
+  ln.span = ln.uncut ? per_cta : cut_span;
   return ln;
 }
 
@@ -106,6 +102,11 @@ struct Walk {
     u = ln.span * blockIdx.x;
     u_end = min(u + ln.span, ln.units);
     if (u >= u_end || u < ln.prefix_units) return;
+    if (p.B == 1) {
+      base = ln.prefix_units;
+      seg = 0;
+      return;
+    }
     base = ln.prefix_units;
     const int lane = threadIdx.x & 31;
     for (int b0 = 0;; b0 += 32) {   // ends: u lies in some sequence's units
@@ -142,7 +143,7 @@ struct Walk {
     pc.whole = n == units;
     pc.tile0 = static_cast<int>(first);
     pc.tile1 = ln.uncut ? ln.tiles_between(pc.key0, pc.total) : static_cast<int>(first + n);
-    pc.hk = static_cast<int>(triple / rts);
+    pc.hk = static_cast<int>(rts == 1 ? triple : triple / rts);
     pc.rt = static_cast<int>(triple - pc.hk * rts);
     // CTA i has share 2 i (of a triple that began before its span) and 2 i + 1 (of one that begins in it and goes on after
     // it); with a prefix, triples inside one span have a share of their own behind those: the prefix's, then the sequences'.
@@ -176,7 +177,7 @@ __device__ __forceinline__ RowId row_of(const CacheAttnParams& p, bool prefix, i
   const int per = p.G * p.T;
   id.b = prefix ? r / per : b;
   const int in = prefix ? r - id.b * per : r;
-  id.t = in / p.G;
+  id.t = p.T == 1 ? 0 : p.G == 1 ? in : in / p.G;
   id.g = in - id.t * p.G;
   return id;
 }

@@ -36,7 +36,7 @@ struct WideCfg {
   static constexpr int kChunk = 128 * 128;
   static constexpr int kSlots = D == 128 ? 6 : 10;   // K and V tiles in flight
   static constexpr int kBars = (1 + kSlots) * kTile;
-  static constexpr int kSmem = kBars + 2560;         // barriers, row states
+  static constexpr int kSmem = kBars + 3072;         // barriers, row states
 };
 
 // Named barrier of the eight softmax warps.
@@ -82,10 +82,11 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   const uint32_t bar_end = bar_o + 16;                  // drain of a launch that gives up
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kBars + 256);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* s_lim = reinterpret_cast<int*>(tmem_slot + 2);                                    // [8] largest limit of a warp's rows
-  uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + Cfg::kBars + 320);      // [kSlots] keys that are there
+  int* s_lim = reinterpret_cast<int*>(tmem_slot + 2);                                    // [8] largest limit of a warp's rows, [8] smallest
+  uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + Cfg::kBars + 336);      // [kSlots] keys that are there
   float* s_m = reinterpret_cast<float*>(smem + Cfg::kBars + 512);                         // [2][128]
   float* s_l = s_m + 256;                                                                 // [2][128]
+  int* s_out = reinterpret_cast<int*>(s_l + 256);                                         // [128] where a row is written
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -102,6 +103,8 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     mbar_init(bar_end, 1);
     *abort_flag = 0;
     mbar_fence_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
   }
   if (warp == 8) {
     tmem_alloc(smem_u32(tmem_slot), 512);
@@ -113,6 +116,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   const uint32_t tmem = *tmem_slot;
   const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
   const long long limit = p.wait_cycles;
+  if (!how.late_wait) grid_wait();   // lengths, queries and pages may be the predecessor's work
   grid_go();
   Walk walk(p, how);
   Piece pc;
@@ -151,19 +155,25 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         fence_async_smem();
         mbar_arrive(bar_q);
       }
-      const int my_row = pc.rt * kWideRows + r;
-      RowId id{0, 0, 0};
+      const int my_row = pc.rt * kWideRows + r, rows = min(kWideRows, pc.rows - pc.rt * kWideRows);
       int lim = 0;
-      if (my_row < pc.rows) {
-        id = row_of(p, pc.prefix, pc.seg, my_row);
+      if (r < rows) {
+        const RowId id = row_of(p, pc.prefix, pc.seg, my_row);
         lim = min(limit_of(p, id.b, id.t), pc.total);
+        if (g == 0) s_out[r] = static_cast<int>(out_row(p, id, pc.hk));
       }
-      const int warp_max = __reduce_max_sync(0xFFFFFFFFu, lim);
-      if (lane == 0) s_lim[warp] = warp_max;
+      const int warp_max = __reduce_max_sync(0xFFFFFFFFu, lim), warp_min = __reduce_min_sync(0xFFFFFFFFu, r < rows ? lim : 0x7FFFFFFF);
+      if (lane == 0) {
+        s_lim[warp] = warp_max;
+        s_lim[8 + warp] = warp_min;
+      }
       named_barrier_sync(2 + g, 128);
-      int lim_max = s_lim[4 * g];
+      int lim_max = s_lim[4 * g], lim_min = s_lim[8 + 4 * g];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) lim_max = max(lim_max, s_lim[4 * g + w]);
+      for (int w = 1; w < 4; ++w) {
+        lim_max = max(lim_max, s_lim[4 * g + w]);
+        lim_min = min(lim_min, s_lim[8 + 4 * g + w]);
+      }
 
       RowState st{-INFINITY, 0.f};
       int mine = 0;   // visits of this group in this piece
@@ -176,25 +186,27 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         }
         __syncwarp();
         tc_fence_after();
-        uint32_t valid[4], allow[4];
-        bool all = true, holes = false;
+        // Masks only where a row's limit falls into the tile or a page of it is not there.
+        uint32_t allow[4];
+        const uint4 there = *const_cast<const uint4*>(reinterpret_cast<volatile uint4*>(&s_valid[vs][0])) ;
+        const bool masked = key + kTileKeys > lim_min || (there.x & there.y & there.z & there.w) != 0xFFFFFFFFu;
+        if (masked) {
+          const uint32_t valid[4] = {there.x & low_bits(lim_max - key), there.y & low_bits(lim_max - key - 32),
+                                     there.z & low_bits(lim_max - key - 64), there.w & low_bits(lim_max - key - 96)};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          valid[w] = *const_cast<volatile uint32_t*>(&s_valid[vs][w]) & low_bits(lim_max - key - 32 * w);
-          holes |= valid[w] != 0xFFFFFFFFu;
-          allow[w] = valid[w] & low_bits(lim - key - 32 * w);
-          all &= allow[w] == 0xFFFFFFFFu;
-        }
-        if (holes && !(valid[r >> 5] >> (r & 31) & 1u)) {   // key r of the tile: zero its V
+          for (int w = 0; w < 4; ++w) allow[w] = valid[w] & low_bits(lim - key - 32 * w);
+          const int quarter = warp & 3;   // key r of the tile is in word r / 32
+          const uint32_t word = quarter == 0 ? valid[0] : quarter == 1 ? valid[1] : quarter == 2 ? valid[2] : valid[3];
+          if (!(word >> lane & 1u)) {     // not there, or no row sees it: zero its V
 #pragma unroll
-          for (int c = 0; c < Cfg::kChunks; ++c) {
-            uint4* at = reinterpret_cast<uint4*>(smem + Cfg::kTile * (1 + vs) + c * Cfg::kChunk + r * 128);
+            for (int c = 0; c < Cfg::kChunks; ++c) {
+              uint4* at = reinterpret_cast<uint4*>(smem + Cfg::kTile * (1 + vs) + c * Cfg::kChunk + r * 128);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) at[j] = make_uint4(0u, 0u, 0u, 0u);
+              for (int j = 0; j < 8; ++j) at[j] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async_smem();
           }
-          fence_async_smem();
         }
-        const bool masked = !__all_sync(0xFFFFFFFFu, all);
 
         float mx = -INFINITY;
 #pragma unroll
@@ -237,7 +249,8 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       }
       fill += 2 * n;
 
-      // ---- the groups' halves of the piece: each takes half of the columns and gets the other's share of them ----
+      // ---- the groups' halves of the piece, added up in shared memory 32 (head_dim 64: 16) columns at a time and written
+      // out row by row, so that a warp's stores are whole lines ----
       if (mine > 0) {
         if (lane == 0) mbar_wait_lim(bar_o + 8 * g, n_pieces & 1, abort_flag, p.status, 44 + g, limit);
         __syncwarp();
@@ -249,52 +262,47 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       softmax_sync();   // (also: every score of the piece is read, its queries are not needed any more)
       const float mo = s_m[128 * (1 - g) + r], lo = s_l[128 * (1 - g) + r];
       const float top = fmaxf(st.M, mo), at = top == -INFINITY ? 0.f : top;
-      const float f = ex2_approx(st.M - at), fo = ex2_approx(mo - at);
-      const float sum = st.l * f + lo * fo;
-      constexpr int C = D / 4;   // columns of a round
-      float* xchg = reinterpret_cast<float*>(smem) + g * (C * 128);
-      const float* theirs = reinterpret_cast<const float*>(smem) + (1 - g) * (C * 128);
+      float f = ex2_approx(st.M - at);
+      const float sum = st.l * f + lo * ex2_approx(mo - at);
       const bool any = !(sum == 0.f);   // NaN shows
-      const float inv = 1.f / sum;
-      const bool have_row = my_row < pc.rows;
-      const long long at_row = have_row ? out_row(p, id, pc.hk) : 0;
       float* share = pc.share >= 0 ? share_at(p, how, pc.share, d_real) : nullptr;
+      if (share == nullptr) f *= 1.f / sum;
+      const bool have = mine > 0 && any;
+      constexpr int C = D / 4, Q4 = C / 4;   // columns of a round, 16-byte pieces of a row
+      float4* xchg = reinterpret_cast<float4*>(smem);   // [2][128][Q4], pieces of a row spread over the banks
 #pragma unroll
-      for (int round = 0; round < 2; ++round) {
+      for (int round = 0; round < 4; ++round) {
+        if (round * C >= d_real) break;
         float o[C];
-        const int give = (1 - g) * (D / 2) + round * C, keep = g * (D / 2) + round * C;
-        if (mine > 0) tmem_ld_cols<C>(tO + give, o);
+        if (mine > 0) tmem_ld_cols<C>(tO + round * C, o);
 #pragma unroll
-        for (int j = 0; j < C; ++j) xchg[j * 128 + r] = mine > 0 ? o[j] * f : 0.f;
+        for (int j = 0; j < Q4; ++j) {
+          xchg[(128 * g + r) * Q4 + (j ^ (r & (Q4 - 1)))] =
+              have ? make_float4(o[4 * j] * f, o[4 * j + 1] * f, o[4 * j + 2] * f, o[4 * j + 3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
         softmax_sync();
-        if (mine > 0) tmem_ld_cols<C>(tO + keep, o);
 #pragma unroll
-        for (int j = 0; j < C; ++j) o[j] = (mine > 0 ? o[j] * f : 0.f) + theirs[j * 128 + r];
-        softmax_sync();   // the next round, or the next piece's queries, go over what was read
-        if (have_row && keep < d_real) {
-          if (share != nullptr) {
-#pragma unroll
-            for (int j = 0; j < C; j += 4) {
-              *reinterpret_cast<float4*>(share + r * d_real + keep + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-            }
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at_row * d_real + keep);
-#pragma unroll
-            for (int j = 0; j < C / 8; ++j) {
-              uint32_t w[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = any ? pack2<BF16>(o[8 * j + 2 * k] * inv, o[8 * j + 2 * k + 1] * inv) : 0u;
-              dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < 128 * Q4 / 256; ++i) {
+          const int item = tid + 256 * i, rr = item / Q4, j = item % Q4;
+          if (rr < rows) {
+            const float4 a = xchg[rr * Q4 + (j ^ (rr & (Q4 - 1)))], b = xchg[(128 + rr) * Q4 + (j ^ (rr & (Q4 - 1)))];
+            const float4 v = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+            if (share != nullptr) {
+              *reinterpret_cast<float4*>(share + rr * d_real + round * C + 4 * j) = v;
+            } else {
+              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + static_cast<long long>(s_out[rr]) * d_real + round * C + 4 * j) =
+                  make_uint2(pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w));
             }
           }
         }
+        softmax_sync();   // the next round, or the next piece's queries, go over what was read
       }
-      if (have_row && g == 0) {
+      if (r < rows && g == 0) {
         if (share != nullptr) {
           share[kWideRows * d_real + r] = top;
           share[kWideRows * d_real + kWideRows + r] = sum;
         } else if (p.lse != nullptr) {
-          p.lse[at_row] = any ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+          p.lse[s_out[r]] = any ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
         }
       }
     }
@@ -368,35 +376,35 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   tc_fence_before();
   __syncthreads();
   if (warp == 8) tmem_dealloc(tmem, 512);
-  grid_wait();   // a launch that was allowed to start early ends after its predecessor
+  if (how.late_wait) grid_wait();
 }
 
 template <int D, bool BF16, bool SOFTCAP>
 cudaError_t launch_wide_t(const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p, const CacheLaunch& how, int d_real,
-                          bool chained, cudaStream_t stream) {
+                          cudaStream_t stream) {
   auto kern = omni_cache_wide_kernel<D, BF16, SOFTCAP>;
   static SmemAttrOnce attr_once[kMaxDevices];
   const cudaError_t e = ensure_smem_attr(kern, WideCfg<D>::kSmem, attr_once);
   if (e != cudaSuccess) return e;
-  return launch_chained(kern, how.ctas, kWideThreads, WideCfg<D>::kSmem, chained, stream, tmK, tmV, p, how, d_real);
+  return launch_chained(kern, how.ctas, kWideThreads, WideCfg<D>::kSmem, stream, tmK, tmV, p, how, d_real);
 }
 
 template <int D, bool BF16>
 cudaError_t launch_wide_c(const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p, const CacheLaunch& how, int d_real,
-                          bool chained, cudaStream_t stream) {
-  return p.softcap > 0.f ? launch_wide_t<D, BF16, true>(tmK, tmV, p, how, d_real, chained, stream)
-                         : launch_wide_t<D, BF16, false>(tmK, tmV, p, how, d_real, chained, stream);
+                          cudaStream_t stream) {
+  return p.softcap > 0.f ? launch_wide_t<D, BF16, true>(tmK, tmV, p, how, d_real, stream)
+                         : launch_wide_t<D, BF16, false>(tmK, tmV, p, how, d_real, stream);
 }
 
 }  // namespace
 
 // head_dim 32 is computed as 64: the TMA unit fills the missing columns with zeros.
 cudaError_t launch_cache_wide(int head_dim, bool bf16, const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p,
-                              const CacheLaunch& how, bool chained, cudaStream_t stream) {
+                              const CacheLaunch& how, cudaStream_t stream) {
   if (head_dim == 128) {
-    return bf16 ? launch_wide_c<128, true>(tmK, tmV, p, how, head_dim, chained, stream) : launch_wide_c<128, false>(tmK, tmV, p, how, head_dim, chained, stream);
+    return bf16 ? launch_wide_c<128, true>(tmK, tmV, p, how, head_dim, stream) : launch_wide_c<128, false>(tmK, tmV, p, how, head_dim, stream);
   }
-  return bf16 ? launch_wide_c<64, true>(tmK, tmV, p, how, head_dim, chained, stream) : launch_wide_c<64, false>(tmK, tmV, p, how, head_dim, chained, stream);
+  return bf16 ? launch_wide_c<64, true>(tmK, tmV, p, how, head_dim, stream) : launch_wide_c<64, false>(tmK, tmV, p, how, head_dim, stream);
 }
 
 }  // namespace omni
