@@ -8,11 +8,11 @@
 // maximum, sum and O, and one group's chain runs under the other's products; at the end of a piece the groups' halves are
 // joined through shared memory.
 //
-// Roles of a CTA (one per SM, 320 threads):
+// Roles of a CTA (one per SM, 384 threads):
 //   warps 0-3, 4-7  softmax groups: thread = query row = TMEM lane. They also gather the rows' queries into shared memory
 //                   (any strides, rows of one tile may belong to different sequences) and write the result.
 //   warp 8          TMA: K and V of each tile of keys page by page into a ring (lane = page of the tile)
-//   warp 9          one elected thread issues every tcgen05.mma
+//   warp 9          one elected thread issues every tcgen05.mma; warps 10 and 11 only give their registers up
 // Hand-overs go through mbarriers; every wait is bounded as in the forward kernels. TMEM: S of the two groups (P, 16 bit,
 // over the first half of S), O of the two groups.
 //
@@ -25,7 +25,10 @@ namespace omni {
 
 namespace {
 
-constexpr int kWideThreads = 320;
+constexpr int kWideThreads = 384;
+// Registers: compiled for 168 a thread (what 384 threads can have); the softmax groups take over most of the third
+// warpgroup's. The increase must be covered by the decrease, or setmaxnreg.inc waits forever (checked before the launch).
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr float kLazyLog2 = 8.f;
 constexpr long long kDrain = 4000000000LL;
 
@@ -78,7 +81,8 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   const uint32_t bar_q = bar_empty + 8 * Cfg::kSlots;   // the rows' queries are in shared memory
   const uint32_t bar_s = bar_q + 8;                     // [2] scores done
   const uint32_t bar_p = bar_s + 16;                    // [2] P stored
-  const uint32_t bar_o = bar_p + 16;                    // [2] the group's last product of the piece done
+  const uint32_t bar_h = bar_p + 16;                    // [2] P of the tile's first 64 keys stored
+  const uint32_t bar_o = bar_h + 16;                    // [2] the group's last product of the piece done
   const uint32_t bar_end = bar_o + 16;                  // drain of a launch that gives up
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kBars + 256);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -98,6 +102,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     for (int g = 0; g < 2; ++g) {
       mbar_init(bar_s + 8 * g, 1);
       mbar_init(bar_p + 8 * g, 128);
+      mbar_init(bar_h + 8 * g, 128);
       mbar_init(bar_o + 8 * g, 1);
     }
     mbar_init(bar_end, 1);
@@ -122,6 +127,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   Piece pc;
 
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // =========================== softmax groups ===================================================
     const int g = warp >> 2, r = tid & 127;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -241,6 +247,11 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           if (!SOFTCAP && masked) apply_allow64(allow[2 * h], allow[2 * h + 1], s);
           sum += exp_and_pack_n<BF16, 0, 1, 64>(s, st.M, scale_log2, inv_scale_log2, pk);
           tmem_st32(tS + 32 * h, pk);
+          if (h == 0) {   // the product over the first 64 keys runs under the second half's exponentials
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar_h + 8 * g);
+          }
         }
         st.l = st.l * alpha + sum;
         tc_wait_st();
@@ -270,9 +281,8 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       const bool have = mine > 0 && any;
       constexpr int C = D / 4, Q4 = C / 4;   // columns of a round, 16-byte pieces of a row
       float4* xchg = reinterpret_cast<float4*>(smem);   // [2][128][Q4], pieces of a row spread over the banks
-#pragma unroll
-      for (int round = 0; round < 4; ++round) {
-        if (round * C >= d_real) break;
+#pragma unroll 1   // the code runs once or twice in a CTA: what counts is to fetch little of it
+      for (int round = 0; round * C < d_real; ++round) {
         float o[C];
         if (mine > 0) tmem_ld_cols<C>(tO + round * C, o);
 #pragma unroll
@@ -306,14 +316,15 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         }
       }
     }
-  } else if (warp == 8) {
-    // =========================== TMA ==============================================================
-    RingState st;
-    while (st.alive && walk.next(p, pc)) ring.stream(p, &tmK, &tmV, pc, pc.tile1, st, 46);
-    ring.drain(st);
   } else {
-    // =========================== MMA issuer =======================================================
-    if (elect_one()) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
+      // =========================== TMA ============================================================
+      RingState st;
+      while (st.alive && walk.next(p, pc)) ring.stream(p, &tmK, &tmV, pc, pc.tile1, st, 46);
+      ring.drain(st);
+    } else if (warp == 9 && elect_one()) {
+      // =========================== MMA issuer =====================================================
       constexpr int fmt = BF16 ? 1 : 0;
       constexpr uint32_t idesc_qk = umma_idesc_f16(128, 128, fmt, 0), idesc_pv = umma_idesc_f16(128, D, fmt, 1);
       constexpr uint32_t hi = umma_desc_hi_sw128(1024);
@@ -347,7 +358,8 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         for (int i = 0; alive && i < n; ++i) {
           const int g = i & 1;
           const uint32_t f = fill + 2 * i + 1, s = f % Cfg::kSlots;
-          alive = mbar_wait_lim(bar_p + 8 * g, (g == 0 ? n_p[0] : n_p[1]) & 1, abort_flag, p.status, 52 + g, limit) &&
+          const uint32_t par = (g == 0 ? n_p[0] : n_p[1]) & 1;
+          alive = mbar_wait_lim(bar_h + 8 * g, par, abort_flag, p.status, 52 + g, limit) &&
                   mbar_wait_lim(bar_full + 8 * s, (f / Cfg::kSlots) & 1, abort_flag, p.status, 54, limit);
           if (!alive) break;
           if (g == 0) {
@@ -359,7 +371,13 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           const uint32_t d = tmem + 256 + D * g, a = tmem + 128 * g, vd = v0 + s * kSlot;
           umma_ts_lo(d, a, vd, hi, idesc_pv, i >= 2 ? 1u : 0u);
 #pragma unroll
-          for (int k = 1; k < 8; ++k) umma_ts_lo_acc(d, a + 8 * k, vd + k * 128, hi, idesc_pv);   // 16 keys = 2048 bytes
+          for (int k = 1; k < 4; ++k) umma_ts_lo_acc(d, a + 8 * k, vd + k * 128, hi, idesc_pv);   // 16 keys = 2048 bytes
+          issued = true;
+          alive = mbar_wait_lim(bar_p + 8 * g, par, abort_flag, p.status, 56 + g, limit);
+          if (!alive) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 4; k < 8; ++k) umma_ts_lo_acc(d, a + 8 * k, vd + k * 128, hi, idesc_pv);
           tc_commit(bar_empty + 8 * s);
           if (i + 2 >= n) tc_commit(bar_o + 8 * g);
           if (i + 2 < n) scores(i + 2);
@@ -386,6 +404,11 @@ cudaError_t launch_wide_t(const CUtensorMap& tmK, const CUtensorMap& tmV, const 
   static SmemAttrOnce attr_once[kMaxDevices];
   const cudaError_t e = ensure_smem_attr(kern, WideCfg<D>::kSmem, attr_once);
   if (e != cudaSuccess) return e;
+  static const int regs = [kern] {
+    cudaFuncAttributes fa{};
+    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;
+  }();
+  if (2 * kSoftmaxRegs + kOtherRegs > 3 * regs) return cudaErrorLaunchOutOfResources;
   return launch_chained(kern, how.ctas, kWideThreads, WideCfg<D>::kSmem, stream, tmK, tmV, p, how, d_real);
 }
 
