@@ -98,7 +98,7 @@ bool vectors(const omni_attn_rotary* r, std::initializer_list<const omni_attn_he
   for (const void* o : out) {
     if (misaligned(o)) return false;
   }
-  return true;
+  return r == nullptr || (!misaligned(r->q_weight) && !misaligned(r->k_weight));
 }
 
 int heads_of(const omni_attn_heads* t) { return t == nullptr ? 0 : t->heads; }
@@ -129,6 +129,7 @@ int omni_attn_rotary_sm100(const omni_attn_heads* q, const omni_attn_heads* k, v
   set_segment(p.seg[1], k, k_out, rotary->k_weight);
   p.heads_total = heads_of(q) + heads_of(k);
   const bool vec = vectors(rotary, {q, k}, {q_out, k_out}, dtype == OMNI_DTYPE_F32 ? 4 : 2);
+  if (!rotary_fits(p, head_dim)) return OMNI_ERR_SHAPE;
   return ended(launch_rotary(dtype, head_dim, rotary->half_layout != 0, vec, false, p, static_cast<cudaStream_t>(cuda_stream)));
 }
 
@@ -181,6 +182,7 @@ int omni_attn_rotary_bwd_sm100(const omni_attn_heads* q, const omni_attn_heads* 
   bp.partial = static_cast<float*>(workspace);
   const bool vec = vectors(rotary, {q, k, q != nullptr ? d_q_out : nullptr, k != nullptr ? d_k_out : nullptr}, {dq, dk},
                            dtype == OMNI_DTYPE_F32 ? 4 : 2);
+  if (!rotary_fits(bp.f, head_dim)) return OMNI_ERR_SHAPE;
   return ended(launch_rotary_bwd(dtype, head_dim, rotary->half_layout != 0, vec, bp, static_cast<cudaStream_t>(cuda_stream)));
 }
 
@@ -213,6 +215,7 @@ int omni_attn_cache_append_sm100(const omni_attn_heads* q, const omni_attn_heads
   p.page_shift = shift_of(cache->page_size);
   p.status = status;
   const bool vec = vectors(rotary, {q, k, v}, {q_out}, 2);
+  if (!rotary_fits(p, head_dim)) return OMNI_ERR_SHAPE;
   const bool half = rotary != nullptr && rotary->half_layout != 0;
   return ended(launch_rotary(dtype, head_dim, half, vec, true, p, static_cast<cudaStream_t>(cuda_stream)));
 }

@@ -63,9 +63,9 @@ bool cache_attn_fits(const CacheAttnParams& p);
 
 // A programmatic dependent launch: may start before its predecessor on the stream has ended (omni_cache_line.cuh: grid_wait).
 template <typename... P, typename... A>
-inline cudaError_t launch_chained(void (*kern)(P...), unsigned grid, int threads, int smem, cudaStream_t stream, A&&... args) {
+inline cudaError_t launch_chained(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, A&&... args) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

@@ -16,7 +16,7 @@
 // elements) of a token and keeps their cosines and sines in registers while it walks over the heads, so that these are
 // computed once per token and group of heads, not once per row; D / 16 threads are a row, and the norm's sums go through
 // that many lanes' shuffles.
-#include "omni_common.cuh"
+#include "omni_cache_line.cuh"
 #include "omni_launch.h"
 #include "omni_rotary.cuh"
 
@@ -25,6 +25,8 @@ namespace omni {
 namespace {
 
 constexpr int kRotThreads = 256;
+constexpr int kRotCtas = 3;        // CTAs of the forward on an SM: 85 registers a thread
+constexpr int kSms = 148;
 
 template <typename T>
 struct Elem;
@@ -122,9 +124,14 @@ __device__ __forceinline__ void load_raw(const T* row, const P& at, Raw<T>& raw)
   }
 }
 
-// a[j], b[j]: the members of pair j.
+// The members of the thread's 8 pairs, two pairs to a packed 32-bit operation: a[i] = first members of pairs 2i and 2i + 1,
+// b[i] = the second ones.
+struct Pairs {
+  float2 a[4], b[4];
+};
+
 template <typename T, bool HALF, bool VEC>
-__device__ __forceinline__ void to_pairs(const Raw<T>& raw, float (&a)[8], float (&b)[8]) {
+__device__ __forceinline__ void to_pairs(const Raw<T>& raw, Pairs& x) {
   float u[8], v[8];
   if constexpr (sizeof(T) == 4) {
     const float* e = reinterpret_cast<const float*>(raw.c);
@@ -138,29 +145,31 @@ __device__ __forceinline__ void to_pairs(const Raw<T>& raw, float (&a)[8], float
     unpack8(raw.c[1], v, T());
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int i = 0; i < 4; ++i) {
     if constexpr (HALF || !VEC) {
-      a[j] = u[j];
-      b[j] = v[j];
-    } else {
-      a[j] = j < 4 ? u[2 * (j & 3)] : v[2 * (j & 3)];
-      b[j] = j < 4 ? u[2 * (j & 3) + 1] : v[2 * (j & 3) + 1];
+      x.a[i] = make_float2(u[2 * i], u[2 * i + 1]);
+      x.b[i] = make_float2(v[2 * i], v[2 * i + 1]);
+    } else {   // interleaved: four pairs in each run
+      const float(&e)[8] = i < 2 ? u : v;
+      x.a[i] = make_float2(e[4 * (i & 1)], e[4 * (i & 1) + 2]);
+      x.b[i] = make_float2(e[4 * (i & 1) + 1], e[4 * (i & 1) + 3]);
     }
   }
 }
 
 template <typename T, bool HALF, bool VEC, typename P>
-__device__ __forceinline__ void store_pairs(T* row, const P& at, const float (&a)[8], const float (&b)[8]) {
+__device__ __forceinline__ void store_pairs(T* row, const P& at, const Pairs& x) {
   if constexpr (VEC) {
     float u[8], v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int i = 0; i < 4; ++i) {
       if constexpr (HALF) {
-        u[j] = a[j];
-        v[j] = b[j];
+        u[2 * i] = x.a[i].x, u[2 * i + 1] = x.a[i].y;
+        v[2 * i] = x.b[i].x, v[2 * i + 1] = x.b[i].y;
       } else {
-        u[j] = (j & 1) ? b[j >> 1] : a[j >> 1];
-        v[j] = (j & 1) ? b[4 + (j >> 1)] : a[4 + (j >> 1)];
+        float(&e)[8] = i < 2 ? u : v;
+        e[4 * (i & 1)] = x.a[i].x, e[4 * (i & 1) + 1] = x.b[i].x;
+        e[4 * (i & 1) + 2] = x.a[i].y, e[4 * (i & 1) + 3] = x.b[i].y;
       }
     }
     if constexpr (sizeof(T) == 4) {
@@ -169,73 +178,89 @@ __device__ __forceinline__ void store_pairs(T* row, const P& at, const float (&a
       reinterpret_cast<float4*>(row + at.o1)[0] = make_float4(v[0], v[1], v[2], v[3]);
       reinterpret_cast<float4*>(row + at.o1)[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-      uint4 x, y;
-      x.x = pack2(u[0], u[1], T());
-      x.y = pack2(u[2], u[3], T());
-      x.z = pack2(u[4], u[5], T());
-      x.w = pack2(u[6], u[7], T());
-      y.x = pack2(v[0], v[1], T());
-      y.y = pack2(v[2], v[3], T());
-      y.z = pack2(v[4], v[5], T());
-      y.w = pack2(v[6], v[7], T());
-      *reinterpret_cast<uint4*>(row + at.o0) = x;
-      *reinterpret_cast<uint4*>(row + at.o1) = y;
+      *reinterpret_cast<uint4*>(row + at.o0) =
+          make_uint4(pack2(u[0], u[1], T()), pack2(u[2], u[3], T()), pack2(u[4], u[5], T()), pack2(u[6], u[7], T()));
+      *reinterpret_cast<uint4*>(row + at.o1) =
+          make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      Elem<T>::store(row + at.first(j), a[j]);
-      Elem<T>::store(row + at.second(j), b[j]);
+    for (int i = 0; i < 4; ++i) {
+      Elem<T>::store(row + at.first(2 * i), x.a[i].x);
+      Elem<T>::store(row + at.second(2 * i), x.b[i].x);
+      Elem<T>::store(row + at.first(2 * i + 1), x.a[i].y);
+      Elem<T>::store(row + at.second(2 * i + 1), x.b[i].y);
     }
   }
 }
 
-// The weight of the thread's elements, from a row of D weights in 32 bits or in the data's type.
+// The weights of the thread's elements, from a row of D weights in 32 bits or in the data's type.
 template <typename T, int D, bool HALF, bool VEC>
-__device__ __forceinline__ void load_weight(const void* w, bool f32, long long row, const Place<D, HALF>& at,
-                                            float (&a)[8], float (&b)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    int e0, e1;
-    if constexpr (VEC && !HALF) {
-      e0 = 2 * at.pair(j);
-      e1 = e0 + 1;
-    } else if constexpr (VEC) {
-      e0 = at.o0 + j;
-      e1 = at.o1 + j;
-    } else {
-      e0 = at.first(j);
-      e1 = at.second(j);
-    }
-    if (f32) {
-      a[j] = __ldg(static_cast<const float*>(w) + row * D + e0);
-      b[j] = __ldg(static_cast<const float*>(w) + row * D + e1);
-    } else {
-      a[j] = Elem<T>::load(static_cast<const T*>(w) + row * D + e0);
-      b[j] = Elem<T>::load(static_cast<const T*>(w) + row * D + e1);
-    }
+__device__ __forceinline__ void load_weight(const void* w, bool f32, int row, const Place<D, HALF>& at, Pairs& x) {
+  if (f32) {
+    Raw<float> raw;
+    load_raw<float, VEC>(static_cast<const float*>(w) + static_cast<long long>(row) * D, at, raw);
+    to_pairs<float, HALF, VEC>(raw, x);
+  } else {
+    Raw<T> raw;
+    load_raw<T, VEC>(static_cast<const T*>(w) + static_cast<long long>(row) * D, at, raw);
+    to_pairs<T, HALF, VEC>(raw, x);
   }
 }
 
-// Cosines and sines of the thread's pairs at position `pos`, with the factor; 1 and 0 for what is not rotated.
+// Cosines and sines of the thread's pairs at a position, with the factor; 1 and 0 for what is not rotated.
+struct Turn {
+  float2 c[4], s[4];
+};
 template <int D, bool HALF>
-__device__ __forceinline__ void turn_of(const RotaryParams& p, const Place<D, HALF>& at, long long pos, float (&c)[8],
-                                        float (&s)[8]) {
+__device__ __forceinline__ void turn_of(const RotaryParams& p, const Place<D, HALF>& at, long long pos, Turn& r) {
   const double t = static_cast<double>(pos) * 0.15915494309189533577;   // 1 / (2 pi)
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
+    float sn = 0.f, cs = 1.f;
     if (at.pair(j) < at.rd2) {
       double turns = t * __ldg(p.inv_freq + at.pair(j));
       turns -= rint(turns);
-      float sn, cs;
       sincospif(2.f * static_cast<float>(turns), &sn, &cs);
-      c[j] = cs * p.factor;
-      s[j] = sn * p.factor * p.sign;
-    } else {
-      c[j] = 1.f;
-      s[j] = 0.f;
+      cs *= p.factor;
+      sn *= p.factor * p.sign;
     }
+    (j & 1 ? r.c[j >> 1].y : r.c[j >> 1].x) = cs;
+    (j & 1 ? r.s[j >> 1].y : r.s[j >> 1].x) = sn;
   }
+}
+__device__ __forceinline__ void rotate(Pairs& x, const Turn& r) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 minus = make_float2(-r.s[i].x, -r.s[i].y);
+    const float2 a = __ffma2_rn(x.b[i], minus, __fmul2_rn(x.a[i], r.c[i]));
+    x.b[i] = __ffma2_rn(x.b[i], r.c[i], __fmul2_rn(x.a[i], r.s[i]));
+    x.a[i] = a;
+  }
+}
+__device__ __forceinline__ void scale_by(Pairs& x, float f) {
+  const float2 f2 = make_float2(f, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x.a[i] = __fmul2_rn(x.a[i], f2);
+    x.b[i] = __fmul2_rn(x.b[i], f2);
+  }
+}
+__device__ __forceinline__ void times(Pairs& x, const Pairs& w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x.a[i] = __fmul2_rn(x.a[i], w.a[i]);
+    x.b[i] = __fmul2_rn(x.b[i], w.b[i]);
+  }
+}
+__device__ __forceinline__ float dot(const Pairs& x, const Pairs& y) {
+  float2 s = __fmul2_rn(x.a[0], y.a[0]), t = __fmul2_rn(x.b[0], y.b[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    s = __ffma2_rn(x.a[i], y.a[i], s);
+    t = __ffma2_rn(x.b[i], y.b[i], t);
+  }
+  return (s.x + s.y) + (t.x + t.y);
 }
 
 __device__ __forceinline__ long long position_of(const RotaryParams& p, int b, int n) {
@@ -251,296 +276,282 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// Forward, and with sign = -1 the backward of a rotation without a norm. grid.x: tiles of tokens (all batch elements in
-// one row of tokens), grid.y: groups of heads. PAGED: k and v go into the pages of a cache, rows beyond a sequence's
-// count are not stored there and are zero in q's result.
+// Forward, and with sign = -1 the backward of a rotation without a norm. The units (tile of tokens, head), heads inside, are
+// cut into equal spans, one per CTA. PAGED: k and v go into the pages of a cache, rows beyond a sequence's count are not
+// stored there and are zero in q's result.
 template <typename T, int D, bool HALF, bool VEC, bool PAGED>
-__global__ void __launch_bounds__(kRotThreads) omni_rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int LPR = D / 16;                       // lanes of a row
   constexpr int ROWS = kRotThreads / LPR;
   const Place<D, HALF> at(threadIdx.x % LPR, p.rotary_dim);
-  const long long token = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / LPR;
-  const bool inside = token < p.tokens;
-  const int b = inside ? static_cast<int>(token / p.N) : 0;
-  const int n = inside ? static_cast<int>(token % p.N) : 0;
+  grid_wait();
+  grid_go();
+  unsigned u = blockIdx.x * p.span;
+  const unsigned end = min(u + p.span, p.units);
+  while (u < end) {
+    const unsigned tile = u / p.heads_total;
+    const int h0 = static_cast<int>(u - tile * p.heads_total), h1 = static_cast<int>(min(static_cast<unsigned>(p.heads_total), h0 + (end - u)));
+    u += h1 - h0;
+    const unsigned token = tile * ROWS + threadIdx.x / LPR;
+    const bool inside = token < p.tokens;
+    const int b = inside ? static_cast<int>(token / p.N) : 0, n = inside ? static_cast<int>(token - static_cast<unsigned>(b) * p.N) : 0;
 
-  float c[8], s[8];
-  turn_of<D, HALF>(p, at, position_of(p, b, n), c, s);
-
-  bool live = inside;
-  long long slot = -1;                              // row of the token's slot in head 0 of its page
-  if constexpr (PAGED) {
-    if (p.counts != nullptr && n >= __ldg(p.counts + b)) live = false;
-    if (live) {
-      const long long key = static_cast<long long>(max(__ldg(p.lengths + b), 0)) + n;
-      const long long entry = key >> p.page_shift;
-      const int page = entry < p.max_pages ? __ldg(p.page_table + b * p.table_stride + entry) : -1;
-      if (page >= 0 && page < p.num_pages) {
-        slot = ((static_cast<long long>(page) * p.seg[1].heads) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-      } else if (p.status != nullptr && at.lane == 0) {
-        atomicCAS(p.status, 0, kStatusBadIndex);
+    bool live = inside;
+    long long slot = -1;                              // row of the token's slot in head 0 of its page
+    if constexpr (PAGED) {
+      if (p.counts != nullptr && n >= __ldg(p.counts + b)) live = false;
+      if (live) {
+        const long long key = static_cast<long long>(max(__ldg(p.lengths + b), 0)) + n;
+        const long long entry = key >> p.page_shift;
+        const int page = entry < p.max_pages ? __ldg(p.page_table + b * p.table_stride + entry) : -1;
+        if (page >= 0 && page < p.num_pages) {
+          slot = ((static_cast<long long>(page) * p.seg[1].heads) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+        } else if (p.status != nullptr && at.lane == 0) {
+          atomicCAS(p.status, 0, kStatusBadIndex);
+        }
       }
     }
-  }
+    Turn turn;
+    bool turned = false;
 
-  const int h_end = min(p.heads_total, (static_cast<int>(blockIdx.y) + 1) * p.heads_per_group);
-  const int hq = p.seg[0].heads, hk = p.seg[1].heads;
-  auto segment = [&](int h) { return h < hq ? 0 : h < hq + hk ? 1 : 2; };
-  auto local = [&](int h, int g) { return h - (g == 0 ? 0 : g == 1 ? hq : hq + hk); };
-  auto source = [&](int h) {
-    const int g = segment(h);
-    const RotarySegment& sg = p.seg[g];
-    return static_cast<const T*>(sg.x) + b * sg.xs_b + local(h, g) * sg.xs_h + n * sg.xs_n;
-  };
-
-  Raw<T> next;
-  int h = blockIdx.y * p.heads_per_group;
-  if (h < h_end) load_raw<T, VEC>(source(h), at, next);
-  float wa[8], wb[8];
-  int weight_of = -1;
-  for (; h < h_end; ++h) {
-    const Raw<T> raw = next;
-    if (h + 1 < h_end) load_raw<T, VEC>(source(h + 1), at, next);
-    const int g = segment(h);
-    const RotarySegment& sg = p.seg[g];
-    const int hl = local(h, g);
-    float a[8], bb[8];
-    to_pairs<T, HALF, VEC>(raw, a, bb);
-    if (sg.w != nullptr) {
-      if (weight_of != g || p.w_per_head) {
-        load_weight<T, D, HALF, VEC>(sg.w, p.w_f32, p.w_per_head ? hl : 0, at, wa, wb);
-        weight_of = g;
+    // the heads of one of q, k, v that lie in the span
+    int base = 0;
+#pragma unroll 1
+    for (int g = 0; g < (PAGED ? 3 : 2); ++g) {
+      const RotarySegment& sg = p.seg[g];
+      const int from = max(h0 - base, 0), to = min(h1 - base, sg.heads);
+      base += sg.heads;
+      if (from >= to) continue;
+      const T* x = static_cast<const T*>(sg.x) + b * sg.xs_b + n * sg.xs_n + from * sg.xs_h;
+      Raw<T> next{};
+      if (live) load_raw<T, VEC>(x, at, next);   // what is not stored is not read
+      if (g < 2 && !turned) {   // the first rows are on their way meanwhile
+        turn_of<D, HALF>(p, at, position_of(p, b, n), turn);
+        turned = true;
       }
-      float sq = 0.f;
+      T* y;
+      long long ys;
+      bool store = inside;
+      if (PAGED && g > 0) {
+        y = static_cast<T*>(sg.y) + (slot + (static_cast<long long>(from) << p.page_shift)) * D;
+        ys = static_cast<long long>(D) << p.page_shift;
+        store = slot >= 0;
+      } else {
+        y = static_cast<T*>(sg.y) + ((static_cast<long long>(b) * sg.heads + from) * p.N + n) * D;
+        ys = static_cast<long long>(p.N) * D;
+      }
+      const bool zero = PAGED && g == 0 && !live;
+      const bool norm = sg.w != nullptr;
+      Pairs w;
+      if (norm) load_weight<T, D, HALF, VEC>(sg.w, p.w_f32, p.w_per_head ? from : 0, at, w);
+#pragma unroll 1
+      for (int h = from; h < to; ++h) {
+        Pairs v;
+        to_pairs<T, HALF, VEC>(next, v);
+        x += sg.xs_h;
+        if (h + 1 < to && live) load_raw<T, VEC>(x, at, next);
+        if (norm) {
+          const float r = rsqrtf(row_sum<LPR>(dot(v, v)) * (1.f / D) + p.eps);
+          times(v, w);
+          if (g < 2) rotate(v, turn);
+          scale_by(v, r);
+          if (p.w_per_head && h + 1 < to) load_weight<T, D, HALF, VEC>(sg.w, p.w_f32, h + 1, at, w);
+        } else if (g < 2) {
+          rotate(v, turn);
+        }
+        if (zero) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sq += a[j] * a[j] + bb[j] * bb[j];
-      const float r = rsqrtf(row_sum<LPR>(sq) * (1.f / D) + p.eps);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        a[j] *= r * wa[j];
-        bb[j] *= r * wb[j];
+          for (int i = 0; i < 4; ++i) v.a[i] = v.b[i] = make_float2(0.f, 0.f);
+        }
+        if (store) store_pairs<T, HALF, VEC>(y, at, v);
+        y += ys;
       }
-    }
-    if (g < 2) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float u = a[j], v = bb[j];
-        a[j] = u * c[j] - v * s[j];
-        bb[j] = u * s[j] + v * c[j];
-      }
-    }
-    if (PAGED && g > 0) {
-      if (slot >= 0) {
-        T* y = static_cast<T*>(sg.y) + (slot + (static_cast<long long>(hl) << p.page_shift)) * D;
-        store_pairs<T, HALF, VEC>(y, at, a, bb);
-      }
-    } else if (inside) {
-      if (PAGED && !live) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) a[j] = bb[j] = 0.f;
-      }
-      T* y = static_cast<T*>(sg.y) + ((static_cast<long long>(b) * sg.heads + hl) * p.N + n) * D;
-      store_pairs<T, HALF, VEC>(y, at, a, bb);
     }
   }
 }
 
 // Backward with a norm: dx of every row and, per CTA, the sum over its rows of the weight's gradient (added up by
-// omni_rotary_dw_kernel in a fixed order, so the result does not depend on which CTA ran first). grid.x: CTAs that share
-// the tiles of tokens, grid.y: groups of heads, none of which holds heads of both q and k.
-template <typename T, int D, bool HALF, bool VEC>
-__global__ void __launch_bounds__(kRotThreads) omni_rotary_bwd_kernel(const __grid_constant__ RotaryBwdParams bp) {
+// omni_rotary_dw_kernel in a fixed order, so the result does not depend on which CTA ran first). The units (tile of tokens,
+// head), those of q and then those of k, are cut into equal spans. With one weight for all heads the heads of a tile follow
+// one another (its angles are computed once), with a weight for each head the tiles of a head do (its sum stays in registers).
+template <typename T, int D, bool HALF, bool VEC, bool PER_HEAD>
+__global__ void __launch_bounds__(kRotThreads, 2) omni_rotary_bwd_kernel(const __grid_constant__ RotaryBwdParams bp) {
   constexpr int LPR = D / 16;
   constexpr int ROWS = kRotThreads / LPR;
+  __shared__ float red[kRotThreads / 32][D];
   const RotaryParams& p = bp.f;
   const Place<D, HALF> at(threadIdx.x % LPR, p.rotary_dim);
-  const int group = blockIdx.y;
-  const int g = group < bp.groups_q ? 0 : 1;
-  const RotarySegment& sg = p.seg[g];
-  const int per = g == 0 ? bp.per_q : bp.per_k;
-  const int h0 = (g == 0 ? group : group - bp.groups_q) * per, h1 = min(sg.heads, h0 + per);
+  grid_wait();
+  grid_go();
+  Pairs dw, w;
+  Turn turn;
+  const unsigned units_q = bp.tiles * p.seg[0].heads;
+  unsigned u = blockIdx.x * p.span;
+  const unsigned end = min(u + p.span, p.units);
 
-  float da[8], db[8], wa[8], wb[8];
+  // adds up the CTA's rows: those of a warp, then the warps, each in a fixed order
+  auto flush = [&](int sum) {
+    float v[16];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) da[j] = db[j] = 0.f;
-  load_weight<T, D, HALF, VEC>(sg.w, p.w_f32, p.w_per_head ? h0 : 0, at, wa, wb);
+    for (int i = 0; i < 4; ++i) v[2 * i] = dw.a[i].x, v[2 * i + 1] = dw.a[i].y, v[8 + 2 * i] = dw.b[i].x, v[9 + 2 * i] = dw.b[i].y;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+      for (int o = 16; o >= LPR; o >>= 1) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], o);
+    }
+    if ((threadIdx.x & 31) < LPR) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        red[threadIdx.x >> 5][VEC && HALF ? at.o0 + j : at.first(j)] = v[j];
+        red[threadIdx.x >> 5][VEC && HALF ? at.o1 + j : at.second(j)] = v[8 + j];
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float total = 0.f;
+#pragma unroll
+      for (int i = 0; i < kRotThreads / 32; ++i) total += red[i][threadIdx.x];
+      bp.partial[static_cast<long long>(blockIdx.x + sum) * D + threadIdx.x] = total;   // sums of a CTA follow one another: a place each
+    }
+    __syncthreads();
+  };
 
-  const long long tiles = (p.tokens + ROWS - 1) / ROWS;
-  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const long long token = tile * ROWS + threadIdx.x / LPR;
+  int sum_of = -1;   // which sum is in dw: 0 and 1 for q's and k's one weight, else the head (k's behind q's)
+  while (u < end) {
+    const int g = u < units_q ? 0 : 1;
+    const RotarySegment& sg = p.seg[g];
+    const unsigned in = g == 0 ? u : u - units_q, per = PER_HEAD ? bp.tiles : sg.heads;
+    const unsigned major = in / per, minor = in - major * per;
+    const unsigned tile = PER_HEAD ? minor : major;
+    const int h0 = static_cast<int>(PER_HEAD ? major : minor);
+    const int h1 = PER_HEAD ? h0 + 1 : static_cast<int>(min(static_cast<unsigned>(sg.heads), h0 + (end - u)));
+    u += h1 - h0;
+    const int sum = PER_HEAD ? h0 + (g == 0 ? 0 : p.seg[0].heads) : g;
+    if (sum != sum_of) {
+      if (sum_of >= 0) flush(sum_of);
+      sum_of = sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dw.a[i] = dw.b[i] = make_float2(0.f, 0.f);
+      load_weight<T, D, HALF, VEC>(sg.w, p.w_f32, PER_HEAD ? h0 : 0, at, w);
+    }
+    const unsigned token = tile * ROWS + threadIdx.x / LPR;
     const bool inside = token < p.tokens;
-    const int b = inside ? static_cast<int>(token / p.N) : 0;
-    const int n = inside ? static_cast<int>(token % p.N) : 0;
-    float c[8], s[8];
-    turn_of<D, HALF>(p, at, position_of(p, b, n), c, s);   // sign = -1: the rotation back
-    const T* xrow = static_cast<const T*>(sg.x) + b * sg.xs_b + n * sg.xs_n;
-    const T* grow = static_cast<const T*>(bp.g[g].x) + b * bp.g[g].xs_b + n * bp.g[g].xs_n;
+    const int b = inside ? static_cast<int>(token / p.N) : 0, n = inside ? static_cast<int>(token - static_cast<unsigned>(b) * p.N) : 0;
+    const T* x = static_cast<const T*>(sg.x) + b * sg.xs_b + n * sg.xs_n + h0 * sg.xs_h;
+    const T* gx = static_cast<const T*>(bp.g[g].x) + b * bp.g[g].xs_b + n * bp.g[g].xs_n + h0 * bp.g[g].xs_h;
+    T* y = static_cast<T*>(sg.y) + ((static_cast<long long>(b) * sg.heads + h0) * p.N + n) * D;
     Raw<T> nx, ng;
-    load_raw<T, VEC>(xrow + h0 * sg.xs_h, at, nx);
-    load_raw<T, VEC>(grow + h0 * bp.g[g].xs_h, at, ng);
+    load_raw<T, VEC>(x, at, nx);
+    load_raw<T, VEC>(gx, at, ng);
+    turn_of<D, HALF>(p, at, position_of(p, b, n), turn);   // sign = -1: the rotation back
+#pragma unroll 1
     for (int h = h0; h < h1; ++h) {
-      float a[8], bb[8], ga[8], gb[8];
-      to_pairs<T, HALF, VEC>(nx, a, bb);
-      to_pairs<T, HALF, VEC>(ng, ga, gb);
+      Pairs v, d;
+      to_pairs<T, HALF, VEC>(nx, v);
+      to_pairs<T, HALF, VEC>(ng, d);
       if (h + 1 < h1) {
-        load_raw<T, VEC>(xrow + (h + 1) * sg.xs_h, at, nx);
-        load_raw<T, VEC>(grow + (h + 1) * bp.g[g].xs_h, at, ng);
+        x += sg.xs_h;
+        gx += bp.g[g].xs_h;
+        load_raw<T, VEC>(x, at, nx);
+        load_raw<T, VEC>(gx, at, ng);
       }
-      float sq = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sq += a[j] * a[j] + bb[j] * bb[j];
-      const float r = rsqrtf(row_sum<LPR>(sq) * (1.f / D) + p.eps);
-      float dot = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float u = ga[j] * c[j] - gb[j] * s[j], v = ga[j] * s[j] + gb[j] * c[j];
-        a[j] *= r;
-        bb[j] *= r;
-        if (inside) {
-          da[j] += u * a[j];
-          db[j] += v * bb[j];
-        }
-        ga[j] = u * wa[j];
-        gb[j] = v * wb[j];
-        dot += ga[j] * a[j] + gb[j] * bb[j];
-      }
-      dot = row_sum<LPR>(dot) * (1.f / D);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        ga[j] = r * (ga[j] - a[j] * dot);
-        gb[j] = r * (gb[j] - bb[j] * dot);
-      }
+      const float r = rsqrtf(row_sum<LPR>(dot(v, v)) * (1.f / D) + p.eps);
+      rotate(d, turn);
+      scale_by(v, r);   // x_hat
       if (inside) {
-        T* y = static_cast<T*>(sg.y) + ((static_cast<long long>(b) * sg.heads + h) * p.N + n) * D;
-        store_pairs<T, HALF, VEC>(y, at, ga, gb);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          dw.a[i] = __ffma2_rn(d.a[i], v.a[i], dw.a[i]);
+          dw.b[i] = __ffma2_rn(d.b[i], v.b[i], dw.b[i]);
+        }
       }
-    }
-  }
-
-  // rows of a warp, then the warps, each in a fixed order
-  __shared__ float red[kRotThreads / 32][D];
+      times(d, w);
+      const float m = -row_sum<LPR>(dot(d, v)) * (1.f / D);
+      const float2 m2 = make_float2(m, m);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-#pragma unroll
-    for (int o = 16; o >= LPR; o >>= 1) {
-      da[j] += __shfl_xor_sync(0xFFFFFFFFu, da[j], o);
-      db[j] += __shfl_xor_sync(0xFFFFFFFFu, db[j], o);
-    }
-  }
-  if ((threadIdx.x & 31) < LPR) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      int e0, e1;
-      if constexpr (VEC && HALF) {
-        e0 = at.o0 + j;
-        e1 = at.o1 + j;
-      } else {
-        e0 = at.first(j);
-        e1 = at.second(j);
+      for (int i = 0; i < 4; ++i) {
+        d.a[i] = __ffma2_rn(v.a[i], m2, d.a[i]);
+        d.b[i] = __ffma2_rn(v.b[i], m2, d.b[i]);
       }
-      red[threadIdx.x >> 5][e0] = da[j];
-      red[threadIdx.x >> 5][e1] = db[j];
+      scale_by(d, r);
+      if (inside) store_pairs<T, HALF, VEC>(y, at, d);
+      y += static_cast<long long>(p.N) * D;
     }
   }
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRotThreads / 32; ++w) sum += red[w][threadIdx.x];
-    bp.partial[(static_cast<long long>(group) * gridDim.x + blockIdx.x) * D + threadIdx.x] = sum;
-  }
+  if (sum_of >= 0) flush(sum_of);
 }
 
-// Sums the CTAs' shares of the weights' gradients. One CTA per weight row: `rows_q` of q's, then those of k's.
+// Adds up the CTAs' shares of each weight row's gradient, 32 columns to a CTA, in the order of the CTAs.
 template <int D>
-__global__ void __launch_bounds__(256) omni_rotary_dw_kernel(const __grid_constant__ RotaryBwdParams bp, int rows_q, int ctas) {
-  constexpr int LANES = 256 / D;
-  __shared__ float red[LANES][D];
-  const int row = blockIdx.x;
-  const int g = row < rows_q ? 0 : 1;
-  const int local = g == 0 ? row : row - rows_q;
-  const bool per_head = bp.f.w_per_head;
-  const int first_group = (g == 0 ? 0 : bp.groups_q) + (per_head ? local : 0);
-  const int groups = per_head ? 1 : (g == 0 ? bp.groups_q : bp.groups_k);
-  const float* at = bp.partial + static_cast<long long>(first_group) * ctas * D;
-  const int col = threadIdx.x % D, lane = threadIdx.x / D;
-  const long long count = static_cast<long long>(groups) * ctas;
-  float sum = 0.f;
-#pragma unroll 8
-  for (long long i = lane; i < count; i += LANES) sum += at[i * D + col];
-  red[lane][col] = sum;
+__global__ void __launch_bounds__(1024) omni_rotary_dw_kernel(const __grid_constant__ RotaryBwdParams bp) {
+  __shared__ float red[32][33];
+  const RotaryParams& p = bp.f;
+  const int sum = blockIdx.x, hq = p.seg[0].heads;
+  const bool per_head = p.w_per_head;
+  const int g = per_head ? (sum < hq ? 0 : 1) : (bp.sums == 2 ? sum : (hq > 0 ? 0 : 1));
+  const int row = per_head ? sum - (g == 0 ? 0 : hq) : 0;
+  const int place = per_head ? sum : g;
+  // the units that went into this sum, and the CTAs that had them
+  const unsigned u0 = per_head ? bp.tiles * sum : (g == 0 ? 0 : bp.tiles * hq), u1 = per_head ? u0 + bp.tiles : u0 + bp.tiles * p.seg[g].heads;
+  const unsigned c0 = u0 / p.span, c1 = (u1 - 1) / p.span;
+  const int col = blockIdx.y * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+  grid_wait();
+  float total = 0.f;
+#pragma unroll 4
+  for (unsigned c = c0 + lane; c <= c1; c += 32) total += __ldcg(bp.partial + static_cast<long long>(c + place) * D + col);
+  red[lane][threadIdx.x & 31] = total;
   __syncthreads();
-  if (threadIdx.x < D) {
-    float total = 0.f;
+  if (lane != 0) return;
+  total = 0.f;
 #pragma unroll
-    for (int l = 0; l < LANES; ++l) total += red[l][threadIdx.x];
-    void* dw = bp.dw[g];
-    const long long e = static_cast<long long>(local) * D + threadIdx.x;
-    if (bp.f.w_f32) {
-      static_cast<float*>(dw)[e] = total;
-    } else if (bp.f.bf16) {
-      static_cast<__nv_bfloat16*>(dw)[e] = __float2bfloat16_rn(total);
-    } else {
-      static_cast<__half*>(dw)[e] = __float2half_rn(total);
-    }
+  for (int i = 0; i < 32; ++i) total += red[i][threadIdx.x];
+  void* to = bp.dw[g];
+  const long long e = static_cast<long long>(row) * D + col;
+  if (p.w_f32) {
+    static_cast<float*>(to)[e] = total;
+  } else if (p.bf16) {
+    static_cast<__nv_bfloat16*>(to)[e] = __float2bfloat16_rn(total);
+  } else {
+    static_cast<__half*>(to)[e] = __float2half_rn(total);
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return sms;
+// Spans of the units, one per CTA: as many CTAs as `most`, or one per unit.
+void cut(RotaryParams& p, long long units, int most, int& ctas) {
+  p.units = static_cast<unsigned>(units);
+  p.span = static_cast<unsigned>((units + most - 1) / most);
+  ctas = static_cast<int>((units + p.span - 1) / p.span);
+}
+unsigned tiles_of(const RotaryParams& p, int D) {
+  const int rows = kRotThreads / (D / 16);
+  return static_cast<unsigned>((p.tokens + rows - 1) / rows);
 }
 
 template <typename T, int D, bool HALF, bool VEC>
 cudaError_t launch_t(RotaryParams p, bool paged, cudaStream_t stream) {
-  constexpr int ROWS = kRotThreads / (D / 16);
-  const long long tiles = (p.tokens + ROWS - 1) / ROWS;
-  // As many groups of heads as it takes to have four CTAs on every SM, no more: each group computes the cosines and sines again.
-  const long long want = (4LL * sm_count() + tiles - 1) / tiles;
-  const int groups = static_cast<int>(want < 1 ? 1 : want > p.heads_total ? p.heads_total : want);
-  p.heads_per_group = (p.heads_total + groups - 1) / groups;
-  const dim3 grid(static_cast<unsigned>(tiles), (p.heads_total + p.heads_per_group - 1) / p.heads_per_group);
-  if (paged) {
-    omni_rotary_kernel<T, D, HALF, VEC, true><<<grid, kRotThreads, 0, stream>>>(p);
-  } else {
-    omni_rotary_kernel<T, D, HALF, VEC, false><<<grid, kRotThreads, 0, stream>>>(p);
+  int ctas = 0;
+  cut(p, static_cast<long long>(tiles_of(p, D)) * p.heads_total, kSms * kRotCtas, ctas);
+  if constexpr (sizeof(T) == 2) {
+    if (paged) return launch_chained(omni_rotary_kernel<T, D, HALF, VEC, true>, ctas, kRotThreads, 0, stream, p);
   }
-  return cudaGetLastError();
+  return launch_chained(omni_rotary_kernel<T, D, HALF, VEC, false>, ctas, kRotThreads, 0, stream, p);
 }
 
-// How the token tiles and heads of a backward with norms are shared out; the workspace holds D floats for each CTA.
-void bwd_grid(const RotaryParams& p, int D, RotaryBwdParams& bp, int& ctas) {
-  const int rows = kRotThreads / (D / 16);
-  const long long tiles = (p.tokens + rows - 1) / rows;
-  const int hq = p.seg[0].heads, hk = p.seg[1].heads;
-  bp.per_q = bp.per_k = 1;
-  if (!p.w_per_head) {
-    const long long want = (4LL * 148 + tiles - 1) / tiles;   // groups, as in the forward
-    const int total = hq + hk;
-    const int per = static_cast<int>((total + want - 1) / want);
-    bp.per_q = per < hq ? per : (hq > 0 ? hq : 1);
-    bp.per_k = per < hk ? per : (hk > 0 ? hk : 1);
-  }
-  bp.groups_q = (hq + bp.per_q - 1) / bp.per_q;
-  bp.groups_k = (hk + bp.per_k - 1) / bp.per_k;
-  const int groups = bp.groups_q + bp.groups_k;
-  long long c = (8LL * 148 + groups - 1) / groups;   // CTAs of a group: eight per SM in all
-  ctas = static_cast<int>(c < tiles ? c : tiles);
+void cut_bwd(RotaryBwdParams& bp, int D, int& ctas) {
+  RotaryParams& p = bp.f;
+  bp.tiles = tiles_of(p, D);
+  bp.sums = p.w_per_head ? p.seg[0].heads + p.seg[1].heads : (p.seg[0].heads > 0) + (p.seg[1].heads > 0);
+  cut(p, static_cast<long long>(bp.tiles) * (p.seg[0].heads + p.seg[1].heads), kSms * 2, ctas);
 }
 
 template <typename T, int D, bool HALF, bool VEC>
 cudaError_t launch_bwd_t(RotaryBwdParams bp, cudaStream_t stream) {
   int ctas = 0;
-  bwd_grid(bp.f, D, bp, ctas);
-  const dim3 grid(ctas, bp.groups_q + bp.groups_k);
-  omni_rotary_bwd_kernel<T, D, HALF, VEC><<<grid, kRotThreads, 0, stream>>>(bp);
-  cudaError_t e = cudaGetLastError();
+  cut_bwd(bp, D, ctas);
+  const cudaError_t e = launch_chained(bp.f.w_per_head ? omni_rotary_bwd_kernel<T, D, HALF, VEC, true> : omni_rotary_bwd_kernel<T, D, HALF, VEC, false>,
+                                       ctas, kRotThreads, 0, stream, bp);
   if (e != cudaSuccess) return e;
-  const int rows_q = bp.f.seg[0].heads == 0 ? 0 : bp.f.w_per_head ? bp.f.seg[0].heads : 1;
-  const int rows_k = bp.f.seg[1].heads == 0 ? 0 : bp.f.w_per_head ? bp.f.seg[1].heads : 1;
-  omni_rotary_dw_kernel<D><<<rows_q + rows_k, 256, 0, stream>>>(bp, rows_q, ctas);
-  return cudaGetLastError();
+  return launch_chained(omni_rotary_dw_kernel<D>, dim3(bp.sums, D / 32), 1024, 0, stream, bp);
 }
 
 // What the kernels are built for: (type, head_dim, layout, vector or element loads).
@@ -580,10 +591,14 @@ cudaError_t launch_rotary_bwd(int dtype, int head_dim, bool half, bool vec, cons
   return dispatch<Backward>(dtype, head_dim, half, vec, p, stream);
 }
 long long rotary_bwd_partials(const RotaryParams& p, int head_dim) {
-  RotaryBwdParams bp;
+  RotaryBwdParams bp{};
+  bp.f = p;
   int ctas = 0;
-  bwd_grid(p, head_dim, bp, ctas);
-  return static_cast<long long>(bp.groups_q + bp.groups_k) * ctas * head_dim;
+  cut_bwd(bp, head_dim, ctas);
+  return static_cast<long long>(ctas + p.seg[0].heads + p.seg[1].heads + 1) * head_dim;
+}
+bool rotary_fits(const RotaryParams& p, int head_dim) {
+  return static_cast<long long>(tiles_of(p, head_dim)) * (p.seg[0].heads + p.seg[1].heads + p.seg[2].heads) < (1LL << 31);
 }
 
 }  // namespace omni

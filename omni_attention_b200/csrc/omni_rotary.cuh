@@ -29,7 +29,8 @@ struct RotaryParams {
   int N;
   int rotary_dim;
   int max_pages, num_pages, page_shift;
-  int heads_total, heads_per_group;
+  int heads_total;
+  unsigned units, span;      // (tile of tokens, head) units, and how many a CTA takes
   float factor, sign, eps;
   int pos64, w_f32, w_per_head, bf16;
 };
@@ -38,8 +39,9 @@ struct RotaryBwdParams {
   RotaryParams f;            // seg[0], seg[1]: x as in the forward, y = its gradient
   RotarySegment g[2];        // gradients of the results (x and strides)
   void* dw[2];
-  float* partial;            // [groups, CTAs of a group, D]
-  int groups_q, groups_k, per_q, per_k;
+  float* partial;            // [CTA + sum, D]: the sums a CTA has shares in follow one another
+  unsigned tiles;
+  int sums;                  // weight rows
 };
 
 // dtype: 0 fp16, 1 bf16, 2 fp32. vec: every row starts on a 16-byte boundary, and in the half layout rotary_dim is a
@@ -48,5 +50,8 @@ cudaError_t launch_rotary(int dtype, int head_dim, bool half, bool vec, bool pag
 cudaError_t launch_rotary_bwd(int dtype, int head_dim, bool half, bool vec, const RotaryBwdParams& p, cudaStream_t stream);
 // floats of RotaryBwdParams::partial
 long long rotary_bwd_partials(const RotaryParams& p, int head_dim);
+
+// Whether the call's units can be counted in 31 bits.
+bool rotary_fits(const RotaryParams& p, int head_dim);
 
 }  // namespace omni
