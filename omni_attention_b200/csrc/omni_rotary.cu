@@ -25,8 +25,10 @@ namespace omni {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotCtas = 3;        // CTAs of the forward on an SM: 85 registers a thread
+constexpr int kRotCtas = 2;        // CTAs on an SM: 128 registers a thread
 constexpr int kSms = 148;
+constexpr int kRotAhead = 4;       // heads that a thread of the forward has on their way
+constexpr int kRotBwdStages = 3;   // stages of the backward's ring
 
 template <typename T>
 struct Elem;
@@ -124,6 +126,69 @@ __device__ __forceinline__ void load_raw(const T* row, const P& at, Raw<T>& raw)
   }
 }
 
+// A warp's ring in shared memory for the rows it is going to need (VEC), copied there with cp.async, so that several heads are
+// on their way without taking registers (with one ahead in registers, 16 to 24 KB on an SM, a third of the time went into
+// waiting). A copy's 32 lanes read whole neighbouring 32-byte sectors - in the threads' own places of an interleaved row
+// half of each was read twice, 66 against 38 us - so lanes copy for one another: a __syncwarp stands between the wait and the
+// reads. The 16-byte chunks are spread over the banks (place), for the copies and for the threads' own reads.
+template <typename T, int D, int STAGES>
+struct RowRing {
+  static constexpr int kLanes = D / 16;                            // of a row
+  static constexpr int kRow = D * static_cast<int>(sizeof(T)) / 16;   // chunks of a row
+  static constexpr int kCopies = kRow / kLanes;                    // chunks that a lane copies, and that it reads
+  static constexpr int kStage = 32 * kCopies * 16;                 // bytes of a warp
+  static constexpr int kBytes = STAGES * kStage * (kRotThreads / 32);
+  uint32_t base;
+  uint32_t own[kCopies];    // where this thread's chunks are
+  const T* from[kCopies];   // what it copies next
+  uint32_t live;            // bit i: copy i is of a row that is needed
+
+  static __device__ __forceinline__ uint32_t place(int chunk) {
+    const int line = chunk >> 3;
+    return (line * 8 + ((chunk & 7) ^ (line & 3))) * 16;
+  }
+  template <typename P>
+  __device__ __forceinline__ RowRing(uint32_t smem, const P& at) : base(smem + (threadIdx.x >> 5) * (STAGES * kStage)), live(0) {
+    const int row = (threadIdx.x & 31) / kLanes;
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) own[c] = base + place(row * kRow + (c < kCopies / 2 ? at.o0 : at.o1) / E + c % (kCopies / 2));
+  }
+  // `x`: the first row that this thread itself is going to need; `needed`: whether it is.
+  __device__ __forceinline__ void start(const T* x, bool needed) {
+    const int lane = threadIdx.x & 31;
+    const unsigned all = __ballot_sync(0xFFFFFFFFu, needed);
+    live = 0;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int chunk = lane + 32 * i, owner = chunk / kRow * kLanes;
+      from[i] = reinterpret_cast<const T*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(x), owner)) + chunk % kRow * (16 / sizeof(T));
+      live |= (all >> owner & 1u) << i;
+    }
+  }
+  // Copies a head's rows, and steps to the next head's.
+  __device__ __forceinline__ void issue(int stage, long long step) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      if (live >> i & 1u) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + stage * kStage + place(lane + 32 * i)), "l"(from[i]) : "memory");
+      }
+      from[i] += step;
+    }
+  }
+  __device__ __forceinline__ void read(int stage, Raw<T>& raw) const {
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) raw.c[c] = lds_v4(own[c] + stage * kStage);
+  }
+};
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void ring_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // The members of the thread's 8 pairs, two pairs to a packed 32-bit operation: a[i] = first members of pairs 2i and 2i + 1,
 // b[i] = the second ones.
 struct Pairs {
@@ -212,7 +277,9 @@ __device__ __forceinline__ void load_weight(const void* w, bool f32, int row, co
 struct Turn {
   float2 c[4], s[4];
 };
-template <int D, bool HALF>
+// EXACT: sincospif (an ulp or two); else the special function unit's sine and cosine of an angle within half a turn, off by
+// 2^-21, which a 16-bit result does not show and takes a tenth of the instructions.
+template <bool EXACT, int D, bool HALF>
 __device__ __forceinline__ void turn_of(const RotaryParams& p, const Place<D, HALF>& at, long long pos, Turn& r) {
   const double t = static_cast<double>(pos) * 0.15915494309189533577;   // 1 / (2 pi)
 #pragma unroll
@@ -221,7 +288,11 @@ __device__ __forceinline__ void turn_of(const RotaryParams& p, const Place<D, HA
     if (at.pair(j) < at.rd2) {
       double turns = t * __ldg(p.inv_freq + at.pair(j));
       turns -= rint(turns);
-      sincospif(2.f * static_cast<float>(turns), &sn, &cs);
+      if constexpr (EXACT) {
+        sincospif(2.f * static_cast<float>(turns), &sn, &cs);
+      } else {
+        __sincosf(6.2831853071795865f * static_cast<float>(turns), &sn, &cs);
+      }
       cs *= p.factor;
       sn *= p.factor * p.sign;
     }
@@ -284,6 +355,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_kernel(cons
   constexpr int LPR = D / 16;                       // lanes of a row
   constexpr int ROWS = kRotThreads / LPR;
   const Place<D, HALF> at(threadIdx.x % LPR, p.rotary_dim);
+  constexpr int kAhead = sizeof(T) == 4 ? 2 : kRotAhead;
   grid_wait();
   grid_go();
   unsigned u = blockIdx.x * p.span;
@@ -314,54 +386,82 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_kernel(cons
     Turn turn;
     bool turned = false;
 
-    // the heads of one of q, k, v that lie in the span
-    int base = 0;
-#pragma unroll 1
-    for (int g = 0; g < (PAGED ? 3 : 2); ++g) {
-      const RotarySegment& sg = p.seg[g];
-      const int from = max(h0 - base, 0), to = min(h1 - base, sg.heads);
-      base += sg.heads;
-      if (from >= to) continue;
-      const T* x = static_cast<const T*>(sg.x) + b * sg.xs_b + n * sg.xs_n + from * sg.xs_h;
-      Raw<T> next{};
-      if (live) load_raw<T, VEC>(x, at, next);   // what is not stored is not read
-      if (g < 2 && !turned) {   // the first rows are on their way meanwhile
-        turn_of<D, HALF>(p, at, position_of(p, b, n), turn);
-        turned = true;
+    // The span's heads in order, of q, then k, then v, kAhead of them on their way. What is not stored is not read.
+    int rd = h0, rd_end = 0, rd_seg = -1;   // next head to be read, where its segment ends
+    const T* rd_x = nullptr;
+    long long rd_step = 0;
+    auto read = [&](Raw<T>& raw) {
+      if (rd >= h1) return;
+      if (rd >= rd_end) {   // the same in all threads
+        do {
+          ++rd_seg;
+          rd_end += p.seg[rd_seg].heads;
+        } while (rd >= rd_end);
+        const RotarySegment& sg = p.seg[rd_seg];
+        rd_step = sg.xs_h;
+        rd_x = static_cast<const T*>(sg.x) + b * sg.xs_b + n * sg.xs_n + (rd - (rd_end - sg.heads)) * rd_step;
       }
-      T* y;
-      long long ys;
-      bool store = inside;
-      if (PAGED && g > 0) {
-        y = static_cast<T*>(sg.y) + (slot + (static_cast<long long>(from) << p.page_shift)) * D;
-        ys = static_cast<long long>(D) << p.page_shift;
-        store = slot >= 0;
-      } else {
-        y = static_cast<T*>(sg.y) + ((static_cast<long long>(b) * sg.heads + from) * p.N + n) * D;
-        ys = static_cast<long long>(p.N) * D;
-      }
-      const bool zero = PAGED && g == 0 && !live;
-      const bool norm = sg.w != nullptr;
-      Pairs w;
-      if (norm) load_weight<T, D, HALF, VEC>(sg.w, p.w_f32, p.w_per_head ? from : 0, at, w);
+      if (live) load_raw<T, VEC>(rd_x, at, raw);
+      rd_x += rd_step;
+      ++rd;
+    };
+    Raw<T> raw[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      raw[i] = Raw<T>{};
+      read(raw[i]);
+    }
+
+    int seg = -1, seg_end = 0, hl = 0;   // of the head at hand; its number in the segment
+    T* y = nullptr;
+    long long ys = 0;
+    bool store = false, zero = false, norm = false;
+    Pairs w;
 #pragma unroll 1
-      for (int h = from; h < to; ++h) {
+    for (int h = h0; h < h1;) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i, ++h) {
+        if (h >= h1) break;
+        if (h >= seg_end) {
+          do {
+            ++seg;
+            seg_end += p.seg[seg].heads;
+          } while (h >= seg_end);
+          const RotarySegment& sg = p.seg[seg];
+          hl = h - (seg_end - sg.heads);
+          if (PAGED && seg > 0) {
+            y = static_cast<T*>(sg.y) + (slot + (static_cast<long long>(hl) << p.page_shift)) * D;
+            ys = static_cast<long long>(D) << p.page_shift;
+            store = slot >= 0;
+            zero = false;
+          } else {
+            y = static_cast<T*>(sg.y) + ((static_cast<long long>(b) * sg.heads + hl) * p.N + n) * D;
+            ys = static_cast<long long>(p.N) * D;
+            store = inside;
+            zero = PAGED && !live;
+          }
+          norm = sg.w != nullptr;
+          if (norm) load_weight<T, D, HALF, VEC>(sg.w, p.w_f32, p.w_per_head ? hl : 0, at, w);
+          if (seg < 2 && !turned) {
+            turn_of<sizeof(T) == 4, D, HALF>(p, at, position_of(p, b, n), turn);
+            turned = true;
+          }
+        }
         Pairs v;
-        to_pairs<T, HALF, VEC>(next, v);
-        x += sg.xs_h;
-        if (h + 1 < to && live) load_raw<T, VEC>(x, at, next);
+        to_pairs<T, HALF, VEC>(raw[i], v);
+        read(raw[i]);
         if (norm) {
           const float r = rsqrtf(row_sum<LPR>(dot(v, v)) * (1.f / D) + p.eps);
           times(v, w);
-          if (g < 2) rotate(v, turn);
+          if (seg < 2) rotate(v, turn);
           scale_by(v, r);
-          if (p.w_per_head && h + 1 < to) load_weight<T, D, HALF, VEC>(sg.w, p.w_f32, h + 1, at, w);
-        } else if (g < 2) {
+          if (p.w_per_head && h + 1 < min(h1, seg_end)) load_weight<T, D, HALF, VEC>(p.seg[seg].w, p.w_f32, ++hl, at, w);
+        } else if (seg < 2) {
           rotate(v, turn);
         }
         if (zero) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v.a[i] = v.b[i] = make_float2(0.f, 0.f);
+          for (int j = 0; j < 4; ++j) v.a[j] = v.b[j] = make_float2(0.f, 0.f);
         }
         if (store) store_pairs<T, HALF, VEC>(y, at, v);
         y += ys;
@@ -375,12 +475,15 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_kernel(cons
 // head), those of q and then those of k, are cut into equal spans. With one weight for all heads the heads of a tile follow
 // one another (its angles are computed once), with a weight for each head the tiles of a head do (its sum stays in registers).
 template <typename T, int D, bool HALF, bool VEC, bool PER_HEAD>
-__global__ void __launch_bounds__(kRotThreads, 2) omni_rotary_bwd_kernel(const __grid_constant__ RotaryBwdParams bp) {
+__global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_bwd_kernel(const __grid_constant__ RotaryBwdParams bp) {
   constexpr int LPR = D / 16;
   constexpr int ROWS = kRotThreads / LPR;
+  constexpr int kStages = kRotBwdStages;
   __shared__ float red[kRotThreads / 32][D];
+  extern __shared__ __align__(16) uint8_t rotary_smem[];
   const RotaryParams& p = bp.f;
   const Place<D, HALF> at(threadIdx.x % LPR, p.rotary_dim);
+  RowRing<T, D, kStages> ring_x(smem_u32(rotary_smem), at), ring_g(smem_u32(rotary_smem) + RowRing<T, D, kStages>::kBytes, at);
   grid_wait();
   grid_go();
   Pairs dw, w;
@@ -440,21 +543,41 @@ __global__ void __launch_bounds__(kRotThreads, 2) omni_rotary_bwd_kernel(const _
     const T* x = static_cast<const T*>(sg.x) + b * sg.xs_b + n * sg.xs_n + h0 * sg.xs_h;
     const T* gx = static_cast<const T*>(bp.g[g].x) + b * bp.g[g].xs_b + n * bp.g[g].xs_n + h0 * bp.g[g].xs_h;
     T* y = static_cast<T*>(sg.y) + ((static_cast<long long>(b) * sg.heads + h0) * p.N + n) * D;
-    Raw<T> nx, ng;
-    load_raw<T, VEC>(x, at, nx);
-    load_raw<T, VEC>(gx, at, ng);
-    turn_of<D, HALF>(p, at, position_of(p, b, n), turn);   // sign = -1: the rotation back
-#pragma unroll 1
-    for (int h = h0; h < h1; ++h) {
-      Pairs v, d;
-      to_pairs<T, HALF, VEC>(nx, v);
-      to_pairs<T, HALF, VEC>(ng, d);
-      if (h + 1 < h1) {
-        x += sg.xs_h;
-        gx += bp.g[g].xs_h;
-        load_raw<T, VEC>(x, at, nx);
-        load_raw<T, VEC>(gx, at, ng);
+    const int n_rows = h1 - h0;
+    if constexpr (VEC) {
+      __syncwarp();
+      ring_x.start(x, inside);
+      ring_g.start(gx, inside);
+    }
+    auto read_ahead = [&](int i) {   // row i of the run
+      if constexpr (VEC) {
+        if (i < n_rows) {
+          ring_x.issue(i % kStages, sg.xs_h);
+          ring_g.issue(i % kStages, bp.g[g].xs_h);
+        }
+        ring_commit();
       }
+    };
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) read_ahead(i);
+    turn_of<sizeof(T) == 4, D, HALF>(p, at, position_of(p, b, n), turn);   // sign = -1: the rotation back
+#pragma unroll 1
+    for (int i = 0; i < n_rows; ++i) {
+      Pairs v, d;
+      {
+        Raw<T> raw_x, raw_g;
+        if constexpr (VEC) {
+          ring_wait<kStages - 2>();
+          ring_x.read(i % kStages, raw_x);
+          ring_g.read(i % kStages, raw_g);
+        } else {
+          load_raw<T, false>(x + i * sg.xs_h, at, raw_x);
+          load_raw<T, false>(gx + i * bp.g[g].xs_h, at, raw_g);
+        }
+        to_pairs<T, HALF, VEC>(raw_x, v);
+        to_pairs<T, HALF, VEC>(raw_g, d);
+      }
+      read_ahead(i + kStages - 1);
       const float r = rsqrtf(row_sum<LPR>(dot(v, v)) * (1.f / D) + p.eps);
       rotate(d, turn);
       scale_by(v, r);   // x_hat
@@ -477,6 +600,7 @@ __global__ void __launch_bounds__(kRotThreads, 2) omni_rotary_bwd_kernel(const _
       if (inside) store_pairs<T, HALF, VEC>(y, at, d);
       y += static_cast<long long>(p.N) * D;
     }
+    if constexpr (VEC) ring_wait<0>();
   }
   if (sum_of >= 0) flush(sum_of);
 }
@@ -527,6 +651,16 @@ unsigned tiles_of(const RotaryParams& p, int D) {
   return static_cast<unsigned>((p.tokens + rows - 1) / rows);
 }
 
+// A launch with `smem` bytes of rings, chained to its predecessor.
+template <int SMEM, typename K, typename P>
+cudaError_t launch_ring(K kern, int ctas, cudaStream_t stream, const P& p, SmemAttrOnce (&once)[kMaxDevices]) {
+  if constexpr (SMEM > 32 * 1024) {   // (beside what a kernel has statically)
+    const cudaError_t e = ensure_smem_attr(kern, SMEM, once);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_chained(kern, ctas, kRotThreads, SMEM, stream, p);
+}
+
 template <typename T, int D, bool HALF, bool VEC>
 cudaError_t launch_t(RotaryParams p, bool paged, cudaStream_t stream) {
   int ctas = 0;
@@ -541,15 +675,17 @@ void cut_bwd(RotaryBwdParams& bp, int D, int& ctas) {
   RotaryParams& p = bp.f;
   bp.tiles = tiles_of(p, D);
   bp.sums = p.w_per_head ? p.seg[0].heads + p.seg[1].heads : (p.seg[0].heads > 0) + (p.seg[1].heads > 0);
-  cut(p, static_cast<long long>(bp.tiles) * (p.seg[0].heads + p.seg[1].heads), kSms * 2, ctas);
+  cut(p, static_cast<long long>(bp.tiles) * (p.seg[0].heads + p.seg[1].heads), kSms * kRotCtas, ctas);
 }
 
 template <typename T, int D, bool HALF, bool VEC>
 cudaError_t launch_bwd_t(RotaryBwdParams bp, cudaStream_t stream) {
   int ctas = 0;
   cut_bwd(bp, D, ctas);
-  const cudaError_t e = launch_chained(bp.f.w_per_head ? omni_rotary_bwd_kernel<T, D, HALF, VEC, true> : omni_rotary_bwd_kernel<T, D, HALF, VEC, false>,
-                                       ctas, kRotThreads, 0, stream, bp);
+  constexpr int kSmem = VEC ? 2 * RowRing<T, D, kRotBwdStages>::kBytes : 0;
+  static SmemAttrOnce once_shared[kMaxDevices], once_head[kMaxDevices];
+  const cudaError_t e = bp.f.w_per_head ? launch_ring<kSmem>(omni_rotary_bwd_kernel<T, D, HALF, VEC, true>, ctas, stream, bp, once_head)
+                                        : launch_ring<kSmem>(omni_rotary_bwd_kernel<T, D, HALF, VEC, false>, ctas, stream, bp, once_shared);
   if (e != cudaSuccess) return e;
   return launch_chained(omni_rotary_dw_kernel<D>, dim3(bp.sums, D / 32), 1024, 0, stream, bp);
 }
