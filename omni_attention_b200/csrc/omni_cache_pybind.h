@@ -8,9 +8,11 @@ int dtype_code(const torch::Tensor& t) {
   return t.scalar_type() == torch::kBFloat16 ? OMNI_DTYPE_BF16 : t.scalar_type() == torch::kHalf ? OMNI_DTYPE_F16 : OMNI_DTYPE_F32;
 }
 
-void require(bool ok, const std::string& msg) {
-  if (!ok) refuse(msg);
-}
+// The text is put together only for a refusal.
+#define OMNI_REQUIRE(ok, msg)  \
+  do {                         \
+    if (!(ok)) refuse(std::string(msg)); \
+  } while (0)
 
 std::string shape_of(const torch::Tensor& t) {
   std::ostringstream os;
@@ -19,23 +21,23 @@ std::string shape_of(const torch::Tensor& t) {
 }
 
 void check_heads(const torch::Tensor& t, const char* name, bool f32) {
-  require(t.dim() == 4, std::string(name) + " must be [B, H, N, D], got " + shape_of(t));
+  OMNI_REQUIRE(t.dim() == 4, std::string(name) + " must be [B, H, N, D], got " + shape_of(t));
   const auto d = t.size(3);
   if (d != 32 && d != 64 && d != 128) {
     pybind11::gil_scoped_acquire gil;
     throw pybind11::value_error("Unsupported head_dim=" + std::to_string(d) + ". Supported: 32, 64, 128.");
   }
   const auto ty = t.scalar_type();
-  require(ty == torch::kHalf || ty == torch::kBFloat16 || (f32 && ty == torch::kFloat32),
+  OMNI_REQUIRE(ty == torch::kHalf || ty == torch::kBFloat16 || (f32 && ty == torch::kFloat32),
           std::string("unsupported dtype of ") + name + (f32 ? ": fp16, bf16 or fp32" : ": fp16 or bf16"));
-  for (int i = 0; i < 3; ++i) require(t.size(i) > 0, std::string(name) + " has an empty dimension: " + shape_of(t));
+  for (int i = 0; i < 3; ++i) OMNI_REQUIRE(t.size(i) > 0, std::string(name) + " has an empty dimension: " + shape_of(t));
 }
 
 // The device that the call runs on, and that every tensor of it must be on.
 void check_device(const torch::Tensor& first, std::initializer_list<const torch::Tensor*> rest) {
-  require(first.is_cuda(), "needs CUDA tensors (there is no CPU path)");
+  OMNI_REQUIRE(first.is_cuda(), "needs CUDA tensors (there is no CPU path)");
   for (const torch::Tensor* t : rest) {
-    require(!t->defined() || t->device() == first.device(), "all tensors must be on one device");
+    OMNI_REQUIRE(!t->defined() || t->device() == first.device(), "all tensors must be on one device");
   }
 }
 
@@ -60,32 +62,32 @@ struct RotaryArgs {
 void check_weight(const torch::Tensor& w, const char* name, const torch::Tensor& x) {
   if (!w.defined()) return;
   const bool shape = (w.dim() == 1 && w.size(0) == x.size(3)) || (w.dim() == 2 && w.size(0) == x.size(1) && w.size(1) == x.size(3));
-  require(shape, std::string(name) + " must be [D] or [heads, D], got " + shape_of(w));
-  require(w.scalar_type() == torch::kFloat32 || w.scalar_type() == x.scalar_type(), std::string(name) + " must be fp32 or of the data's dtype");
+  OMNI_REQUIRE(shape, std::string(name) + " must be [D] or [heads, D], got " + shape_of(w));
+  OMNI_REQUIRE(w.scalar_type() == torch::kFloat32 || w.scalar_type() == x.scalar_type(), std::string(name) + " must be fp32 or of the data's dtype");
 }
 
 // x: one of the tensors to be rotated ([B, H, N, D]).
 void check_rotary_args(const RotaryArgs& r, const torch::Tensor& q, const torch::Tensor& k) {
   const torch::Tensor& x = q.defined() ? q : k;
   if (r.inv_freq.defined()) {
-    require(r.inv_freq.dim() == 1 && r.inv_freq.scalar_type() == torch::kFloat64 && r.inv_freq.is_contiguous(),
+    OMNI_REQUIRE(r.inv_freq.dim() == 1 && r.inv_freq.scalar_type() == torch::kFloat64 && r.inv_freq.is_contiguous(),
             "inv_freq must be a contiguous float64 tensor [rotary_dim / 2]");
-    require(2 * r.inv_freq.size(0) <= x.size(3), "rotary_dim is larger than head_dim");
+    OMNI_REQUIRE(2 * r.inv_freq.size(0) <= x.size(3), "rotary_dim is larger than head_dim");
   }
   if (r.positions.defined()) {
     const auto& p = r.positions;
-    require(p.scalar_type() == torch::kInt32 || p.scalar_type() == torch::kInt64, "positions must be int32 or int64");
-    require((p.dim() == 1 && p.size(0) == x.size(2)) || (p.dim() == 2 && (p.size(0) == x.size(0) || p.size(0) == 1) && p.size(1) == x.size(2)),
+    OMNI_REQUIRE(p.scalar_type() == torch::kInt32 || p.scalar_type() == torch::kInt64, "positions must be int32 or int64");
+    OMNI_REQUIRE((p.dim() == 1 && p.size(0) == x.size(2)) || (p.dim() == 2 && (p.size(0) == x.size(0) || p.size(0) == 1) && p.size(1) == x.size(2)),
             "positions must be [N], [1, N] or [B, N], got " + shape_of(p));
   }
-  require(std::isfinite(r.factor), "the rotary factor must be finite");
-  require(r.eps >= 0.0 && std::isfinite(r.eps), "eps must be finite and not negative");
+  OMNI_REQUIRE(std::isfinite(r.factor), "the rotary factor must be finite");
+  OMNI_REQUIRE(r.eps >= 0.0 && std::isfinite(r.eps), "eps must be finite and not negative");
   if (r.q_weight.defined() && q.defined()) check_weight(r.q_weight, "q_weight", q);
   if (r.k_weight.defined() && k.defined()) check_weight(r.k_weight, "k_weight", k);
-  require(!r.q_weight.defined() || q.defined(), "q_weight without q");
-  require(!r.k_weight.defined() || k.defined(), "k_weight without k");
+  OMNI_REQUIRE(!r.q_weight.defined() || q.defined(), "q_weight without q");
+  OMNI_REQUIRE(!r.k_weight.defined() || k.defined(), "k_weight without k");
   if (r.q_weight.defined() && r.k_weight.defined()) {
-    require(r.q_weight.dim() == r.k_weight.dim() && r.q_weight.scalar_type() == r.k_weight.scalar_type(),
+    OMNI_REQUIRE(r.q_weight.dim() == r.k_weight.dim() && r.q_weight.scalar_type() == r.k_weight.scalar_type(),
             "q_weight and k_weight must be of one form and dtype");
   }
 }
@@ -226,11 +228,11 @@ pybind11::tuple rotary(const Optional& q_in, const Optional& k_in, const Optiona
   std::pair<torch::Tensor, torch::Tensor> out;
   {
     pybind11::gil_scoped_release nogil;
-    require(q.defined() || k.defined(), "omni_rotary needs q or k");
+    OMNI_REQUIRE(q.defined() || k.defined(), "omni_rotary needs q or k");
     if (q.defined()) check_heads(q, "q", true);
     if (k.defined()) check_heads(k, "k", true);
     if (q.defined() && k.defined()) {
-      require(q.scalar_type() == k.scalar_type() && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.size(3) == k.size(3),
+      OMNI_REQUIRE(q.scalar_type() == k.scalar_type() && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.size(3) == k.size(3),
               "q and k must share dtype, batch, length and head_dim: " + shape_of(q) + " and " + shape_of(k));
     }
     check_rotary_args(r, q, k);
@@ -256,15 +258,15 @@ pybind11::tuple rotary(const Optional& q_in, const Optional& k_in, const Optiona
 // The tensors of a paged cache, as the C ABI takes them.
 omni_attn_paged_cache cache_arg(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& table,
                                 const torch::Tensor& lengths, int64_t B, int64_t D, c10::ScalarType dtype) {
-  require(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), "k_pages and v_pages must be [num_pages, heads, page_size, D] of one shape");
-  require(k_pages.scalar_type() == dtype && v_pages.scalar_type() == dtype, "the cache and the new tokens must share a dtype");
-  require(k_pages.size(3) == D, "the cache's head_dim is not that of the new tokens");
-  require(k_pages.is_contiguous() && v_pages.is_contiguous(), "k_pages and v_pages must be contiguous");
-  require(table.dim() == 2 && table.size(0) == B && table.scalar_type() == torch::kInt32 && (table.size(1) <= 1 || table.stride(1) == 1),
+  OMNI_REQUIRE(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), "k_pages and v_pages must be [num_pages, heads, page_size, D] of one shape");
+  OMNI_REQUIRE(k_pages.scalar_type() == dtype && v_pages.scalar_type() == dtype, "the cache and the new tokens must share a dtype");
+  OMNI_REQUIRE(k_pages.size(3) == D, "the cache's head_dim is not that of the new tokens");
+  OMNI_REQUIRE(k_pages.is_contiguous() && v_pages.is_contiguous(), "k_pages and v_pages must be contiguous");
+  OMNI_REQUIRE(table.dim() == 2 && table.size(0) == B && table.scalar_type() == torch::kInt32 && (table.size(1) <= 1 || table.stride(1) == 1),
           "page_table must be int32 [B, max_pages]");
-  require(lengths.dim() == 1 && lengths.size(0) == B && lengths.scalar_type() == torch::kInt32 && (B == 1 || lengths.stride(0) == 1),
+  OMNI_REQUIRE(lengths.dim() == 1 && lengths.size(0) == B && lengths.scalar_type() == torch::kInt32 && (B == 1 || lengths.stride(0) == 1),
           "lengths must be int32 [B]");
-  require(k_pages.size(0) <= INT_MAX && table.size(1) <= INT_MAX, "too many pages");
+  OMNI_REQUIRE(k_pages.size(0) <= INT_MAX && table.size(1) <= INT_MAX, "too many pages");
   return {k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr<int32_t>(), B > 1 ? table.stride(0) : 0, lengths.data_ptr<int32_t>(),
           static_cast<int>(k_pages.size(0)), static_cast<int>(table.size(1)), static_cast<int>(k_pages.size(2)),
           static_cast<int>(k_pages.size(1))};
@@ -272,7 +274,7 @@ omni_attn_paged_cache cache_arg(const torch::Tensor& k_pages, const torch::Tenso
 
 const int32_t* int32_or_null(const torch::Tensor& t, c10::IntArrayRef shape, const char* what) {
   if (!t.defined()) return nullptr;
-  require(t.scalar_type() == torch::kInt32 && t.sizes() == shape && t.is_contiguous(), what);
+  OMNI_REQUIRE(t.scalar_type() == torch::kInt32 && t.sizes() == shape && t.is_contiguous(), what);
   return t.data_ptr<int32_t>();
 }
 
@@ -286,19 +288,19 @@ pybind11::object cache_append(const torch::Tensor& k_pages, const torch::Tensor&
     pybind11::gil_scoped_release nogil;
     check_heads(k, "k", false);
     check_heads(v, "v", false);
-    require(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "k and v must share shape and dtype");
+    OMNI_REQUIRE(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "k and v must share shape and dtype");
     if (q.defined()) {
       check_heads(q, "q", false);
-      require(q.scalar_type() == k.scalar_type() && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.size(3) == k.size(3),
+      OMNI_REQUIRE(q.scalar_type() == k.scalar_type() && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.size(3) == k.size(3),
               "q and k must share dtype, batch, length and head_dim: " + shape_of(q) + " and " + shape_of(k));
     }
     check_rotary_args(r, q, k);
     const int64_t B = k.size(0), N = k.size(2), D = k.size(3);
     const omni_attn_paged_cache cache = cache_arg(k_pages, v_pages, table, lengths, B, D, k.scalar_type());
-    require(cache.heads == k.size(1), "the cache's heads are not those of k");
+    OMNI_REQUIRE(cache.heads == k.size(1), "the cache's heads are not those of k");
     const int32_t* counts_ptr = int32_or_null(counts, {B}, "counts must be contiguous int32 [B]");
     int32_t* status_ptr = const_cast<int32_t*>(int32_or_null(status, {1}, "status must be int32 [1]"));
-    require(!wants_grad({&q, &k, &v, &r.q_weight, &r.k_weight}),
+    OMNI_REQUIRE(!wants_grad({&q, &k, &v, &r.q_weight, &r.k_weight}),
             "omni_cache_append has no backward: call it under torch.no_grad(), or on tensors that need no gradient");
     check_device(k, {&v, &q, &k_pages, &v_pages, &table, &lengths, &counts, &status, &r.inv_freq, &r.positions, &r.q_weight, &r.k_weight});
     at::AutoDispatchBelowADInplaceOrView below;
@@ -331,13 +333,13 @@ pybind11::object cache_attention(torch::Tensor q, const torch::Tensor& k_pages, 
     check_heads(q, "q", false);
     const int64_t B = q.size(0), H = q.size(1), T = q.size(2), D = q.size(3);
     const omni_attn_paged_cache cache = cache_arg(k_pages, v_pages, table, lengths, B, D, q.scalar_type());
-    require(cache.heads > 0 && H % cache.heads == 0, "the cache's heads must divide the queries' heads");
+    OMNI_REQUIRE(cache.heads > 0 && H % cache.heads == 0, "the cache's heads must divide the queries' heads");
     const int32_t* counts_ptr = int32_or_null(counts, {B}, "counts must be contiguous int32 [B]");
     const int32_t* limits_ptr = int32_or_null(limits, {B, T}, "limits must be contiguous int32 [B, T]");
     int32_t* status_ptr = const_cast<int32_t*>(int32_or_null(status, {1}, "status must be int32 [1]"));
-    require(std::isfinite(scale) && std::isfinite(softcap), "scale and softcap must be finite");
-    require(shared_prefix >= 0 && shared_prefix <= table.size(1) * k_pages.size(2), "shared_prefix must be from 0 to the tokens that the page table holds");
-    require(!wants_grad({&q, &k_pages, &v_pages}),
+    OMNI_REQUIRE(std::isfinite(scale) && std::isfinite(softcap), "scale and softcap must be finite");
+    OMNI_REQUIRE(shared_prefix >= 0 && shared_prefix <= table.size(1) * k_pages.size(2), "shared_prefix must be from 0 to the tokens that the page table holds");
+    OMNI_REQUIRE(!wants_grad({&q, &k_pages, &v_pages}),
             "omni_cache_attention has no backward: call it under torch.no_grad(), or on tensors that need no gradient");
     check_device(q, {&k_pages, &v_pages, &table, &lengths, &counts, &limits, &status});
     at::AutoDispatchBelowADInplaceOrView below;
@@ -362,6 +364,8 @@ pybind11::object cache_attention(torch::Tensor q, const torch::Tensor& k_pages, 
   if (want_lse) return pybind11::make_tuple(out, lse);
   return pybind11::cast(out);
 }
+
+#undef OMNI_REQUIRE
 
 void define_cache(pybind11::module_& m) {
   m.def("rotary", &rotary, "norms and rotation of queries and keys");

@@ -92,14 +92,19 @@ class OmniRotary:
     def to(self, device) -> "OmniRotary":
         return OmniRotary(self.inv_freq.to(device), self.layout, self.factor)
 
-    def at(self, positions: Optional[Tensor]) -> "RotaryAt":
-        """This rotation at the positions of a batch: what a patched attention module takes as ``rotary_emb``."""
-        return RotaryAt(self, positions)
+    def at(self, positions: Optional[Tensor] = None, q_weight: Optional[Tensor] = None, k_weight: Optional[Tensor] = None,
+           eps: float = 1e-6) -> "RotaryAt":
+        """This rotation at the positions of a batch, with the norms before it if there are any: what a patched attention
+        module takes as ``rotary_emb`` (``transfusion.patch_attention``)."""
+        return RotaryAt(self, positions, q_weight, k_weight, eps)
 
 
 class RotaryAt(NamedTuple):
     rotary: OmniRotary
-    positions: Optional[Tensor]
+    positions: Optional[Tensor] = None
+    q_weight: Optional[Tensor] = None
+    k_weight: Optional[Tensor] = None
+    eps: float = 1e-6
 
 
 def rotary_fields(rotary: Optional[OmniRotary]):

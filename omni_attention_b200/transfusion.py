@@ -5,7 +5,9 @@ the mask hook of ``Transformer.forward`` (:1108-1125).
 ``patch_attention(module)`` puts the kernels into a model: it replaces the ``forward`` of an attention
 module that has the reference ``Attention``'s attributes with one that runs the same projections, value
 residual, rotary, gates and output projection through the module's own sub-modules and hands the core
-to ``transfusion_attention_core`` whenever the call brings an ``OmniBlockMask``.
+to ``transfusion_attention_core`` whenever the call brings an ``OmniBlockMask``, and to ``omni_cache_append`` and
+``omni_cache_attention`` whenever it brings an ``OmniPagedCache`` (generation). An ``OmniRotary`` at the batch's positions
+(``rotary.at(positions)``) as ``rotary_emb`` turns q and k with ``omni_rotary``.
 
 In the reference model the core is either ``flex_attention(q, k, v, block_mask=...,
 score_mod=softcap_score_mod(softcap_value))`` (:953-961) or, without FlexAttention, scaled q k^T ->
@@ -21,7 +23,9 @@ import torch
 from torch import Tensor
 
 from .block_mask import OmniBlockMask, create_omni_block_mask_from_modality_positions
+from .cache import OmniPagedCache, omni_cache_append, omni_cache_attention
 from .ops import omni_attention, omni_attention_autograd
+from .rotary import RotaryAt, omni_rotary
 
 
 def transfusion_block_mask(modality_positions: Tensor, heads: int, seq_len: int, device=None) -> OmniBlockMask:
@@ -46,14 +50,46 @@ def transfusion_attention_core(q: Tensor, k: Tensor, v: Tensor, block_mask: Omni
 
 def _attention_forward_with_omni_core(module, original_forward):
     """The replacement ``forward``: the reference's argument list (transfusion_pytorch/transfusion.py:899-
-    910) and, for a call with ``block_mask`` an OmniBlockMask and no kv cache, the reference's steps
+    910) and, for a call with ``block_mask`` an OmniBlockMask or ``cache`` an OmniPagedCache, the reference's steps
     around the core (:921-950 before it, :987-1003 after it) on the module's own sub-modules, with the
-    core itself (:953-983) computed by the kernels. Every other call (decoding with a cache, a dense
-    ``attn_mask``, ``causal=True``, a flex BlockMask) goes to the module's original forward untouched."""
+    core itself (:953-983) computed by the kernels. Every other call (decoding with the reference's dense cache, a dense
+    ``attn_mask``, ``causal=True`` with a block mask, a flex BlockMask) goes to the module's original forward untouched.
+
+    With an OmniPagedCache the x of the call are the sequences' new tokens: their keys and values are stored behind the
+    cache's ``lengths`` (which the caller moves on after the last layer) and they attend to the cache and to each other,
+    ``causal`` or all of them (an image that is denoised). With a block mask as well it is the prompt, on an empty
+    cache: its tokens attend to each other by the mask and are stored."""
+
+    def rotated(q, k, rotary_emb):
+        if isinstance(rotary_emb, RotaryAt):
+            return omni_rotary(q, k, *rotary_emb)
+        rotate = getattr(module, "apply_rotary", None)
+        if rotate is None:
+            raise ValueError("rotary_emb given: pass an OmniRotary at the batch's positions (rotary.at(positions)), or set "
+                             "module.apply_rotary(rotary_emb, t) to the model's rotary function "
+                             "(transfusion_pytorch/transfusion.py:941-942 calls apply_rotary_emb(rotary_emb, t, freqs_seq_dim=-2))")
+        return rotate(rotary_emb, q), rotate(rotary_emb, k)
+
+    def cached_core(q, k, v, rotary_emb, cache, causal):
+        at = rotary_emb if isinstance(rotary_emb, RotaryAt) else None
+        if rotary_emb is not None and at is None:
+            q, k = rotated(q, k, rotary_emb)
+        q, k, v = (t.to(cache.k_pages.dtype) for t in (q, k, v))
+        if at is None:
+            omni_cache_append(cache, k, v)
+        else:
+            q = omni_cache_append(cache, k, v, q, at.rotary, at.positions, None, at.q_weight, at.k_weight, at.eps)
+        cap = float(module.softcap_value)
+        return omni_cache_attention(q, cache, causal=causal, scale=float(module.scale), softcap=cap if cap > 0 else None)
 
     def forward(x, attn_mask=None, rotary_emb=None, cache=None, causal=False, block_mask=None,
                 return_kv_cache=False, return_values=False, value_residual=None):
-        if not isinstance(block_mask, OmniBlockMask) or cache is not None or attn_mask is not None or causal:
+        masked, paged = isinstance(block_mask, OmniBlockMask), isinstance(cache, OmniPagedCache)
+        taken = attn_mask is None and (paged and (masked or block_mask is None) or masked and cache is None)
+        taken = taken and not (masked and causal)
+        if paged and not taken:
+            raise ValueError("a call with an OmniPagedCache takes an OmniBlockMask (the prompt) or no mask; `causal` goes with the latter")
+        if not taken:
             return original_forward(x, attn_mask=attn_mask, rotary_emb=rotary_emb, cache=cache, causal=causal,
                                     block_mask=block_mask, return_kv_cache=return_kv_cache, return_values=return_values,
                                     value_residual=value_residual)
@@ -63,20 +99,23 @@ def _attention_forward_with_omni_core(module, original_forward):
         if value_residual is not None:
             mix = module.to_learned_value_residual(x)
             v = v * mix + value_residual * (1.0 - mix)
-        kv_cache = torch.stack((k, v)) if return_kv_cache else None
-        if rotary_emb is not None:
-            rotate = getattr(module, "apply_rotary", None)
-            if rotate is None:
-                raise ValueError("rotary_emb given: set module.apply_rotary(rotary_emb, t) to the model's rotary function "
-                                 "(transfusion_pytorch/transfusion.py:941-942 calls apply_rotary_emb(rotary_emb, t, freqs_seq_dim=-2))")
-            q, k = rotate(rotary_emb, q), rotate(rotary_emb, k)
+        kv_cache = None
+        if return_kv_cache:
+            kv_cache = cache if paged else torch.stack((k, v))
         if getattr(module, "laser", False):
             v = ((v / module.laser_softclamp_value).tanh() * module.laser_softclamp_value).exp()
-        dtype = q.dtype
-        if dtype not in (torch.float16, torch.bfloat16):   # the kernels compute on 16-bit operands
-            q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
-        out = transfusion_attention_core(q.contiguous(), k.contiguous(), v.contiguous(), block_mask,
-                                         softcap_value=float(module.softcap_value), scale=float(module.scale)).to(dtype)
+        if paged and not masked:
+            out = cached_core(q, k, v, rotary_emb, cache, causal).to(q.dtype)
+        else:
+            if rotary_emb is not None:
+                q, k = rotated(q, k, rotary_emb)
+            dtype = q.dtype
+            if dtype not in (torch.float16, torch.bfloat16):   # the kernels compute on 16-bit operands
+                q, k, v = (t.to(cache.k_pages.dtype if paged else torch.bfloat16) for t in (q, k, v))
+            if paged:
+                omni_cache_append(cache, k, v)
+            out = transfusion_attention_core(q.contiguous(), k.contiguous(), v.contiguous(), block_mask,
+                                             softcap_value=float(module.softcap_value), scale=float(module.scale)).to(dtype)
         if getattr(module, "laser", False):
             out = out.log()
         if getattr(module, "to_gates", None) is not None:
@@ -98,7 +137,8 @@ def patch_attention(module):
     ``to_gates``, ``to_learned_value_residual``, ``laser`` / ``laser_softclamp_value``. Attention dropout
     is not applied by the kernels: a module whose ``dropout.p`` is non-zero in training mode is refused.
     The mask arrives through the ``block_mask`` argument the reference's forward already has, as an
-    OmniBlockMask (``transfusion_block_mask``). Returns the module; ``unpatch_attention`` undoes it."""
+    OmniBlockMask (``transfusion_block_mask``), a paged cache through ``cache``, the positions through ``rotary_emb``.
+    Returns the module; ``unpatch_attention`` undoes it."""
     for name in ("to_qk", "to_v", "to_out", "scale", "softcap_value"):
         if not hasattr(module, name):
             raise TypeError(f"patch_attention: the module has no attribute {name!r}")
