@@ -97,10 +97,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  const int bytes = ok ? 16 : 0;   // 0: the 16 bytes are filled with zeros, nothing is read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 // Arrives on `bar` (one of the arrivals it was initialised for) when this thread's cp.asyncs have landed.
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
@@ -175,19 +171,18 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   __syncthreads();
   const long long limit = p.wait_cycles;
 
-  if (warp == kWarps) {
-    // =========================== K and V ==========================================================
-    const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
+  if (warp >= kWarps) {
     Walk walk(p, how);
     Piece pc;
-    RingState st;
-    while (st.alive && walk.next(p, pc)) ring.stream(p, &tmK, &tmV, pc, pc.tile1, st, 61);
-    ring.drain(st);
-  } else if (warp > kWarps) {
+    if (warp == kWarps) {
+      // =========================== K and V ========================================================
+      const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
+      RingState st;
+      while (st.alive && walk.next(p, pc)) ring.stream(p, &tmK, &tmV, pc, pc.tile1, st, 61);
+      ring.drain(st);
+    }
     // =========================== queries and what is known of the rows ============================
-    Walk walk(p, how);
-    Piece pc;
-    for (int piece = 0;; ++piece) {
+    for (int piece = 0; warp > kWarps; ++piece) {
       const int buf = piece & 1;
       if (piece >= 2) {
         bool ok = true;
@@ -212,7 +207,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         to.out[lane] = static_cast<int>(out_row(p, id, pc.hk));
       }
       constexpr int CH = D / 8;
-#pragma unroll
+#pragma unroll 1   // code that runs once comes at about 7 cycles an instruction
       for (int i = 0; i < ROWS * CH / 32; ++i) {
         const int item = lane + 32 * i, r = item / CH, c = item % CH;
         const uint16_t* from = reinterpret_cast<const uint16_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(src), r));
@@ -546,12 +541,21 @@ __global__ void __launch_bounds__(256) omni_cache_join_kernel(const __grid_const
     const int seq = p.B == 1 ? 0 : static_cast<int>(item / per_seq);
     const int in_seq = static_cast<int>(item - seq * per_seq), hk = in_seq / rows, row = in_seq - hk * rows;
     unsigned before = 0;
-    for (int b = lane; b < seq; b += 32) before += lo.own_units(p, b);
-    before = __reduce_add_sync(0xFFFFFFFFu, before);
+    if (!lo.even) {
+      for (int b = lane; b < seq; b += 32) before += lo.own_units(p, b);
+      before = __reduce_add_sync(0xFFFFFFFFu, before);
+    }
     const unsigned units = lo.units_between(p.prefix, total_of(p, seq));
     const unsigned triple = static_cast<unsigned>(hk) * lo.rt_own + row / own.rows;
-    const unsigned first = lo.prefix_units + before + triple * units;
-    const unsigned c0 = first / lo.span, n1 = (first + units - 1) / lo.span - c0 + 1;
+    unsigned c0, n1;
+    if (lo.even) {
+      c0 = lo.first_cta(p, seq, triple);
+      n1 = lo.parts(units);
+    } else {
+      const unsigned first = lo.prefix_units + before + triple * units;
+      c0 = first / lo.span;
+      n1 = (first + units - 1) / lo.span - c0 + 1;
+    }
     if (p.prefix == 0 && n1 == 1) continue;   // written already
     // the row's shares: n0 of the prefix, then n1 of its own keys
     unsigned d0 = 0, n0 = 0, pt = 0;
@@ -561,8 +565,8 @@ __global__ void __launch_bounds__(256) omni_cache_join_kernel(const __grid_const
       pt = static_cast<unsigned>(hk) * lp.rt_prefix + gr / pre.rows;
       in0 = static_cast<int>(gr % pre.rows);
       const unsigned pu = lp.units_between(0, lp.prefix_end), f = pt * pu;
-      d0 = f / lp.span;
-      n0 = (f + pu - 1) / lp.span - d0 + 1;
+      d0 = lp.even ? lp.first_cta(p, -1, pt) : f / lp.span;
+      n0 = lp.even ? lp.parts(pu) : (f + pu - 1) / lp.span - d0 + 1;
     }
     const long long whole0 = 2LL * pre.ctas + pt;
     const long long whole1 = 2LL * own.ctas + static_cast<long long>(p.Hkv) * (lo.rt_prefix + static_cast<long long>(seq) * lo.rt_own) + triple;
@@ -663,7 +667,7 @@ Plan make_plan(int B, int Hkv, long long per, int head_dim, int prefix, long lon
   Plan pl{};
   const long long rows[2] = {B * per, per};
   auto tile = [](long long n) { return n > kNarrowRows ? kWideRows : n > 8 ? 16 : 8; };
-  const bool one = prefix == 0 || tile(rows[0]) == tile(rows[1]);
+  const bool one = prefix == 0 || (rows[0] > kNarrowRows) == (rows[1] > kNarrowRows);
   const long long tiles = (capacity + kTileKeys - 1) / kTileKeys;
   for (int i = 0; i < 2; ++i) {
     CacheLaunch& how = pl.of[i];
@@ -673,7 +677,7 @@ Plan make_plan(int B, int Hkv, long long per, int head_dim, int prefix, long lon
     }
     how.prefix = prefix > 0 && (one || i == 0);
     how.own = one || i == 1;
-    how.rows = tile(rows[how.own ? 1 : 0]);
+    how.rows = tile(rows[how.prefix ? 0 : 1]);
     how.uncut = prefix > 0 ? kUncutTilesPrefix : kUncutTiles;
     how.late_wait = i;
     how.rt_prefix = how.prefix ? static_cast<int>((rows[0] + how.rows - 1) / how.rows) : 0;
@@ -682,6 +686,7 @@ Plan make_plan(int B, int Hkv, long long per, int head_dim, int prefix, long lon
     pl.units += most;
     how.ctas = static_cast<int>(most < kCacheCtas ? most : kCacheCtas);
     how.per_cta = static_cast<unsigned>((triples + how.ctas - 1) / how.ctas);
+    how.even = static_cast<unsigned>(how.ctas / triples);
     how.share0 = pl.floats;
     pl.floats += (2LL * kCacheCtas + (prefix > 0 ? triples : 0)) * how.rows * (head_dim + 2);
     pl.join = prefix > 0 || how.per_cta * tiles > 1 + kUncutTiles;   // else it is never cut

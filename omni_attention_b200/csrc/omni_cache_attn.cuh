@@ -39,6 +39,7 @@ struct CacheLaunch {
   int rt_prefix, rt_own;        // row tiles of the prefix (0 without it), of a sequence
   unsigned per_cta;             // triples / ctas, rounded up
   unsigned uncut;               // see Line::uncut
+  unsigned even;                // CTAs for each triple, if there are that many (see Line::even)
   int late_wait;                // 0: waits for its predecessor before it reads anything; 1: only before it ends
   long long share0;             // its shares in the workspace, in floats
 };
@@ -60,6 +61,9 @@ cudaError_t launch_cache_wide(int head_dim, bool bf16, const CUtensorMap& tmK, c
                               const CacheLaunch& how, cudaStream_t stream);
 // Whether the call's line of units can be counted in 31 bits.
 bool cache_attn_fits(const CacheAttnParams& p);
+
+// What a second piece costs a CTA, in tiles: its queries, the first tile's way through the chain, the join of its shares.
+constexpr int kPieceTiles = 4;
 
 // A programmatic dependent launch: may start before its predecessor on the stream has ended (omni_cache_line.cuh: grid_wait).
 template <typename... P, typename... A>

@@ -39,7 +39,18 @@ struct Line {
   // A triple is one unit, none is cut and nothing has to be joined: where the CTA with most to do then has at most how.uncut
   // tiles of keys more than an even cut would give it.
   bool uncut;
+  // Or each triple is cut into this many parts by itself, one per CTA (0: not so): where that makes no CTA's part longer than
+  // an even cut's by more than a CTA's second piece would cost it.
+  unsigned even;
 
+  __device__ __forceinline__ unsigned part(unsigned units) const { return (units + even - 1) / even; }
+  __device__ __forceinline__ unsigned parts(unsigned units) const {
+    const unsigned n = part(units);
+    return (units + n - 1) / n;
+  }
+  __device__ __forceinline__ unsigned first_cta(const CacheAttnParams& p, int seq, unsigned triple) const {
+    return even * (seq < 0 ? triple : static_cast<unsigned>(p.Hkv) * (rt_prefix + static_cast<unsigned>(seq) * rt_own) + triple);
+  }
   __device__ __forceinline__ int tiles_between(int from, int to) const {
     return to > from ? (to - from + kTileKeys - 1) / kTileKeys : 1;   // a triple without keys still has rows to write
   }
@@ -77,6 +88,11 @@ __device__ __forceinline__ Line make_line(const CacheAttnParams& p, const CacheL
   const unsigned cut_units = heads * (ln.rt_prefix * tiles_prefix + rt_own * sum), cut_span = (cut_units + how.ctas - 1) / how.ctas;
   const unsigned triples = heads * (ln.rt_prefix + rt_own * p.B), per_cta = how.per_cta;
   ln.uncut = static_cast<unsigned long long>(per_cta) * max(tiles_prefix, tiles_own) <= cut_span + how.uncut;
+  ln.even = 0;
+  if (!ln.uncut && how.even >= 2) {
+    const unsigned longest = max(tiles_prefix, tiles_own);
+    if ((longest + how.even - 1) / how.even <= cut_span + kPieceTiles) ln.even = how.even;
+  }
   ln.prefix_units = how.prefix ? heads * ln.rt_prefix * ln.units_between(0, ln.prefix_end) : 0u;
   ln.units = ln.uncut ? triples : cut_units;
   ln.span = ln.uncut ? per_cta : cut_span;
@@ -99,6 +115,11 @@ struct Walk {
   int seg;
 
   __device__ __forceinline__ Walk(const CacheAttnParams& p, const CacheLaunch& how) : ln(make_line(p, how)), base(0), seg(-1) {
+    if (ln.even) {   // u: the triple, u_end: the part
+      u = blockIdx.x / ln.even;
+      u_end = blockIdx.x - u * ln.even;
+      return;
+    }
     u = ln.span * blockIdx.x;
     u_end = min(u + ln.span, ln.units);
     if (u >= u_end || u < ln.prefix_units) return;
@@ -130,16 +151,32 @@ struct Walk {
   }
 
   __device__ __forceinline__ bool next(const CacheAttnParams& p, Piece& pc) {
-    if (u >= u_end) return false;
+    unsigned triple = 0, first, n, rts;
+    if (ln.even) {
+      const unsigned np = static_cast<unsigned>(p.Hkv) * ln.rt_prefix, per = static_cast<unsigned>(p.Hkv) * ln.rt_own;
+      if (u >= np + (ln.how.own ? per * p.B : 0u)) return false;
+      seg = u < np ? -1 : static_cast<int>((u - np) / per);
+      triple = u < np ? u : u - np - static_cast<unsigned>(seg) * per;
+    } else if (u >= u_end) {
+      return false;
+    }
     pc.prefix = seg < 0;
     pc.seg = seg;
-    const unsigned rts = pc.prefix ? ln.rt_prefix : ln.rt_own;
+    rts = pc.prefix ? ln.rt_prefix : ln.rt_own;
     pc.table_of = pc.prefix ? ln.prefix_seq : seg;
     pc.key0 = pc.prefix ? 0 : p.prefix;
     pc.total = pc.prefix ? ln.prefix_end : total_of(p, seg);
     pc.rows = pc.prefix ? p.B * p.G * p.T : p.G * p.T;
     const unsigned units = ln.units_between(pc.key0, pc.total);
-    const unsigned triple = (u - base) / units, first = u - base - triple * units, n = min(units - first, u_end - u);
+    if (ln.even) {
+      first = u_end * ln.part(units);
+      if (first >= units) return false;   // a short triple has fewer parts
+      n = min(ln.part(units), units - first);
+    } else {
+      triple = (u - base) / units;
+      first = u - base - triple * units;
+      n = min(units - first, u_end - u);
+    }
     pc.whole = n == units;
     pc.tile0 = static_cast<int>(first);
     pc.tile1 = ln.uncut ? ln.tiles_between(pc.key0, pc.total) : static_cast<int>(first + n);
@@ -153,6 +190,10 @@ struct Walk {
     } else if (p.prefix > 0) {
       pc.share = 2LL * ln.how.ctas + triple;
       if (!pc.prefix) pc.share += static_cast<long long>(p.Hkv) * (ln.rt_prefix + static_cast<long long>(seg) * ln.rt_own);
+    }
+    if (ln.even) {
+      u = 0xFFFFFFFFu;   // that was all
+      return true;
     }
     u += n;
     if (u - base >= p.Hkv * rts * units) {
@@ -189,6 +230,11 @@ __device__ __forceinline__ long long out_row(const CacheAttnParams& p, const Row
 // pieces of the two kernels
 // ---------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  const int bytes = ok ? 16 : 0;   // 0: the 16 bytes are filled with zeros, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 
 // x: element along head_dim (a multiple of 64), y: row of the matrix of pages.
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y) {

@@ -138,7 +138,8 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     uint32_t fill = 0;                  // ring entries of the pieces before this one
     while (walk.next(p, pc)) {
       const int n = pc.tile1 - pc.tile0;
-      // ---- the rows' queries: thread (row tid / 2, half of its chunks) ----
+      // ---- the rows' queries: thread (row tid / 2, half of its chunks). (Two warps of their own with cp.async took longer:
+      // their copies stood behind the other warps' polls, 700 cycles each.) ----
       {
         const int row = pc.rt * kWideRows + (tid >> 1);
         const uint4* src = nullptr;
@@ -281,7 +282,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       const bool have = mine > 0 && any;
       constexpr int C = D / 4, Q4 = C / 4;   // columns of a round, 16-byte pieces of a row
       float4* xchg = reinterpret_cast<float4*>(smem);   // [2][128][Q4], pieces of a row spread over the banks
-#pragma unroll 1   // the code runs once or twice in a CTA: what counts is to fetch little of it
+#pragma unroll 1   // code that runs once comes at about 7 cycles an instruction: little of it counts
       for (int round = 0; round * C < d_real; ++round) {
         float o[C];
         if (mine > 0) tmem_ld_cols<C>(tO + round * C, o);
