@@ -23,7 +23,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import Tensor
 
-from .ops import STATUS_BAD_INDEX, OmniAttnError, load_extension
+from .ops import STATUS_BAD_INDEX, STATUS_WAIT_TIMEOUT, OmniAttnError, load_extension
 from .rotary import OmniRotary, rotary_fields
 
 
@@ -77,8 +77,11 @@ def _status(check: bool, device) -> Optional[Tensor]:
     return torch.zeros(1, dtype=torch.int32, device=device) if check else None
 
 
-def _raise_bad_index(status: Optional[Tensor]) -> None:
-    if status is not None and int(status.item()) & 0xFF == STATUS_BAD_INDEX:
+def _raise_for(status: Optional[Tensor]) -> None:
+    code = 0 if status is None else int(status.item())
+    if code & 0xFF == STATUS_WAIT_TIMEOUT:
+        raise OmniAttnError(f"kernel gave up waiting (status {code:#x}); output is not valid")
+    if code & 0xFF == STATUS_BAD_INDEX:
         raise OmniAttnError("page_table: a token's page is not there (id outside [0, num_pages), beyond the table's end, or "
                             "not the shared one); the token was left out")
 
@@ -99,7 +102,7 @@ def omni_cache_append(cache: OmniPagedCache, k: Tensor, v: Tensor, q: Optional[T
     status = _status(check_status, k.device)
     out = load_extension().cache_append(cache.k_pages, cache.v_pages, cache.page_table, cache.lengths, k, v, q, inv_freq, half,
                                         factor, positions, counts, q_weight, k_weight, eps, status)
-    _raise_bad_index(status)
+    _raise_for(status)
     return out
 
 
@@ -120,5 +123,5 @@ def omni_cache_attention(q: Tensor, cache: OmniPagedCache, counts: Optional[Tens
     status = _status(check_status, q.device)
     res = load_extension().cache_attention(q, cache.k_pages, cache.v_pages, cache.page_table, cache.lengths, counts, causal,
                                            limits, scale or 0.0, softcap or 0.0, return_lse, shared_prefix, status)
-    _raise_bad_index(status)
+    _raise_for(status)
     return res

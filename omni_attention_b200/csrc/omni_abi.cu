@@ -607,7 +607,7 @@ const char* omni_attn_error_string(int code) {
     case OMNI_ERR_PARTIAL: return "num_partial is negative, or positive without a partial mask pool";
     case OMNI_ERR_TOO_LONG:
       return "sequence longer than the kernel's block tables hold (131072 tokens with 128-blocks; see "
-             "omni_attn_max_seqlen)";
+             "omni_attn_max_seqlen), or a paged cache of more than 2^31 rows, tokens a sequence or units of work";
     case OMNI_ERR_ALIGNMENT: return "q, k, v, o and the partial mask pools must be 16-byte aligned";
     case OMNI_ERR_CUDA: return "a CUDA call failed (see omni_attn_last_cuda_error)";
     case OMNI_ERR_NO_DRIVER_ENTRY: return "cuTensorMapEncodeTiled not available from the CUDA driver";

@@ -170,16 +170,15 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   grid_go();
   __syncthreads();
   const long long limit = p.wait_cycles;
+  const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
+  RingState st;
 
   if (warp >= kWarps) {
     Walk walk(p, how);
     Piece pc;
     if (warp == kWarps) {
       // =========================== K and V ========================================================
-      const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
-      RingState st;
       while (st.alive && walk.next(p, pc)) ring.stream(p, &tmK, &tmV, pc, pc.tile1, st, 61);
-      ring.drain(st);
     }
     // =========================== queries and what is known of the rows ============================
     for (int piece = 0; warp > kWarps; ++piece) {
@@ -507,6 +506,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     }
   }
   __syncthreads();
+  if (*abort_flag && warp == kWarps) ring.drain(st);
   if (how.late_wait) grid_wait();
 }
 

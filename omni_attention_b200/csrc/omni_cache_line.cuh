@@ -317,9 +317,10 @@ struct Ring {
     }
   }
 
-  // A launch that gives up: nothing may still be on its way into shared memory when the CTA ends.
+  // A CTA that gave up: nothing may still be on its way into shared memory when it ends. By the producing warp, once no
+  // other warp can give up any more.
   __device__ __forceinline__ void drain(const RingState& st) const {
-    if (*abort_flag && (threadIdx.x & 31) == 0) {
+    if ((threadIdx.x & 31) == 0) {
       for (uint32_t s = 0; s < SLOTS && s < st.fill; ++s) {
         const uint32_t last = ((st.fill - 1 - s) / SLOTS) * SLOTS + s;
         mbar_wait_drain(full + 8 * s, (last / SLOTS) & 1, 4000000000LL);

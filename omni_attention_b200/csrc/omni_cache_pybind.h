@@ -164,6 +164,8 @@ struct OmniRotaryFn : torch::autograd::Function<OmniRotaryFn> {
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    // The kernels' results have no graph of their own: what create_graph=True asks for would be missing, silently.
+    if (at::GradMode::is_enabled()) refuse("omni_rotary has no second derivative (create_graph=True)");
     const auto saved = ctx->get_saved_variables();
     RotaryArgs r{saved[4], saved[5], saved[2], saved[3], ctx->saved_data["half"].toBool(), ctx->saved_data["factor"].toDouble(),
                  ctx->saved_data["eps"].toDouble()};
@@ -337,7 +339,7 @@ pybind11::object cache_attention(torch::Tensor q, const torch::Tensor& k_pages, 
     const int32_t* counts_ptr = int32_or_null(counts, {B}, "counts must be contiguous int32 [B]");
     const int32_t* limits_ptr = int32_or_null(limits, {B, T}, "limits must be contiguous int32 [B, T]");
     int32_t* status_ptr = const_cast<int32_t*>(int32_or_null(status, {1}, "status must be int32 [1]"));
-    OMNI_REQUIRE(std::isfinite(scale) && std::isfinite(softcap), "scale and softcap must be finite");
+    OMNI_REQUIRE(std::isfinite(scale) && std::isfinite(softcap) && scale >= 0.0, "scale and softcap must be finite, scale not negative");
     OMNI_REQUIRE(shared_prefix >= 0 && shared_prefix <= table.size(1) * k_pages.size(2), "shared_prefix must be from 0 to the tokens that the page table holds");
     OMNI_REQUIRE(!wants_grad({&q, &k_pages, &v_pages}),
             "omni_cache_attention has no backward: call it under torch.no_grad(), or on tensors that need no gradient");

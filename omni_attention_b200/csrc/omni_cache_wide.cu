@@ -121,6 +121,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   const uint32_t tmem = *tmem_slot;
   const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
   const long long limit = p.wait_cycles;
+  RingState st;
   if (!how.late_wait) grid_wait();   // lengths, queries and pages may be the predecessor's work
   grid_go();
   Walk walk(p, how);
@@ -321,9 +322,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
       // =========================== TMA ============================================================
-      RingState st;
       while (st.alive && walk.next(p, pc)) ring.stream(p, &tmK, &tmV, pc, pc.tile1, st, 46);
-      ring.drain(st);
     } else if (warp == 9 && elect_one()) {
       // =========================== MMA issuer =====================================================
       constexpr int fmt = BF16 ? 1 : 0;
@@ -332,7 +331,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       constexpr uint32_t kSlot = Cfg::kTile >> 4, kChunk = Cfg::kChunk >> 4;
       const uint32_t q0 = umma_desc_lo(sQ, 16), k0 = umma_desc_lo(sRing, 16), v0 = umma_desc_lo(sRing, Cfg::kChunk);
       uint32_t fill = 0, n_piece = 0, n_p[2] = {0, 0};
-      bool alive = true, issued = false;
+      bool alive = true;
       while (alive && walk.next(p, pc)) {
         const int n = pc.tile1 - pc.tile0;
         alive = mbar_wait_lim(bar_q, n_piece & 1, abort_flag, p.status, 50, limit);
@@ -352,7 +351,6 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           }
           tc_commit(bar_empty + 8 * s);
           tc_commit(bar_s + 8 * (i & 1));
-          issued = true;
         };
         if (alive) scores(0);
         if (alive && n > 1) scores(1);
@@ -373,7 +371,6 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           umma_ts_lo(d, a, vd, hi, idesc_pv, i >= 2 ? 1u : 0u);
 #pragma unroll
           for (int k = 1; k < 4; ++k) umma_ts_lo_acc(d, a + 8 * k, vd + k * 128, hi, idesc_pv);   // 16 keys = 2048 bytes
-          issued = true;
           alive = mbar_wait_lim(bar_p + 8 * g, par, abort_flag, p.status, 56 + g, limit);
           if (!alive) break;
           tc_fence_after();
@@ -385,15 +382,19 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         }
         fill += 2 * n;
       }
-      if (*abort_flag && issued) {   // giving up: wait for the MMAs in flight
-        tc_commit(bar_end);
-        mbar_wait_drain(bar_end, 0, kDrain);
-      }
     }
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {   // the same in all threads now: wait for what is in flight
+    if (warp == 8) ring.drain(st);
+    if (warp == 9 && elect_one()) {
+      tc_commit(bar_end);
+      mbar_wait_drain(bar_end, 0, kDrain);
+    }
+    __syncthreads();
+  }
   if (warp == 8) tmem_dealloc(tmem, 512);
   if (how.late_wait) grid_wait();
 }

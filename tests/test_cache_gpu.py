@@ -401,3 +401,24 @@ def test_a_denoised_block_is_written_again(cuda_device):
         got, lse = omni.omni_cache_attention(q, cache, causal=False, return_lse=True)
     want = orc.attention(q.cpu(), cache.k_pages.cpu(), cache.v_pages.cpu(), table, lens, causal=False)
     check(got, lse, *want, q.cpu(), cache.k_pages.cpu(), cache.v_pages.cpu(), 64 ** -0.5, "second pass", True)
+
+
+@pytest.mark.parametrize("H", [4, 48])      # 16-row and 128-row tiles
+@pytest.mark.parametrize("lengths", [[300, 20], [9000, 5000]])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(cuda_device, H, lengths):
+    """With a budget of one cycle every hand-over that is not there yet counts as run out: the CTAs give up, what they have
+    in flight is waited for, the status says so, and the next call is right."""
+    from omni_attention_b200 import ops
+
+    kp, vp, table, lens, g = make_cache(2, 2, 64, 64, lengths, 1, torch.float16)
+    q = torch.randn(2, H, 1, 64, generator=g).half().cuda()
+    cache = on_gpu(kp, vp, table, lens)
+    want = omni.omni_cache_attention(q, cache, check_status=True)
+    lib = ops.load_library()
+    lib.omni_attn_set_wait_cycles(1)
+    try:
+        with pytest.raises(omni.OmniAttnError, match="gave up waiting"):
+            omni.omni_cache_attention(q, cache, check_status=True)
+    finally:
+        lib.omni_attn_set_wait_cycles(0)       # back to the default budget
+    assert torch.equal(omni.omni_cache_attention(q, cache, check_status=True), want)

@@ -140,6 +140,7 @@ def test_attention_call():
     for bad in (-1, 33):
         refused("shared_prefix", f, q, c, shared_prefix=bad)
     refused("finite", f, q, c, scale=float("nan"))
+    refused("negative", f, q, c, scale=-1.0)
     refused("finite", f, q, c, softcap=float("inf"))
     refused("no backward", f, q.requires_grad_(), c)
 

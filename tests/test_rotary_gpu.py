@@ -224,3 +224,10 @@ def test_infinite_and_zero_rows_stay_where_they_are(cuda_device):
     clean[0, 3] = clean[1, 5] = False
     assert torch.isfinite(out[0].cpu()[clean]).all() and not torch.isfinite(out[0, 0, 3]).any()
     assert not out[0, 1, 6].any()
+
+
+def test_no_second_derivative(cuda_device):
+    q = torch.randn(1, 1, 4, 32, device="cuda", requires_grad=True)
+    out, _ = omni.omni_rotary(q, None, omni.OmniRotary.from_base(32, device="cuda"))
+    with pytest.raises(omni.OmniAttnError, match="second derivative"):
+        torch.autograd.grad(out.square().sum(), q, create_graph=True)
