@@ -33,11 +33,11 @@ template <int D>
 struct CacheCfg {
   static constexpr int kTile = 128 * D * 2;
   static constexpr int kChunks = D / 64;
-  static constexpr int kSlots = D == 128 ? 6 : 10;
+  static constexpr int kSlots = D == 128 ? 3 : 5;                            // pairs of K and V tiles
   static constexpr int kRound = D / 2;                                       // columns of a round of the join, 8 rows
   static constexpr int kJoin = kWarps * 8 * (kRound + 8) * 4;                // (16 rows: half of the columns)
   static constexpr int kQ = kNarrowRows * D * 2;                             // queries of a triple
-  static constexpr int kSmem = kSlots * kTile + kJoin + 2 * kQ + 2560;       // + barriers, descriptions
+  static constexpr int kSmem = kSlots * 2 * kTile + kJoin + 2 * kQ + 2560;       // + barriers, descriptions
 };
 
 // What the computing warps are told of a piece.
@@ -138,9 +138,9 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     if (p.status != nullptr && threadIdx.x == 0) atomicExch(p.status, kStatusWaitTimeout | (69 << 8));
     return;
   }
-  const uint32_t sRing = smem_u32(smem), sQ = sRing + Cfg::kSlots * Cfg::kTile;
-  float* s_join = reinterpret_cast<float*>(smem + Cfg::kSlots * Cfg::kTile + 2 * Cfg::kQ);
-  uint8_t* rest = smem + Cfg::kSlots * Cfg::kTile + 2 * Cfg::kQ + Cfg::kJoin;
+  const uint32_t sRing = smem_u32(smem), sQ = sRing + Cfg::kSlots * 2 * Cfg::kTile;
+  float* s_join = reinterpret_cast<float*>(smem + Cfg::kSlots * 2 * Cfg::kTile + 2 * Cfg::kQ);
+  uint8_t* rest = smem + Cfg::kSlots * 2 * Cfg::kTile + 2 * Cfg::kQ + Cfg::kJoin;
   uint64_t* bars = reinterpret_cast<uint64_t*>(rest);
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * Cfg::kSlots;
   const uint32_t bar_q = bar_empty + 8 * Cfg::kSlots;      // [2] a piece's description and queries are there
@@ -170,7 +170,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   grid_go();
   __syncthreads();
   const long long limit = p.wait_cycles;
-  const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
+  const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots, true> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
   RingState st;
 
   if (warp >= kWarps) {
@@ -284,19 +284,20 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         l[j] = 0.f;
       }
 
-      for (int t = 0; t < n; ++t, fill += 2) {
-        const uint32_t ks = fill % Cfg::kSlots, vs = (fill + 1) % Cfg::kSlots;
+      for (int t = 0; t < n; ++t, ++fill) {
+        const uint32_t slot = fill % Cfg::kSlots;
         const int key = key0 + t * kTileKeys;
-        if (lane == 0) mbar_wait_lim(bar_full + 8 * ks, (fill / Cfg::kSlots) & 1, abort_flag, p.status, 63, limit);
+        if (lane == 0) mbar_wait_lim(bar_full + 8 * slot, (fill / Cfg::kSlots) & 1, abort_flag, p.status, 63, limit);
         __syncwarp();
-        float s[NT][4];   // [rows 8 j ..]: keys quad (0, 1) and quad + 8 (2, 3), rows 2 pos and 2 pos + 1
-        if (key < lim_max) {   // else: nothing for this warp in the tile
-          const uint32_t sk = sRing + ks * Cfg::kTile;
+        const bool there = *const_cast<volatile uint32_t*>(&s_valid[slot][warp >> 1]) >> (16 * (warp & 1)) & 1u;   // a page has 16 keys at least
+        if (key < lim_max && there) {   // else: nothing for this warp in the tile
+          const uint32_t sk = sRing + slot * (2 * Cfg::kTile), sv = sk + Cfg::kTile;
+          float s[NT][4], s2[NT][4];   // [rows 8 j ..]: keys quad (0, 1) and quad + 8 (2, 3), rows 2 pos and 2 pos + 1
 #pragma unroll
-          for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-          float s2[NT][4];
-#pragma unroll
-          for (int j = 0; j < NT; ++j) s2[j][0] = s2[j][1] = s2[j][2] = s2[j][3] = 0.f;
+          for (int j = 0; j < NT; ++j) {
+            s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+            s2[j][0] = s2[j][1] = s2[j][2] = s2[j][3] = 0.f;
+          }
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
             uint32_t a[4];
@@ -309,22 +310,12 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[j][e] += s2[j][e];
           }
-        }
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bar_empty + 8 * ks);
-          mbar_wait_lim(bar_full + 8 * vs, ((fill + 1) / Cfg::kSlots) & 1, abort_flag, p.status, 64, limit);
-        }
-        __syncwarp();
-        const bool there = *const_cast<volatile uint32_t*>(&s_valid[vs][warp >> 1]) >> (16 * (warp & 1)) & 1u;   // a page has 16 keys at least
-        if (key < lim_max && there) {
-          const uint32_t sv = sRing + vs * Cfg::kTile;
           if (key + 16 > lim_max) {   // V that no row sees may be anything: 0 * NaN
 #pragma unroll
             for (int i = 0; i < 16 * Cfg::kChunks * 8 / 32; ++i) {
               const int item = lane + 32 * i, r = item & 15, c = item >> 4;
               if (key + r >= lim_max) {
-                *reinterpret_cast<uint4*>(smem + vs * Cfg::kTile + swizzled(warp * 16 + r, c, 128 * 128)) = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(smem + slot * (2 * Cfg::kTile) + Cfg::kTile + swizzled(warp * 16 + r, c, 128 * 128)) = make_uint4(0u, 0u, 0u, 0u);
               }
             }
             fence_async_smem();   // the ring's next copy goes over it
@@ -367,22 +358,20 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
               }
             }
           }
-          // running maximum: moved only when it would grow by more than 8 (p <= 2^8 in 32 bits and in either 16-bit type)
+          // Running maximum: looked for and moved only when a score is above it by more than 8 (p <= 2^8 in 32 bits and in
+          // either 16-bit type).
           bool move = false;
-          float top[2 * NT];
 #pragma unroll
-          for (int j = 0; j < 2 * NT; ++j) top[j] = fmaxf(s[j >> 1][j & 1], s[j >> 1][2 + (j & 1)]);
+          for (int j = 0; j < NT; ++j) {
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-#pragma unroll
-            for (int j = 0; j < 2 * NT; ++j) top[j] = fmaxf(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], o));
+            for (int e = 0; e < 4; ++e) move |= s[j][e] > m[2 * j + (e & 1)] + 8.f;
           }
-#pragma unroll
-          for (int j = 0; j < 2 * NT; ++j) move |= top[j] > m[j] + 8.f;
           if (__any_sync(0xFFFFFFFFu, move)) {
 #pragma unroll
             for (int j = 0; j < 2 * NT; ++j) {
-              const float to = fmaxf(m[j], top[j]);
+              float to = fmaxf(m[j], fmaxf(s[j >> 1][j & 1], s[j >> 1][2 + (j & 1)]));
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) to = fmaxf(to, __shfl_xor_sync(0xFFFFFFFFu, to, o));
               const float f = m[j] == -INFINITY ? 0.f : ex2_approx(m[j] - to);
               m[j] = to;
               l[j] *= f;
@@ -420,7 +409,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_empty + 8 * vs);
+        if (lane == 0) mbar_arrive(bar_empty + 8 * slot);
       }
 
       // ---- the warps' shares of the piece, joined: kRound columns at a time ----

@@ -250,13 +250,14 @@ __device__ __forceinline__ void grid_go() { asm volatile("griddepcontrol.launch_
 
 // The ring of K and V tiles (128 keys, [64 columns][128 rows][128 bytes], 128-byte swizzle) that a warp fills page by page.
 struct RingState {
-  uint32_t fill = 0;
+  uint32_t fill = 0;                // entries filled so far
   bool alive = true;
 };
-template <int TILE, int CHUNKS, int SLOTS>
+// An entry is a tile of K or V (PAIR: K and V of the same keys, one behind the other).
+template <int TILE, int CHUNKS, int SLOTS, bool PAIR>
 struct Ring {
   uint32_t data, full, empty;       // shared addresses
-  uint32_t (*valid)[4];             // [SLOTS]: of a V tile, which keys are there
+  uint32_t (*valid)[4];             // [SLOTS]: of an entry with V, which keys are there
   volatile int* abort_flag;
 
   // All lanes of the producing warp: tiles tile0 .. tile1 of a piece, K then V of each.
@@ -289,7 +290,7 @@ struct Ring {
       const int y = ok ? ((page * p.Hkv + pc.hk) << p.page_shift) + (key & (page_rows - 1)) : 0;
       const uint32_t bytes = __popc(there) * box * 128 * CHUNKS;
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv, ++st.fill) {
+      for (int kv = 0; kv < (PAIR ? 1 : 2); ++kv, ++st.fill) {
         const uint32_t s = st.fill % SLOTS;
         if (lane == 0 && st.fill >= SLOTS) {
           st.alive = mbar_wait_lim(empty + 8 * s, ((st.fill / SLOTS) - 1) & 1, abort_flag, p.status, where, p.wait_cycles);
@@ -297,20 +298,23 @@ struct Ring {
         st.alive = __shfl_sync(0xFFFFFFFFu, st.alive, 0) && !*abort_flag;
         st.alive = __all_sync(0xFFFFFFFFu, st.alive);
         if (!st.alive) break;
-        if (kv == 1 && lane < 4) valid[s][lane] = word;
+        if ((PAIR || kv == 1) && lane < 4) valid[s][lane] = word;
         __syncwarp();
         if (lane == 0) {
           if (bytes > 0) {
-            mbar_expect_tx(full + 8 * s, bytes);
+            mbar_expect_tx(full + 8 * s, PAIR ? 2 * bytes : bytes);
           } else {
             mbar_arrive(full + 8 * s);
           }
         }
         __syncwarp();
         if (ok) {
+          const uint32_t to = data + s * (PAIR ? 2 * TILE : TILE) + lane * box * 128;
 #pragma unroll
-          for (int c = 0; c < CHUNKS; ++c) {
-            tma_load_2d(data + s * TILE + c * (128 * 128) + lane * box * 128, kv == 0 ? tmK : tmV, full + 8 * s, c * 64, y);
+          for (int c = 0; c < CHUNKS; ++c) tma_load_2d(to + c * (128 * 128), kv == 0 ? tmK : tmV, full + 8 * s, c * 64, y);
+          if constexpr (PAIR) {
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) tma_load_2d(to + TILE + c * (128 * 128), tmV, full + 8 * s, c * 64, y);
           }
         }
       }

@@ -119,7 +119,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
+  const Ring<Cfg::kTile, Cfg::kChunks, Cfg::kSlots, false> ring{sRing, bar_full, bar_empty, s_valid, abort_flag};
   const long long limit = p.wait_cycles;
   RingState st;
   if (!how.late_wait) grid_wait();   // lengths, queries and pages may be the predecessor's work
