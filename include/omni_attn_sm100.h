@@ -394,10 +394,11 @@ int omni_attn_cache_append_sm100(const omni_attn_heads* q, const omni_attn_heads
  *  shared_prefix  the first that many tokens of all sequences are in the same pages (rounded down to whole pages): they
  *                 are read once for the batch. 0 = nothing is known to be shared. With a status word, table entries that
  *                 break the promise are reported as OMNI_STATUS_BAD_INDEX.
- *  workspace      omni_attn_cache_attention_workspace_bytes(...) bytes, 16-byte aligned; no state between calls, calls
- *                 that overlap in time need two
+ *  workspace      omni_attn_cache_attention_workspace_bytes(..., max_pages * page_size) bytes, 16-byte aligned; no state
+ *                 between calls, calls that overlap in time need two. May be NULL where that is 0 (a small cache).
  * What a page holds behind a sequence's last token is never used. */
-long long omni_attn_cache_attention_workspace_bytes(int B, int H, int kv_heads, int T, int head_dim, int shared_prefix);
+long long omni_attn_cache_attention_workspace_bytes(int B, int H, int kv_heads, int T, int head_dim, int shared_prefix,
+                                                    long long capacity);
 int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* lse_or_null,
                                     const omni_attn_paged_cache* cache, const int32_t* counts_or_null,
                                     const int32_t* limits_or_null, int causal, int B, int T, int head_dim, int dtype,

@@ -220,9 +220,10 @@ int omni_attn_cache_append_sm100(const omni_attn_heads* q, const omni_attn_heads
   return ended(launch_rotary(dtype, head_dim, half, vec, true, p, static_cast<cudaStream_t>(cuda_stream)));
 }
 
-long long omni_attn_cache_attention_workspace_bytes(int B, int H, int kv_heads, int T, int head_dim, int shared_prefix) {
-  if (B <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads != 0 || T <= 0) return 0;
-  return omni::cache_attn_workspace_bytes(B, H, kv_heads, T, head_dim, shared_prefix > 0);
+long long omni_attn_cache_attention_workspace_bytes(int B, int H, int kv_heads, int T, int head_dim, int shared_prefix,
+                                                    long long capacity) {
+  if (B <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads != 0 || T <= 0 || capacity <= 0) return 0;
+  return omni::cache_attn_workspace_bytes(B, H, kv_heads, T, head_dim, shared_prefix > 0, capacity);
 }
 
 int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* lse, const omni_attn_paged_cache* cache,
@@ -230,7 +231,7 @@ int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* 
                                     int dtype, float scale, float softcap, int shared_prefix, void* workspace,
                                     long long workspace_bytes, void* cuda_stream, int32_t* status) {
   using namespace omni;
-  if (q == nullptr || q->data == nullptr || out == nullptr || workspace == nullptr) return OMNI_ERR_NULL_POINTER;
+  if (q == nullptr || q->data == nullptr || out == nullptr) return OMNI_ERR_NULL_POINTER;
   if (dtype != OMNI_DTYPE_F16 && dtype != OMNI_DTYPE_BF16) return OMNI_ERR_DTYPE;
   int rc = check_sizes(B, T, head_dim);
   if (rc != OMNI_OK) return rc;
@@ -244,7 +245,9 @@ int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* 
   p.prefix = shared_prefix / cache->page_size * cache->page_size;
   p.capacity = static_cast<long long>(cache->max_pages) * cache->page_size;
   if (p.prefix > p.capacity) return OMNI_ERR_SEQLEN;
-  if (workspace_bytes < cache_attn_workspace_bytes(B, q->heads, cache->heads, T, head_dim, p.prefix > 0)) return OMNI_ERR_WORKSPACE;
+  const long long need = cache_attn_workspace_bytes(B, q->heads, cache->heads, T, head_dim, p.prefix > 0, p.capacity);
+  if (need > 0 && workspace == nullptr) return OMNI_ERR_NULL_POINTER;
+  if (workspace_bytes < need) return OMNI_ERR_WORKSPACE;
   p.q = q->data;
   p.qs_b = q->stride_b;
   p.qs_h = q->stride_h;

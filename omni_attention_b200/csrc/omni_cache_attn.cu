@@ -714,8 +714,9 @@ cudaError_t launch_t(const CacheAttnParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-long long cache_attn_workspace_bytes(int B, int H, int Hkv, int T, int head_dim, bool prefix) {
-  return make_plan(B, Hkv, static_cast<long long>(H / Hkv) * T, head_dim, prefix ? 1 : 0, 1 << 30).floats * 4;
+long long cache_attn_workspace_bytes(int B, int H, int Hkv, int T, int head_dim, bool prefix, long long capacity) {
+  const Plan pl = make_plan(B, Hkv, static_cast<long long>(H / Hkv) * T, head_dim, prefix ? 1 : 0, capacity);
+  return pl.join ? pl.floats * 4 : 0;
 }
 
 bool cache_attn_fits(const CacheAttnParams& p) {

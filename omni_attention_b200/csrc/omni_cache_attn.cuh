@@ -45,7 +45,7 @@ struct CacheLaunch {
 };
 
 cudaError_t launch_cache_attn(int head_dim, bool bf16, const CacheAttnParams& p, cudaStream_t stream);
-long long cache_attn_workspace_bytes(int B, int H, int Hkv, int T, int head_dim, bool prefix);
+long long cache_attn_workspace_bytes(int B, int H, int Hkv, int T, int head_dim, bool prefix, long long capacity);
 
 // Tensor maps of k_pages and v_pages (omni_abi.cu): the pages as a matrix of rows, one box = 64 columns of
 // min(page_size, 128) tokens of one page and head.

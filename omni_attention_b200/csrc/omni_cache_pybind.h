@@ -353,13 +353,15 @@ pybind11::object cache_attention(torch::Tensor q, const torch::Tensor& k_pages, 
     out = at::empty(q.sizes(), q.options());
     if (want_lse) lse = at::empty({B, H, T}, q.options().dtype(torch::kFloat32));
     const long long need = library.cache_attention_workspace(static_cast<int>(B), static_cast<int>(H), cache.heads, static_cast<int>(T),
-                                                             static_cast<int>(D), shared_prefix > 0);
-    auto workspace = at::empty({need}, q.options().dtype(torch::kUInt8));
+                                                             static_cast<int>(D), shared_prefix > 0,
+                                                             static_cast<long long>(cache.max_pages) * cache.page_size);
+    torch::Tensor workspace;
+    if (need > 0) workspace = at::empty({need}, q.options().dtype(torch::kUInt8));
     const omni_attn_heads hq = heads_arg(q);
     const int rc = library.cache_attention(&hq, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, &cache, counts_ptr, limits_ptr,
                                            causal ? 1 : 0, static_cast<int>(B), static_cast<int>(T), static_cast<int>(D), dtype_code(q),
                                            static_cast<float>(scale), static_cast<float>(softcap > 0 ? softcap : 0.0),
-                                           static_cast<int>(shared_prefix), workspace.data_ptr(), need,
+                                           static_cast<int>(shared_prefix), need > 0 ? workspace.data_ptr() : nullptr, need,
                                            at::cuda::getCurrentCUDAStream().stream(), status_ptr);
     if (rc != OMNI_OK) refuse_rc(rc);
   }

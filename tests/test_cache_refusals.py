@@ -218,12 +218,16 @@ def test_c_entries_return_codes():
     assert append(k=None) == append(v=None) == append(q=heads()) == E["OMNI_ERR_NULL_POINTER"]
     assert append(heads=3) == E["OMNI_ERR_CACHE"]
     assert append(rot=Rotary(A, 65)) == E["OMNI_ERR_ROTARY"]
-    assert attend(q=None) == attend(out=None) == attend(ws=None) == E["OMNI_ERR_NULL_POINTER"]
+    assert attend(q=None) == attend(out=None) == attend(ws=None, size=0, max_pages=100) == attend(ws=None, prefix=16) == E["OMNI_ERR_NULL_POINTER"]
     assert attend(heads=3) == attend(heads=0) == E["OMNI_ERR_CACHE"]
     assert attend(q=heads(A + 2, 4)) == attend(q=heads(A, 4, 65)) == attend(out=A + 8) == attend(k=A + 2) == E["OMNI_ERR_ALIGNMENT"]
     assert attend(softcap=-1.0) == attend(softcap=float("nan")) == attend(softcap=float("inf")) == E["OMNI_ERR_SOFTCAP"]
     assert attend(prefix=-1) == attend(prefix=80) == E["OMNI_ERR_SEQLEN"]
-    assert attend(size=100) == E["OMNI_ERR_WORKSPACE"]
+    assert attend(size=100, max_pages=100) == E["OMNI_ERR_WORKSPACE"]
+    size = lib.omni_attn_cache_attention_workspace_bytes
+    size.restype = L
+    assert size(1, 4, 2, 1, 64, 0, L(64)) == 0 and size(1, 4, 2, 1, 64, 0, L(1600)) > 0 and size(1, 4, 2, 1, 64, 16, L(64)) > 0
+    assert size(1, 3, 2, 1, 64, 0, L(1600)) == size(0, 2, 2, 1, 64, 0, L(1600)) == 0
     assert attend(T=2 ** 30) == E["OMNI_ERR_SHAPE"]
     for name in ("OMNI_ERR_ROTARY", "OMNI_ERR_CACHE"):
         lib.omni_attn_error_string.restype = ctypes.c_char_p
