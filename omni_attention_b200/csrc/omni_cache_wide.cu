@@ -221,10 +221,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         for (int h = 0; h < 2; ++h) {
           float s[64];
           load_scores64(tS + 64 * h, s);
-          if constexpr (SOFTCAP) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) s[j] = cap_out * tanhf(s[j] * cap_in);
-          }
+          if constexpr (SOFTCAP) soft_cap_scores(s, cap_in, cap_out);
           if (masked) apply_allow64(allow[2 * h], allow[2 * h + 1], s);
           if constexpr (SOFTCAP) {
             uint32_t w[32];

@@ -415,10 +415,11 @@ __device__ __forceinline__ float absmax3(float a, float b, float c) {
   return d;
 }
 
-__device__ __forceinline__ void soft_cap_scores(float (&s)[128], float cap_in, float cap_out) {
+template <int N>   // scores at hand
+__device__ __forceinline__ void soft_cap_scores(float (&s)[N], float cap_in, float cap_out) {
   float a = 0.f, b = 0.f;
 #pragma unroll
-  for (int j = 0; j < 128; j += 4) {
+  for (int j = 0; j < N; j += 4) {
     a = absmax3(a, s[j], s[j + 1]);
     b = absmax3(b, s[j + 2], s[j + 3]);
   }
@@ -429,7 +430,7 @@ __device__ __forceinline__ void soft_cap_scores(float (&s)[128], float cap_in, f
     const float b1 = (-1.f / 3.f) * c2, b2 = (2.f / 15.f) * c2 * c2, b3 = (-17.f / 315.f) * c2 * c2 * c2;
     const float2 b1v = make_float2(b1, b1), b2v = make_float2(b2, b2), b3v = make_float2(b3, b3);
 #pragma unroll
-    for (int j = 0; j < 128; j += 2) {
+    for (int j = 0; j < N; j += 2) {
       const float2 x = make_float2(s[j], s[j + 1]);
       const float2 z = __fmul2_rn(x, x);
       float2 p = __ffma2_rn(z, b3v, b2v);
@@ -441,7 +442,7 @@ __device__ __forceinline__ void soft_cap_scores(float (&s)[128], float cap_in, f
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 128; ++j) s[j] = cap_out * tanh_exact(s[j] * cap_in);
+    for (int j = 0; j < N; ++j) s[j] = cap_out * tanh_exact(s[j] * cap_in);
   }
 }
 
