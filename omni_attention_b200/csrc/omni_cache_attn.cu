@@ -646,6 +646,7 @@ __global__ void __launch_bounds__(256) omni_cache_join_kernel(const __grid_const
 
 // The launches of a call: one over everything, or one over the prefix and one over the sequences' own keys where only one
 // of the two has more than 16 rows to a key/value head (the narrow kernel would read its keys once for every 16 rows).
+// 8 sequences of 4K keys, 8 key/value heads of 128: 16 rows 29.7 us here and 34.4 on 128-row tiles, 32 rows 38.4 and 34.4.
 struct Plan {
   CacheLaunch of[2];   // the prefix's, the sequences'; equal if one launch has both
   bool join;

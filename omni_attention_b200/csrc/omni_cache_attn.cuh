@@ -38,8 +38,8 @@ struct CacheLaunch {
   int prefix, own;              // which segments
   int rt_prefix, rt_own;        // row tiles of the prefix (0 without it), of a sequence
   unsigned per_cta;             // triples / ctas, rounded up
-  unsigned uncut;               // see Line::uncut
-  unsigned even;                // CTAs for each triple, if there are that many (see Line::even)
+  unsigned uncut;               // kUncutTiles or kUncutTilesPrefix
+  unsigned even;                // CTAs for each triple, if there are that many (Line::even)
   int late_wait;                // 0: waits for its predecessor before it reads anything; 1: only before it ends
   long long share0;             // its shares in the workspace, in floats
 };
@@ -54,16 +54,17 @@ cudaError_t make_page_maps(const CacheAttnParams& p, int head_dim, bool bf16, CU
 constexpr int kTileKeys = 128;     // of both kernels
 constexpr int kNarrowRows = 16, kWideRows = 128;   // most rows of the narrow kernel's tile: 8 or 16
 constexpr int kCacheCtas = 148;    // one CTA per SM
-// What cutting costs, in tiles of keys: the shares' way through memory and the kernel that joins them.
-constexpr int kUncutTiles = 6, kUncutTilesPrefix = 1;   // with a prefix they are joined in any case
+// What cutting costs, in tiles of keys: the shares' way through memory and the kernel that joins them (with a prefix they are
+// joined in any case). 8 triples of 3 tiles: uncut 7.0 us, cut 7.3; of 5 tiles 8.7 and 7.9; of 16 tiles 16.5 and 11.4.
+constexpr int kUncutTiles = 2, kUncutTilesPrefix = 0;
+// What a second piece costs a CTA, in tiles: its queries, the first tile's way through the chain, the join of its shares.
+// 40 triples of 64 tiles on 148 CTAs: in even spans 34.8 us, three CTAs for each triple 32.8.
+constexpr int kPieceTiles = 4;
 // Tiles of 128 rows on the tcgen05 tensor cores (omni_cache_wide.cu).
 cudaError_t launch_cache_wide(int head_dim, bool bf16, const CUtensorMap& tmK, const CUtensorMap& tmV, const CacheAttnParams& p,
                               const CacheLaunch& how, cudaStream_t stream);
 // Whether the call's line of units can be counted in 31 bits.
 bool cache_attn_fits(const CacheAttnParams& p);
-
-// What a second piece costs a CTA, in tiles: its queries, the first tile's way through the chain, the join of its shares.
-constexpr int kPieceTiles = 4;
 
 // A programmatic dependent launch: may start before its predecessor on the stream has ended (omni_cache_line.cuh: grid_wait).
 template <typename... P, typename... A>

@@ -36,12 +36,11 @@ struct Line {
   int prefix_seq;           // the sequence whose page table the prefix is read through: the longest
   int prefix_end;
   int rt_prefix, rt_own;
-  // A triple is one unit, none is cut and nothing has to be joined: where the CTA with most to do then has at most how.uncut
-  // tiles of keys more than an even cut would give it.
+  // The busiest CTA's tiles of keys decide how the line is cut. uncut: a triple is one unit, none is cut and nothing has to
+  // be joined (cutting costs how.uncut tiles); even: each triple is cut into that many parts by itself, one per CTA; else
+  // even spans of the whole line, where a CTA may have two pieces (kPieceTiles).
   bool uncut;
-  // Or each triple is cut into this many parts by itself, one per CTA (0: not so): where that makes no CTA's part longer than
-  // an even cut's by more than a CTA's second piece would cost it.
-  unsigned even;
+  unsigned even;   // 0: not so
 
   __device__ __forceinline__ unsigned part(unsigned units) const { return (units + even - 1) / even; }
   __device__ __forceinline__ unsigned parts(unsigned units) const {
@@ -87,12 +86,10 @@ __device__ __forceinline__ Line make_line(const CacheAttnParams& p, const CacheL
   const unsigned heads = p.Hkv, rt_own = how.own ? ln.rt_own : 0;
   const unsigned cut_units = heads * (ln.rt_prefix * tiles_prefix + rt_own * sum), cut_span = (cut_units + how.ctas - 1) / how.ctas;
   const unsigned triples = heads * (ln.rt_prefix + rt_own * p.B), per_cta = how.per_cta;
-  ln.uncut = static_cast<unsigned long long>(per_cta) * max(tiles_prefix, tiles_own) <= cut_span + how.uncut;
-  ln.even = 0;
-  if (!ln.uncut && how.even >= 2) {
-    const unsigned longest = max(tiles_prefix, tiles_own);
-    if ((longest + how.even - 1) / how.even <= cut_span + kPieceTiles) ln.even = how.even;
-  }
+  const unsigned longest = max(tiles_prefix, tiles_own), even = how.even >= 2 ? (longest + how.even - 1) / how.even : 0xFFFFFFFFu;
+  const unsigned cut = min(even, cut_span + kPieceTiles);
+  ln.uncut = static_cast<unsigned long long>(per_cta) * longest <= cut + how.uncut;
+  ln.even = !ln.uncut && even == cut ? how.even : 0u;
   ln.prefix_units = how.prefix ? heads * ln.rt_prefix * ln.units_between(0, ln.prefix_end) : 0u;
   ln.units = ln.uncut ? triples : cut_units;
   ln.span = ln.uncut ? per_cta : cut_span;
