@@ -252,7 +252,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       for (int j = 0; j < 2 * NT; ++j) {
         const int r = 8 * (j >> 1) + 2 * pos + (j & 1);
         lim[j] = in.lim[r];
-        if (r < rows) lim_min = min(lim_min, lim[j]);
+        if (r < rows && lim[j] > 0) lim_min = min(lim_min, lim[j]);   // rows that see nothing are zeroed at the end
       }
       lim_min = __reduce_min_sync(0xFFFFFFFFu, lim_min);
       uint32_t qf[KS][2 * NT];   // Q^T, two steps to an ldmatrix for 8 rows, one for 16
@@ -389,12 +389,52 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float a = ex2_approx(s[j][2 * h] - at0), b = ex2_approx(s[j][2 * h + 1] - at1);
+              s[j][2 * h] = a;
+              s[j][2 * h + 1] = b;
               l[2 * j] += a;
               l[2 * j + 1] += b;
               const uint32_t w = pack16<BF16>(a, b);
               const float2 v = unpack16<BF16>(w);
               hi[j][h] = movmatrix(w);
               lo[j][h] = movmatrix(pack16<BF16>(a - v.x, b - v.y));
+            }
+          }
+          if (key + 16 > lim_min && lim_min < lim_max) {
+            // A value that is infinite or NaN must not reach the rows that do not see its key (0 * NaN): such a key's share is
+            // added here, row by row, and its V is zero in the product. Only where rows of the tile see different numbers of keys.
+            bool bad = false;
+            const uint8_t* v_tile = smem + slot * (2 * Cfg::kTile) + Cfg::kTile;
+#pragma unroll 1
+            for (int c = lane >> 4; c < Cfg::kChunks * 8; c += 2) {
+              bad |= not_finite<BF16>(*reinterpret_cast<const uint4*>(v_tile + swizzled(warp * 16 + (lane & 15), c, 128 * 128)));
+            }
+            uint32_t keys = __ballot_sync(0xFFFFFFFFu, bad);
+            keys = (keys | keys >> 16) & 0xFFFFu;
+#pragma unroll 1
+            for (; keys != 0; keys &= keys - 1) {
+              const int r = __ffs(keys) - 1, row = warp * 16 + r;
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                const int from = (r & 7) * 4 + pos;
+                const float p_lo0 = __shfl_sync(0xFFFFFFFFu, s[j][0], from), p_hi0 = __shfl_sync(0xFFFFFFFFu, s[j][2], from);
+                const float p_lo1 = __shfl_sync(0xFFFFFFFFu, s[j][1], from), p_hi1 = __shfl_sync(0xFFFFFFFFu, s[j][3], from);
+                const float p0 = r < 8 ? p_lo0 : p_hi0, p1 = r < 8 ? p_lo1 : p_hi1;
+                const bool sees0 = key + r < lim[2 * j], sees1 = key + r < lim[2 * j + 1];
+#pragma unroll
+                for (int d = 0; d < KS; ++d) {
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const uint32_t raw = *reinterpret_cast<const uint16_t*>(v_tile + swizzled(row, 2 * d + h, 128 * 128) + 2 * quad);
+                    const float v = unpack16<BF16>(raw).x;
+                    if (sees0) o_acc[d][j][2 * h] += p0 * v;
+                    if (sees1) o_acc[d][j][2 * h + 1] += p1 * v;
+                  }
+                }
+              }
+              __syncwarp();
+              if (lane < Cfg::kChunks * 8) *reinterpret_cast<uint4*>(const_cast<uint8_t*>(v_tile) + swizzled(row, lane, 128 * 128)) = make_uint4(0u, 0u, 0u, 0u);
+              fence_async_smem();
+              __syncwarp();
             }
           }
 #pragma unroll
@@ -428,6 +468,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       constexpr int P = C + 4;                                           // pitch of a row
       const int r = threadIdx.x / TR;                                    // the row this thread finishes
       const long long at_row = in.out[r];
+      const bool sees = in.lim[r] > 0;
       float f[kWarps], top = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int round = 0; round < D / C; ++round) {
@@ -453,6 +494,10 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             f[w] = ex2_approx(s_m[w * kNarrowRows + r] - at);
             sum += f[w] * s_l[w * kNarrowRows + r];
           }
+          if (!sees) {
+            top = -INFINITY;
+            sum = 0.f;
+          }
         }
         const int in_round = (threadIdx.x % TR) * V, col = round * C + in_round;
         if (r < rows && col < d_real) {
@@ -467,7 +512,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           if (share >= 0) {
             float* to = share_at(p, how, share, d_real) + r * d_real + col;
 #pragma unroll
-            for (int i = 0; i < V; ++i) to[i] = acc[i];
+            for (int i = 0; i < V; ++i) to[i] = sees ? acc[i] : 0.f;
           } else {
             const bool any = !(sum == 0.f);   // NaN shows
             const float inv = 1.f / sum;

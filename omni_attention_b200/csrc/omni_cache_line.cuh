@@ -240,6 +240,17 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm,
                : "memory");
 }
 
+// Whether one of the eight 16-bit values is infinite or NaN.
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(const uint4& v) {
+  constexpr uint32_t m = BF16 ? 0x7F80u : 0x7C00u;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (w[i] & m) == m || (w[i] & (m << 16)) == m << 16;
+  return bad;
+}
+
 // Programmatic dependent launch: a kernel so launched may start before its predecessor has ended; what that one wrote is
 // there behind grid_wait. grid_go lets a successor start. Both are no-ops without such launches.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -16,6 +16,10 @@
 // Hand-overs go through mbarriers; every wait is bounded as in the forward kernels. TMEM: S of the two groups (P, 16 bit,
 // over the first half of S), O of the two groups.
 //
+// A value that is infinite or NaN must not reach the rows that do not see its key (0 * NaN): where rows of a tile see
+// different numbers of keys such a key's V is zeroed too, and its share is added to the rows that see it when the piece is
+// written (add_not_finite).
+//
 // Keys that are not there - behind the last token, in a page that does not exist - are never loaded; what the ring holds in
 // their places is zeroed in V (0 * NaN) and masked in S.
 #include "omni_cache_line.cuh"
@@ -39,7 +43,8 @@ struct WideCfg {
   static constexpr int kChunk = 128 * 128;
   static constexpr int kSlots = D == 128 ? 6 : 10;   // K and V tiles in flight
   static constexpr int kBars = (1 + kSlots) * kTile;
-  static constexpr int kSmem = kBars + 3072;         // barriers, row states
+  static constexpr int kPiece = D == 128 ? 432 : 3072;   // where the piece's description is, behind the barriers
+  static constexpr int kSmem = kBars + (D == 128 ? 3072 : 3136);   // barriers, row states, description
 };
 
 // Named barrier of the eight softmax warps.
@@ -65,6 +70,52 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t addr, float (&f)[COLS]) {
   }
 }
 
+template <bool BF16>
+__device__ __forceinline__ float value16(uint16_t raw) {
+  return BF16 ? __uint_as_float(static_cast<uint32_t>(raw) << 16) : __half2float(__ushort_as_half(raw));
+}
+
+// Whether a row of a V tile (chunks of 128 bytes, `pitch` apart) has a value that is not finite.
+template <bool BF16, int CHUNKS>
+__device__ __noinline__ bool row_not_finite(uint32_t row, uint32_t pitch) {
+  bool bad = false;
+#pragma unroll 4
+  for (int c = 0; c < CHUNKS * 8; ++c) bad |= not_finite<BF16>(lds_v4(row + (c >> 3) * pitch + (c & 7) * 16));
+  return bad;
+}
+
+// What the product left out for one query row: keys [key_lo, key_hi) whose V is not finite, as far as the row sees them and a
+// page has them, columns [c0, c1). Everything from memory; `out` (16 bit, divided by the row's sum) or `share` (32 bit).
+template <bool BF16>
+__device__ __noinline__ void add_not_finite(const CacheAttnParams& p, const Piece& pc, const RowId& id, int key_lo, int key_hi, float top, float sum, int d,
+                                            int c0, int c1, float* share, uint16_t* out) {
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + id.b * p.qs_b + (static_cast<long long>(pc.hk) * p.G + id.g) * p.qs_h + id.t * p.qs_t;
+  for (int key = key_lo; key < key_hi; ++key) {
+    const int page = __ldg(p.page_table + pc.table_of * p.table_stride + (key >> p.page_shift));
+    if (page < 0 || page >= p.num_pages) continue;
+    const long long at = (((static_cast<long long>(page) * p.Hkv + pc.hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * d;
+    const uint16_t *k = static_cast<const uint16_t*>(p.k_pages) + at, *v = static_cast<const uint16_t*>(p.v_pages) + at;
+    bool bad = false;
+    for (int c = 0; c < d; c += 8) bad |= not_finite<BF16>(*reinterpret_cast<const uint4*>(v + c));
+    if (!bad) continue;
+    float s = 0.f;
+    for (int c = 0; c < d; ++c) s += value16<BF16>(q[c]) * value16<BF16>(k[c]);
+    s *= p.scale;
+    if (p.softcap > 0.f) s = tanhf(s / p.softcap) * p.softcap;
+    float w = ex2_approx(s * 1.4426950408889634f - (top == -INFINITY ? 0.f : top));
+    if (share == nullptr) w /= sum;
+    for (int c = c0; c < c1; ++c) {
+      const float x = w * value16<BF16>(v[c]);
+      if (share != nullptr) {
+        share[c] += x;
+      } else {
+        const uint32_t both = pack2<BF16>(value16<BF16>(out[c]) + x, 0.f);
+        out[c] = static_cast<uint16_t>(both);
+      }
+    }
+  }
+}
+
 template <int D, bool BF16, bool SOFTCAP>
 __global__ void __launch_bounds__(kWideThreads, 1)
 omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -87,6 +138,9 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kBars + 256);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_lim = reinterpret_cast<int*>(tmem_slot + 2);                                    // [8] largest limit of a warp's rows, [8] smallest
+  Piece* s_piece = reinterpret_cast<Piece*>(smem + Cfg::kBars + Cfg::kPiece);
+  static_assert(sizeof(Piece) <= 64 && 336 + 16 * Cfg::kSlots <= (D == 128 ? Cfg::kPiece : 512), "shared memory layout");
+  volatile int* s_bad = s_lim + 16;                                                       // a V that is not finite was left out
   uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + Cfg::kBars + 336);      // [kSlots] keys that are there
   float* s_m = reinterpret_cast<float*>(smem + Cfg::kBars + 512);                         // [2][128]
   float* s_l = s_m + 256;                                                                 // [2][128]
@@ -107,6 +161,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     }
     mbar_init(bar_end, 1);
     *abort_flag = 0;
+    *s_bad = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -137,7 +192,11 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     const float cap_in = SOFTCAP ? p.scale / p.softcap : 0.f, cap_out = SOFTCAP ? p.softcap / p.scale : 0.f;
     uint32_t n_vis = 0, n_pieces = 0;   // this group's visits and pieces with visits so far = phases of its barriers
     uint32_t fill = 0;                  // ring entries of the pieces before this one
-    while (walk.next(p, pc)) {
+    // The walk is kept in local memory here: it is wanted once a piece, and its twenty registers throughout (spills in the
+    // loop otherwise: 527 -> 590 us for 32 heads of 4096 rows on 4K keys).
+    Walk own_walk = walk;
+    asm volatile("" ::"l"(&own_walk) : "memory");
+    while (own_walk.next(p, pc)) {
       const int n = pc.tile1 - pc.tile0;
       // ---- the rows' queries: thread (row tid / 2, half of its chunks). (Two warps of their own with cp.async took longer:
       // their copies stood behind the other warps' polls, 700 cycles each.) ----
@@ -170,11 +229,12 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         lim = min(limit_of(p, id.b, id.t), pc.total);
         if (g == 0) s_out[r] = static_cast<int>(out_row(p, id, pc.hk));
       }
-      const int warp_max = __reduce_max_sync(0xFFFFFFFFu, lim), warp_min = __reduce_min_sync(0xFFFFFFFFu, r < rows ? lim : 0x7FFFFFFF);
+      const int warp_max = __reduce_max_sync(0xFFFFFFFFu, lim), warp_min = __reduce_min_sync(0xFFFFFFFFu, lim > 0 ? lim : 0x7FFFFFFF);   // (rows that see nothing are zeroed at the end)
       if (lane == 0) {
         s_lim[warp] = warp_max;
         s_lim[8 + warp] = warp_min;
       }
+      if (tid == 0) *s_piece = pc;   // for the piece's end: its registers are wanted in between
       named_barrier_sync(2 + g, 128);
       int lim_max = s_lim[4 * g], lim_min = s_lim[8 + 4 * g];
 #pragma unroll
@@ -183,11 +243,12 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         lim_min = min(lim_min, s_lim[8 + 4 * g + w]);
       }
 
+      const int key_first = pc.key0 + pc.tile0 * kTileKeys;
       RowState st{-INFINITY, 0.f};
       int mine = 0;   // visits of this group in this piece
       for (int i = g; i < n; i += 2, ++mine, ++n_vis) {
         const uint32_t vs = (fill + 2 * i + 1) % Cfg::kSlots;   // V's place in the ring
-        const int key = pc.key0 + (pc.tile0 + i) * kTileKeys;
+        const int key = key_first + i * kTileKeys;
         if (lane == 0) {
           mbar_wait_lim(bar_s + 8 * g, n_vis & 1, abort_flag, p.status, 40 + g, limit);
           mbar_wait_lim(bar_full + 8 * vs, ((fill + 2 * i + 1) / Cfg::kSlots) & 1, abort_flag, p.status, 42, limit);
@@ -205,7 +266,12 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           for (int w = 0; w < 4; ++w) allow[w] = valid[w] & low_bits(lim - key - 32 * w);
           const int quarter = warp & 3;   // key r of the tile is in word r / 32
           const uint32_t word = quarter == 0 ? valid[0] : quarter == 1 ? valid[1] : quarter == 2 ? valid[2] : valid[3];
-          if (!(word >> lane & 1u)) {     // not there, or no row sees it: zero its V
+          bool drop = !(word >> lane & 1u);   // not there, or no row sees it: zero its V
+          if (!drop && key + r >= lim_min) {  // not every row sees it
+            drop = row_not_finite<BF16, Cfg::kChunks>(sRing + Cfg::kTile * vs + r * 128, Cfg::kChunk);
+            if (drop) *s_bad = 1;
+          }
+          if (drop) {
 #pragma unroll
             for (int c = 0; c < Cfg::kChunks; ++c) {
               uint4* at = reinterpret_cast<uint4*>(smem + Cfg::kTile * (1 + vs) + c * Cfg::kChunk + r * 128);
@@ -270,12 +336,15 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       s_m[128 * g + r] = st.M;
       s_l[128 * g + r] = st.l;
       softmax_sync();   // (also: every score of the piece is read, its queries are not needed any more)
+      const bool left_out = *s_bad != 0;
       const float mo = s_m[128 * (1 - g) + r], lo = s_l[128 * (1 - g) + r];
-      const float top = fmaxf(st.M, mo), at = top == -INFINITY ? 0.f : top;
+      const float top = lim > 0 ? fmaxf(st.M, mo) : -INFINITY, at = top == -INFINITY ? 0.f : top;
       float f = ex2_approx(st.M - at);
-      const float sum = st.l * f + lo * ex2_approx(mo - at);
+      const float sum = lim > 0 ? st.l * f + lo * ex2_approx(mo - at) : 0.f;
       const bool any = !(sum == 0.f);   // NaN shows
-      float* share = pc.share >= 0 ? share_at(p, how, pc.share, d_real) : nullptr;
+      const long long share_no = *reinterpret_cast<volatile long long*>(&s_piece->share);
+      float* share = share_no >= 0 ? share_at(p, how, share_no, d_real) : nullptr;
+      const int rows_here = min(kWideRows, *reinterpret_cast<volatile int*>(&s_piece->rows) - *reinterpret_cast<volatile int*>(&s_piece->rt) * kWideRows);
       if (share == nullptr) f *= 1.f / sum;
       const bool have = mine > 0 && any;
       constexpr int C = D / 4, Q4 = C / 4;   // columns of a round, 16-byte pieces of a row
@@ -290,10 +359,11 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
               have ? make_float4(o[4 * j] * f, o[4 * j + 1] * f, o[4 * j + 2] * f, o[4 * j + 3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         softmax_sync();
+        if (tid == 0) *s_bad = 0;   // everyone has read it, nobody sets it before the next piece
 #pragma unroll
         for (int i = 0; i < 128 * Q4 / 256; ++i) {
           const int item = tid + 256 * i, rr = item / Q4, j = item % Q4;
-          if (rr < rows) {
+          if (rr < rows_here) {
             const float4 a = xchg[rr * Q4 + (j ^ (rr & (Q4 - 1)))], b = xchg[(128 + rr) * Q4 + (j ^ (rr & (Q4 - 1)))];
             const float4 v = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
             if (share != nullptr) {
@@ -306,7 +376,18 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         }
         softmax_sync();   // the next round, or the next piece's queries, go over what was read
       }
-      if (r < rows && g == 0) {
+      if (left_out) {   // what is written is there for all of the softmax threads behind the barrier above
+        const Piece whole = *s_piece;
+        const int key_lo = max(lim_min, key_first), key_hi = min(lim, whole.key0 + whole.tile1 * kTileKeys);
+        const int half = d_real / 2;
+        if (r < rows_here) {
+          add_not_finite<BF16>(p, whole, row_of(p, whole.prefix, whole.seg, whole.rt * kWideRows + r), key_lo, key_hi, top, sum, d_real, g * half, (g + 1) * half,
+                               share != nullptr ? share + r * d_real : nullptr,
+                               static_cast<uint16_t*>(p.out) + static_cast<long long>(s_out[r]) * d_real);
+        }
+        softmax_sync();
+      }
+      if (r < rows_here && g == 0) {
         if (share != nullptr) {
           share[kWideRows * d_real + r] = top;
           share[kWideRows * d_real + kWideRows + r] = sum;

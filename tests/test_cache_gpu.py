@@ -158,6 +158,37 @@ def test_lengths_at_the_ends(cuda_device):
     run(q, kp, vp, table, lens, "ends", causal=False)
 
 
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("H,T,lengths", [(4, 6, [40, 300]), (2, 4, [0, 17]), (8, 30, [100, 2100]), (4, 130, [0, 500])])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(cuda_device, value, H, T, lengths):
+    """Keys and values of new tokens that are infinite or NaN: rows before them are as if they were not there."""
+    B, Hkv, D, page = 2, 2, 64, 16
+    for dtype in (torch.float16, torch.bfloat16):
+        kp, vp, table, lens, g = make_cache(B, Hkv, D, page, lengths, T, dtype, seed=5)
+        q = torch.randn(B, H, T, D, generator=g).to(dtype)
+        at = T // 2
+        kp2, vp2 = kp.clone(), vp.clone()
+        for b in range(B):
+            for t in (at, T - 1):
+                i = lengths[b] + t
+                p, row = int(table[b, i // page]), i % page
+                vp2[p, :, row, 5] = value
+                if t == T - 1:
+                    kp2[p, :, row] = math.nan
+                    vp2[p, :, row] = value
+        clean = omni.omni_cache_attention(q.cuda(), on_gpu(kp, vp, table, lens))
+        got = omni.omni_cache_attention(q.cuda(), on_gpu(kp2, vp2, table, lens))
+        assert torch.equal(got[:, :, :at], clean[:, :, :at]), "rows that do not see it"
+        seen = got[:, :, at:T - 1].double().cpu()
+        rest = [c for c in range(D) if c != 5]
+        assert not torch.isfinite(seen[..., 5]).any(), "rows that see it, its column"
+        want, _, size = orc.attention(q, kp, vp, table, lens)
+        # the other columns are the product's and one more addition, rounded once more
+        tol = torch.finfo(dtype).eps * (size[:, :, at:T - 1] + want[:, :, at:T - 1].abs()) + 1e-3
+        assert ((seen - want[:, :, at:T - 1]).abs() <= tol)[..., rest].all()
+        assert not torch.isfinite(got[:, :, T - 1]).any()
+
+
 @pytest.mark.parametrize("bad", [-1, 10 ** 6, -2 ** 31, 2 ** 31 - 1])
 @pytest.mark.parametrize("heads", [4, 48])
 def test_pages_that_are_not_there(cuda_device, bad, heads):
