@@ -453,3 +453,102 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(cuda_device
     finally:
         lib.omni_attn_set_wait_cycles(0)       # back to the default budget
     assert torch.equal(omni.omni_cache_attention(q, cache, check_status=True), want)
+
+
+@pytest.mark.parametrize("H,prefix", [(8, 0), (64, 0), (8, 1024)])
+def test_graphs_side_by_side(cuda_device, H, prefix):
+    """Two captured calls replayed at once on two streams: each has a workspace of its own."""
+    kp, vp, table, lens, g = make_cache(4, 2, 128, 64, [6000, 1100, 3000, 1024], 1, torch.bfloat16, shared=prefix)
+    cache = on_gpu(kp, vp, table, lens)
+    qs = [torch.randn(4, H, 1, 128, generator=g).bfloat16().cuda() for _ in range(2)]
+    want = [omni.omni_cache_attention(q, cache, shared_prefix=prefix) for q in qs]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for q in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(omni.omni_cache_attention(q, cache, shared_prefix=prefix))
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_a_captured_step_among_copies_and_other_streams(cuda_device):
+    """A captured step whose kernels stand behind copies, another stream's work and each other, as launches that may begin
+    before their predecessor ends do: the values are those of the same calls with a wait after each."""
+    B, H, Hkv, D, page, T = 3, 4, 2, 64, 16, 2
+    kp, vp, table, lens, g = make_cache(B, Hkv, D, page, [1500, 40, 700], T, torch.float16)
+    rot = omni.OmniRotary.from_base(D, device="cuda")
+    src = [torch.randn(B, h, T, D, generator=g).half().cuda() for h in (H, Hkv, Hkv)]
+    weight = (1 + 0.1 * torch.randn(D, generator=g)).cuda()
+
+    def step(cache, x, wait=lambda: None, side=None):
+        q, k, v = (t.clone() for t in x)                       # copies
+        wait()
+        if side is not None:                                   # keys from another stream
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                k = k * 2
+            torch.cuda.current_stream().wait_stream(side)
+        else:
+            k = k * 2
+        wait()
+        q, _ = omni.omni_rotary(q, None, None, None, weight)
+        wait()
+        q = omni.omni_cache_append(cache, k, v, q, rot)
+        wait()
+        out, lse = omni.omni_cache_attention(q, cache, return_lse=True)
+        wait()
+        again = omni.omni_cache_attention(q, cache, shared_prefix=0, causal=False)
+        wait()
+        q2, _ = omni.omni_rotary(out, None, rot)
+        wait()
+        return out, lse, again, q2
+
+    plain = on_gpu(kp, vp, table, lens)
+    want = step(plain, src, torch.cuda.synchronize)
+    cache, side = on_gpu(kp, vp, table, lens), torch.cuda.Stream()
+    inp = [torch.zeros_like(t) for t in src]
+    step(cache, inp)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(cache, inp, side=side)
+    for dst, x in zip(inp, src):
+        dst.copy_(x)
+    for _ in range(10):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert torch.equal(cache.k_pages.view(torch.int16), plain.k_pages.view(torch.int16))
+    for a, b in zip(step(cache, src), want):                   # and without a graph
+        assert torch.equal(a, b)
+
+
+def test_host_threads_on_one_stream(cuda_device):
+    """Calls that threads enqueue onto one stream, in whatever order their launches interleave."""
+    import threading
+
+    kp, vp, table, lens, g = make_cache(4, 2, 128, 64, [3000, 100, 2100, 1024], 1, torch.bfloat16, shared=64)
+    cache = on_gpu(kp, vp, table, lens)
+    calls = []
+    for H, prefix in ((8, 0), (64, 0), (8, 64), (32, 64)):
+        q = torch.randn(4, H, 1, 128, generator=g).bfloat16().cuda()
+        calls.append((q, prefix, omni.omni_cache_attention(q, cache, shared_prefix=prefix)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(q, prefix, want):
+        outs = [omni.omni_cache_attention(q, cache, shared_prefix=prefix) for _ in range(40)]
+        torch.cuda.current_stream().synchronize()
+        wrong.extend(1 for o in outs if not torch.equal(o, want))
+
+    threads = [threading.Thread(target=work, args=c) for c in calls]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
