@@ -6,13 +6,14 @@
 // (2 800 cycles), its two products 1 024; from 256 rows on the second row tile finds the keys in L2 and the chain scores ->
 // softmax -> P -> product bounds it. So the tiles of keys go to two softmax groups in turn, each with its own scores,
 // maximum, sum and O, and one group's chain runs under the other's products; at the end of a piece the groups' halves are
-// joined through shared memory.
+// joined through shared memory. Measured, head_dim 128, bf16: 2 x 32 heads of 256 rows on 4 352 keys 53 us = 690 TFLOP/s (67 with
+// the soft-cap), 1 900 cycles a tile; the 16 384 shared tokens of 64 sequences, 8 key/value heads, 31 us.
 //
 // Roles of a CTA (one per SM, 384 threads):
 //   warps 0-3, 4-7  softmax groups: thread = query row = TMEM lane. They also gather the rows' queries into shared memory
 //                   (any strides, rows of one tile may belong to different sequences) and write the result.
 //   warp 8          TMA: K and V of each tile of keys page by page into a ring (lane = page of the tile)
-//   warp 9          one elected thread issues every tcgen05.mma; warps 10 and 11 only give their registers up
+//   warp 9          one elected thread issues every tcgen05.mma (warps 10 and 11 only give their registers up)
 // Hand-overs go through mbarriers; every wait is bounded as in the forward kernels. TMEM: S of the two groups (P, 16 bit,
 // over the first half of S), O of the two groups.
 //
