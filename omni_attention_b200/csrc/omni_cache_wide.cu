@@ -194,7 +194,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     uint32_t n_vis = 0, n_pieces = 0;   // this group's visits and pieces with visits so far = phases of its barriers
     uint32_t fill = 0;                  // ring entries of the pieces before this one
     // The walk is kept in local memory here: it is wanted once a piece, and its twenty registers throughout (spills in the
-    // loop otherwise: 527 -> 590 us for 32 heads of 4096 rows on 4K keys).
+    // loop otherwise: 532 -> 577 us for 32 heads of 4096 rows on 4K keys).
     Walk own_walk = walk;
     asm volatile("" ::"l"(&own_walk) : "memory");
     while (own_walk.next(p, pc)) {
