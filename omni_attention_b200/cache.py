@@ -115,11 +115,13 @@ def omni_cache_attention(q: Tensor, cache: OmniPagedCache, counts: Optional[Tens
     q [B, H, T, D]; H a multiple of the cache's heads (query head h reads key/value head h // (H / Hkv)). Row t of sequence
     b attends its first ``cache.lengths[b] + t + 1`` tokens, with ``causal=False`` all ``cache.lengths[b] + counts[b]`` of
     them, with ``limits`` (int32 [B, T]) its first ``limits[b, t]``. Rows behind a sequence's count (``counts`` int32 [B],
-    None = T) and rows with no key are zero (LSE -inf). ``scale`` defaults to D ** -0.5, ``softcap`` > 0 caps the scaled
+    None = T) and rows with no key are zero (LSE -inf). ``scale`` (positive) defaults to D ** -0.5, ``softcap`` > 0 caps the scaled
     scores with tanh. ``shared_prefix``: that many first tokens of all sequences are in the same pages (a prompt with
     several continuations): they are read once for the whole batch. Keys in pages that are not there are left out;
     ``check_status=True`` waits for the GPU and raises then, also when ``shared_prefix`` tokens are not in the same pages.
     Returns out [B, H, T, D] (and lse [B, H, T], natural log, with ``return_lse``). No gradients."""
+    if scale is not None and not scale >= torch.finfo(torch.float32).tiny:
+        raise OmniAttnError(f"scale must be finite and positive (not zero, negative or NaN), got {scale}")
     status = _status(check_status, q.device)
     res = load_extension().cache_attention(q, cache.k_pages, cache.v_pages, cache.page_table, cache.lengths, counts, causal,
                                            limits, scale or 0.0, softcap or 0.0, return_lse, shared_prefix, status)

@@ -80,8 +80,8 @@ void check_rotary_args(const RotaryArgs& r, const torch::Tensor& q, const torch:
     OMNI_REQUIRE((p.dim() == 1 && p.size(0) == x.size(2)) || (p.dim() == 2 && (p.size(0) == x.size(0) || p.size(0) == 1) && p.size(1) == x.size(2)),
             "positions must be [N], [1, N] or [B, N], got " + shape_of(p));
   }
-  OMNI_REQUIRE(std::isfinite(r.factor), "the rotary factor must be finite");
-  OMNI_REQUIRE(r.eps >= 0.0 && std::isfinite(r.eps), "eps must be finite and not negative");
+  OMNI_REQUIRE(std::isfinite(static_cast<float>(r.factor)), "the rotary factor must be finite");
+  OMNI_REQUIRE(r.eps >= 0.0 && std::isfinite(static_cast<float>(r.eps)), "eps must be finite and not negative");
   if (r.q_weight.defined() && q.defined()) check_weight(r.q_weight, "q_weight", q);
   if (r.k_weight.defined() && k.defined()) check_weight(r.k_weight, "k_weight", k);
   OMNI_REQUIRE(!r.q_weight.defined() || q.defined(), "q_weight without q");
@@ -322,6 +322,10 @@ pybind11::object cache_append(const torch::Tensor& k_pages, const torch::Tensor&
                                         &a, static_cast<int>(B), static_cast<int>(N), static_cast<int>(D), dtype_code(k),
                                         at::cuda::getCurrentCUDAStream().stream(), status_ptr);
     if (rc != OMNI_OK) refuse_rc(rc);
+    // A backward that saved the pages before this write must not use them after it, as behind any operation in place.
+    for (const torch::Tensor* t : {&k_pages, &v_pages}) {
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    }
   }
   return result(q_out);
 }
@@ -339,7 +343,7 @@ pybind11::object cache_attention(torch::Tensor q, const torch::Tensor& k_pages, 
     const int32_t* counts_ptr = int32_or_null(counts, {B}, "counts must be contiguous int32 [B]");
     const int32_t* limits_ptr = int32_or_null(limits, {B, T}, "limits must be contiguous int32 [B, T]");
     int32_t* status_ptr = const_cast<int32_t*>(int32_or_null(status, {1}, "status must be int32 [1]"));
-    OMNI_REQUIRE(std::isfinite(scale) && std::isfinite(softcap) && scale >= 0.0, "scale and softcap must be finite, scale not negative");
+    OMNI_REQUIRE(std::isfinite(static_cast<float>(scale)) && std::isfinite(static_cast<float>(softcap)) && scale >= 0.0, "scale and softcap must be finite, scale not negative");
     OMNI_REQUIRE(shared_prefix >= 0 && shared_prefix <= table.size(1) * k_pages.size(2), "shared_prefix must be from 0 to the tokens that the page table holds");
     OMNI_REQUIRE(!wants_grad({&q, &k_pages, &v_pages}),
             "omni_cache_attention has no backward: call it under torch.no_grad(), or on tensors that need no gradient");

@@ -552,3 +552,22 @@ def test_host_threads_on_one_stream(cuda_device):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not wrong
+
+
+def test_a_backward_does_not_use_pages_written_since(cuda_device):
+    """Pages that an autograd graph saved and that are appended to before its backward: an error, as behind k_pages.add_(...)."""
+    c = omni.OmniPagedCache.allocate(4, 1, 16, 32, 1, 4, torch.float16, cuda_device)
+    c.page_table.copy_(torch.arange(4, dtype=torch.int32)[None])
+    new = torch.ones(1, 1, 3, 32, dtype=torch.float16, device=cuda_device)
+    for pages in (c.k_pages, c.v_pages):
+        x = torch.ones(32, dtype=torch.float16, device=cuda_device, requires_grad=True)
+        y = (pages * x).sum()
+        with torch.no_grad():
+            omni.omni_cache_append(c, new, new)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        c = omni.OmniPagedCache.allocate(4, 1, 16, 32, 1, 4, torch.float16, cuda_device)
+        c.page_table.copy_(torch.arange(4, dtype=torch.int32)[None])
+        omni.omni_cache_append(c, new, new)
+        assert torch.equal(c.k_pages[0, 0, :3], new[0, 0])

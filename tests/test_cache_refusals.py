@@ -145,6 +145,17 @@ def test_attention_call():
     refused("no backward", f, q.requires_grad_(), c)
 
 
+@pytest.mark.parametrize("value", [0.0, 1e-60, 1e60, float("inf")])
+def test_numbers_that_32_bits_do_not_hold(value):
+    c, q = cache(), t(2, 4, 3, 64)
+    refused("scale", omni.omni_cache_attention, q, c, scale=value)     # 0 must not turn into the default
+    if value > 1:
+        refused("finite", omni.omni_cache_attention, q, c, softcap=value)
+        refused("eps", omni.omni_rotary, q, None, None, q_weight=torch.ones(64), eps=value)
+        if value != float("inf"):
+            refused("factor", omni.omni_rotary, q, None, omni.OmniRotary(torch.ones(4, dtype=torch.float64), factor=value))
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the C entry points
 # ---------------------------------------------------------------------------------------------------------------------
