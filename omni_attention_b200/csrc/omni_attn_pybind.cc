@@ -12,6 +12,7 @@
 #include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/extension.h>
 
 #include <climits>

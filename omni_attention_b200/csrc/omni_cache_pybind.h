@@ -141,6 +141,27 @@ std::pair<torch::Tensor, torch::Tensor> rotate(const torch::Tensor& q, const tor
   return {q_out, k_out};
 }
 
+// A backward that is being captured, into leaves whose accumulators belong to the default stream (made by a graph outside the
+// capture that is still alive): autograd would make the default stream wait for the captured one, which fails inside its
+// engine and can end the process. Said here instead, while the capture is still sound.
+void refuse_leaves_outside_the_capture() {
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream().stream(), &capturing) != cudaSuccess) {
+    (void)cudaGetLastError();   // the launch will say it
+    return;
+  }
+  const auto node = torch::autograd::get_current_node();
+  if (!node || capturing == cudaStreamCaptureStatusNone) return;
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.function || dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) == nullptr) continue;
+    const auto stream = edge.function->stream();
+    if (stream && stream->device_type() == c10::DeviceType::CUDA && c10::cuda::CUDAStream(*stream).stream() == nullptr) {
+      refuse("omni_rotary: this backward is captured into a CUDA graph, but a leaf's gradient accumulator belongs to the default stream: "
+             "drop every graph of the same leaves that was built outside the capture (warm up on a side stream)");
+    }
+  }
+}
+
 struct OmniRotaryFn : torch::autograd::Function<OmniRotaryFn> {
   // The result of q, if there is a q, then that of k.
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Optional& q_in, const Optional& k_in,
@@ -166,6 +187,7 @@ struct OmniRotaryFn : torch::autograd::Function<OmniRotaryFn> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     // The kernels' results have no graph of their own: what create_graph=True asks for would be missing, silently.
     if (at::GradMode::is_enabled()) refuse("omni_rotary has no second derivative (create_graph=True)");
+    refuse_leaves_outside_the_capture();
     const auto saved = ctx->get_saved_variables();
     RotaryArgs r{saved[4], saved[5], saved[2], saved[3], ctx->saved_data["half"].toBool(), ctx->saved_data["factor"].toDouble(),
                  ctx->saved_data["eps"].toDouble()};

@@ -231,3 +231,34 @@ def test_no_second_derivative(cuda_device):
     out, _ = omni.omni_rotary(q, None, omni.OmniRotary.from_base(32, device="cuda"))
     with pytest.raises(omni.OmniAttnError, match="second derivative"):
         torch.autograd.grad(out.square().sum(), q, create_graph=True)
+
+
+@pytest.mark.parametrize("alive", ["nothing", "default", "side"])
+def test_a_captured_backward_and_graphs_of_the_same_leaves(cuda_device, alive):
+    """An eager graph of the leaves that lives on the default stream would end the capture inside autograd: refused before that."""
+    q, k, wq, wk = cuda(*make(1, 2, 1, 40, 64, torch.bfloat16, "shared"))
+    leaves = [x.requires_grad_() for x in (q, k, wq, wk)]
+    rot = omni.OmniRotary.from_base(64, device="cuda")
+    go = [torch.randn_like(x) for x in (q, k)]
+    run = lambda: omni.omni_rotary(q, k, rot, None, wq, wk)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = torch.autograd.grad(run(), leaves, go)
+        kept = run() if alive == "side" else None
+    torch.cuda.current_stream().wait_stream(side)
+    if alive == "default":
+        kept = run()
+    graph, got = torch.cuda.CUDAGraph(), None
+    try:
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(run(), leaves, go)
+    except omni.OmniAttnError as e:
+        assert alive == "default" and "captured" in str(e)
+    assert (got is None) == (alive == "default")
+    if got is not None:
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del kept
+    again = torch.autograd.grad(run(), leaves, go)
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
