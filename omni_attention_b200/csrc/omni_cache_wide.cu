@@ -43,9 +43,17 @@ struct WideCfg {
   static constexpr int kChunks = D / 64;
   static constexpr int kChunk = 128 * 128;
   static constexpr int kSlots = D == 128 ? 6 : 10;   // K and V tiles in flight
+  // Scores of a tile in two halves of 64 keys: the second half is computed as soon as the group has read the scores before for
+  // the last time, under their exponentials, and its maximum is looked for under the first half's product. 2 x 16 heads of 256
+  // rows on 4 352 keys: head_dim 64 33.9 -> 31.2 us; head_dim 128 (32 heads) 53.2 -> 55.9, because a product 64 keys wide
+  // reads the queries twice as often and shared memory is what bounds it.
+  static constexpr bool kHalves = D == 64;
   static constexpr int kBars = (1 + kSlots) * kTile;
-  static constexpr int kPiece = D == 128 ? 432 : 3072;   // where the piece's description is, behind the barriers
-  static constexpr int kSmem = kBars + (D == 128 ? 3072 : 3136);   // barriers, row states, description
+  // Behind the tiles: barriers, flags and limits, which keys are there, row states, the piece's description.
+  static constexpr int kFlags = D == 128 ? 256 : 288, kValid = kFlags + 80, kRows = D == 128 ? 512 : 576;
+  static constexpr int kPiece = D == 128 ? kValid + 16 * kSlots : kRows + 2560;
+  static constexpr int kSmem = kBars + (D == 128 ? 3072 : 3200);
+  static_assert((2 * kSlots + 16) * 8 <= kFlags && (D == 128 ? kPiece + 64 : kValid + 16 * kSlots) <= kRows && kPiece % 16 == 0, "shared memory layout");
 };
 
 // Named barrier of the eight softmax warps.
@@ -135,15 +143,17 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   const uint32_t bar_p = bar_s + 16;                    // [2] P stored
   const uint32_t bar_h = bar_p + 16;                    // [2] P of the tile's first 64 keys stored
   const uint32_t bar_o = bar_h + 16;                    // [2] the group's last product of the piece done
-  const uint32_t bar_end = bar_o + 16;                  // drain of a launch that gives up
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kBars + 256);
+  const uint32_t bar_s2 = bar_o + 16;                   // [2] scores of the tile's last 64 keys done (kHalves)
+  const uint32_t bar_e = bar_s2 + 16;                   // [2] and read for the last time
+  const uint32_t bar_end = bar_e + 16;                  // drain of a launch that gives up
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kBars + Cfg::kFlags);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_lim = reinterpret_cast<int*>(tmem_slot + 2);                                    // [8] largest limit of a warp's rows, [8] smallest
   Piece* s_piece = reinterpret_cast<Piece*>(smem + Cfg::kBars + Cfg::kPiece);
-  static_assert(sizeof(Piece) <= 64 && 336 + 16 * Cfg::kSlots <= (D == 128 ? Cfg::kPiece : 512), "shared memory layout");
+  static_assert(sizeof(Piece) <= 64, "shared memory layout");
   volatile int* s_bad = s_lim + 16;                                                       // a V that is not finite was left out
-  uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + Cfg::kBars + 336);      // [kSlots] keys that are there
-  float* s_m = reinterpret_cast<float*>(smem + Cfg::kBars + 512);                         // [2][128]
+  uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + Cfg::kBars + Cfg::kValid);      // [kSlots] keys that are there
+  float* s_m = reinterpret_cast<float*>(smem + Cfg::kBars + Cfg::kRows);                         // [2][128]
   float* s_l = s_m + 256;                                                                 // [2][128]
   int* s_out = reinterpret_cast<int*>(s_l + 256);                                         // [128] where a row is written
 
@@ -159,6 +169,8 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       mbar_init(bar_p + 8 * g, 128);
       mbar_init(bar_h + 8 * g, 128);
       mbar_init(bar_o + 8 * g, 1);
+      mbar_init(bar_s2 + 8 * g, 1);
+      mbar_init(bar_e + 8 * g, 128);
     }
     mbar_init(bar_end, 1);
     *abort_flag = 0;
@@ -251,7 +263,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         const uint32_t vs = (fill + 2 * i + 1) % Cfg::kSlots;   // V's place in the ring
         const int key = key_first + i * kTileKeys;
         if (lane == 0) {
-          mbar_wait_lim(bar_s + 8 * g, n_vis & 1, abort_flag, p.status, 40 + g, limit);
+          mbar_wait_lim((Cfg::kHalves ? bar_s2 : bar_s) + 8 * g, n_vis & 1, abort_flag, p.status, 40 + g, limit);
           mbar_wait_lim(bar_full + 8 * vs, ((fill + 2 * i + 1) / Cfg::kSlots) & 1, abort_flag, p.status, 42, limit);
         }
         __syncwarp();
@@ -285,7 +297,12 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 
         float mx = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 1; h >= 0; --h) {   // (halves: the last 64 keys' scores are there first)
+          if (Cfg::kHalves && h == 0) {
+            if (lane == 0) mbar_wait_lim(bar_s + 8 * g, n_vis & 1, abort_flag, p.status, 58 + g, limit);
+            __syncwarp();
+            tc_fence_after();
+          }
           float s[64];
           load_scores64(tS + 64 * h, s);
           if constexpr (SOFTCAP) soft_cap_scores(s, cap_in, cap_out);
@@ -310,6 +327,10 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           float s[64];
           uint32_t pk[32];
           load_scores64(tS + 64 * h, s);
+          if (Cfg::kHalves && h == 1) {   // the next scores may go over these
+            tc_fence_before();
+            mbar_arrive(bar_e + 8 * g);
+          }
           if (!SOFTCAP && masked) apply_allow64(allow[2 * h], allow[2 * h + 1], s);
           sum += exp_and_pack_n<BF16, 0, 1, 64>(s, st.M, scale_log2, inv_scale_log2, pk);
           tmem_st32(tS + 32 * h, pk);
@@ -405,7 +426,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     } else if (warp == 9 && elect_one()) {
       // =========================== MMA issuer =====================================================
       constexpr int fmt = BF16 ? 1 : 0;
-      constexpr uint32_t idesc_qk = umma_idesc_f16(128, 128, fmt, 0), idesc_pv = umma_idesc_f16(128, D, fmt, 1);
+      constexpr uint32_t idesc_qk = umma_idesc_f16(128, Cfg::kHalves ? 64 : 128, fmt, 0), idesc_pv = umma_idesc_f16(128, D, fmt, 1);
       constexpr uint32_t hi = umma_desc_hi_sw128(1024);
       constexpr uint32_t kSlot = Cfg::kTile >> 4, kChunk = Cfg::kChunk >> 4;
       const uint32_t q0 = umma_desc_lo(sQ, 16), k0 = umma_desc_lo(sRing, 16), v0 = umma_desc_lo(sRing, Cfg::kChunk);
@@ -416,23 +437,25 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         alive = mbar_wait_lim(bar_q, n_piece & 1, abort_flag, p.status, 50, limit);
         ++n_piece;
         tc_fence_after();
-        auto scores = [&](int i) {   // S_g = Q K^T of visit i
+        auto scores = [&](int i, int half) {   // S_g = Q K^T of visit i; kHalves: the keys 64 * half .. of it, the upper half first
           const uint32_t f = fill + 2 * i, s = f % Cfg::kSlots;
-          alive = alive && mbar_wait_lim(bar_full + 8 * s, (f / Cfg::kSlots) & 1, abort_flag, p.status, 51, limit);
+          if (!Cfg::kHalves || half == 1) alive = alive && mbar_wait_lim(bar_full + 8 * s, (f / Cfg::kSlots) & 1, abort_flag, p.status, 51, limit);
           if (!alive) return;
           tc_fence_after();
-          const uint32_t d = tmem + 128 * (i & 1), kd = k0 + s * kSlot;
+          const uint32_t d = tmem + 128 * (i & 1) + 64 * half, kd = k0 + s * kSlot + half * 512;   // 64 rows = 8192 bytes
           umma_ss_lo<false>(d, q0, kd, hi, idesc_qk);
 #pragma unroll
           for (int k = 1; k < D / 16; ++k) {
             const uint32_t off = (k / 4) * kChunk + (k % 4) * 2;
             umma_ss_lo<true>(d, q0 + off, kd + off, hi, idesc_qk);
           }
-          tc_commit(bar_empty + 8 * s);
-          tc_commit(bar_s + 8 * (i & 1));
+          if (half == 0) tc_commit(bar_empty + 8 * s);
+          tc_commit((half == 0 ? bar_s : bar_s2) + 8 * (i & 1));
         };
-        if (alive) scores(0);
-        if (alive && n > 1) scores(1);
+        for (int i = 0; i < min(n, 2); ++i) {
+          if (Cfg::kHalves) scores(i, 1);
+          scores(i, 0);
+        }
         for (int i = 0; alive && i < n; ++i) {
           const int g = i & 1;
           const uint32_t f = fill + 2 * i + 1, s = f % Cfg::kSlots;
@@ -450,6 +473,11 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           umma_ts_lo(d, a, vd, hi, idesc_pv, i >= 2 ? 1u : 0u);
 #pragma unroll
           for (int k = 1; k < 4; ++k) umma_ts_lo_acc(d, a + 8 * k, vd + k * 128, hi, idesc_pv);   // 16 keys = 2048 bytes
+          if (Cfg::kHalves && i + 2 < n) {   // half of the next scores under the second half's exponentials
+            alive = mbar_wait_lim(bar_e + 8 * g, par, abort_flag, p.status, 43, limit);
+            if (alive) scores(i + 2, 1);
+            if (!alive) break;
+          }
           alive = mbar_wait_lim(bar_p + 8 * g, par, abort_flag, p.status, 56 + g, limit);
           if (!alive) break;
           tc_fence_after();
@@ -457,7 +485,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           for (int k = 4; k < 8; ++k) umma_ts_lo_acc(d, a + 8 * k, vd + k * 128, hi, idesc_pv);
           tc_commit(bar_empty + 8 * s);
           if (i + 2 >= n) tc_commit(bar_o + 8 * g);
-          if (i + 2 < n) scores(i + 2);
+          if (i + 2 < n) scores(i + 2, 0);
         }
         fill += 2 * n;
       }
