@@ -52,7 +52,7 @@ struct WideCfg {
   // Behind the tiles: barriers, flags and limits, which keys are there, row states, the piece's description.
   static constexpr int kFlags = D == 128 ? 256 : 288, kValid = kFlags + 80, kRows = D == 128 ? 512 : 576;
   static constexpr int kPiece = D == 128 ? kValid + 16 * kSlots : kRows + 2560;
-  static constexpr int kSmem = kBars + (D == 128 ? 3072 : 3200);
+  static constexpr int kSmem = kBars + kRows + 2560 + (D == 128 ? 0 : 64);
   static_assert((2 * kSlots + 16) * 8 <= kFlags && (D == 128 ? kPiece + 64 : kValid + 16 * kSlots) <= kRows && kPiece % 16 == 0, "shared memory layout");
 };
 
