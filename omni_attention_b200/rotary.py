@@ -50,8 +50,9 @@ class OmniRotary:
         {"type": "ntk", "factor": s}                       base * s ** (rotary_dim / (rotary_dim - 2))
         {"type": "yarn", "factor": s, "original_length": n, "beta_fast": 32, "beta_slow": 1}
             pairs that turn more than beta_fast times in n positions stay, those below beta_slow are divided by s, those
-            between are mixed linearly in the pair number; cosine and sine are multiplied by 0.1 ln(s) + 1 (or by
-            "attention_factor")."""
+            between are mixed linearly in the pair number (from the last whole number that is still "more" to the first that is
+            "below", which may lie behind the last pair, at most at rotary_dim - 1); cosine and sine are multiplied by
+            0.1 ln(s) + 1 (or by "attention_factor")."""
         if rotary_dim < 2 or rotary_dim % 2:
             raise OmniAttnError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
         if not (math.isfinite(base) and base > 1.0):
@@ -83,7 +84,7 @@ class OmniRotary:
                 if not (n > 0 and fast > slow > 0):
                     raise OmniAttnError("rotary scaling 'yarn' needs original_length > 0 and beta_fast > beta_slow > 0")
                 at = lambda turns: rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
-                lo, hi = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), rotary_dim // 2 - 1)
+                lo, hi = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), rotary_dim - 1)
                 keep = 1.0 - ((pair - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
                 inv = inv / s * (1 - keep) + inv * keep
                 factor = float(scaling.get("attention_factor", 0.1 * math.log(s) + 1.0))

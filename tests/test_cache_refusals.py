@@ -1,6 +1,7 @@
 """What omni_rotary, OmniPagedCache, omni_cache_append and omni_cache_attention refuse, and what the C entry points return
 for it. Nothing here needs a GPU: every check comes before the device is touched."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -47,6 +48,27 @@ def test_rotary_object():
     assert torch.equal(y.inv_freq[0], plain[0]) and torch.allclose(y.inv_freq[-1] * 8, plain[-1]) and y.factor > 1
     n = make.from_base(64, scaling={"type": "ntk", "factor": 8})
     assert torch.allclose(n.inv_freq[-1] * 8, plain[-1]) and n.inv_freq[0] == plain[0]
+
+
+@pytest.mark.parametrize("rotary_dim,length", [(64, 4096), (128, 32768), (64, 131072), (16, 32768), (4, 4096), (32, 300000)])
+def test_yarn_frequencies(rotary_dim, length):
+    """Every pair by how often it turns in the trained length. A pair between the two borders is mixed: the ramp ends where a pair
+    would turn beta_slow times, not at the last pair there is."""
+    base, s, fast, slow = 10000.0, 8.0, 32.0, 1.0
+    got = omni.OmniRotary.from_base(rotary_dim, base, scaling={"type": "yarn", "factor": s, "original_length": length}).inv_freq
+    pair_of = lambda turns: rotary_dim / 2 * math.log(length / (2 * math.pi * turns), base)
+    lo, hi = max(math.floor(pair_of(fast)), 0), math.ceil(pair_of(slow))
+    assert hi < rotary_dim
+    for p in range(rotary_dim // 2):
+        plain = base ** (-2 * p / rotary_dim)
+        turns = length * plain / (2 * math.pi)
+        stretched = min(max((p - lo) / (hi - lo), 0.0), 1.0)
+        assert math.isclose(float(got[p]), plain * (1 - stretched) + plain / s * stretched, rel_tol=1e-12), p
+        # by the definition's own words, wherever the whole-numbered borders leave room
+        if turns > fast and p <= lo:
+            assert math.isclose(float(got[p]), plain, rel_tol=1e-12)
+        if slow < turns < fast and lo < p:
+            assert plain / s < float(got[p]) < plain
 
 
 def test_rotary_call():
