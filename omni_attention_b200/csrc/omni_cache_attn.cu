@@ -44,6 +44,7 @@ struct CacheCfg {
 // What the computing warps are told of a piece.
 struct PieceInfo {
   int n, key0, rows, lim_max;   // tiles of keys (-1: no more pieces), first key, rows, most keys that a row sees
+  int table_of, hk;             // whose page table, which key/value head
   long long share;
   int lim[kNarrowRows];         // keys that a row sees
   int out[kNarrowRows];         // where it is written
@@ -222,6 +223,8 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         to.key0 = pc.key0 + pc.tile0 * kTileKeys;
         to.rows = min(ROWS, pc.rows - pc.rt * ROWS);
         to.lim_max = lim_max;
+        to.table_of = pc.table_of;
+        to.hk = pc.hk;
         to.share = pc.share;
       }
       mbar_arrive(bar_q + 8 * buf);
@@ -285,6 +288,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         l[j] = 0.f;
       }
 
+      bool taken_out = false;   // of V, what is not finite
       for (int t = 0; t < n; ++t, ++fill) {
         const uint32_t slot = fill % Cfg::kSlots;
         const int key = key0 + t * kTileKeys;
@@ -401,39 +405,19 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             }
           }
           if (key + 16 > lim_min && lim_min < lim_max) {
-            // A value that is infinite or NaN must not reach the rows that do not see its key (0 * NaN): such a key's share is
-            // added here, row by row, and its V is zero in the product. Only where rows of the tile see different numbers of keys.
+            // An infinite or NaN value must not reach the rows that do not see its key (0 * NaN): it is taken out of the product
+            // and added at the end of the piece. Looked for only where rows of the tile see different numbers of keys.
             bool bad = false;
-            const uint8_t* v_tile = smem + slot * (2 * Cfg::kTile) + Cfg::kTile;
 #pragma unroll 1
             for (int c = lane >> 4; c < Cfg::kChunks * 8; c += 2) {
-              bad |= not_finite<BF16>(*reinterpret_cast<const uint4*>(v_tile + swizzled(warp * 16 + (lane & 15), c, 128 * 128)));
-            }
-            uint32_t keys = __ballot_sync(0xFFFFFFFFu, bad);
-            keys = (keys | keys >> 16) & 0xFFFFu;
-#pragma unroll 1
-            for (; keys != 0; keys &= keys - 1) {
-              const int r = __ffs(keys) - 1, row = warp * 16 + r;
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                const int from = (r & 7) * 4 + pos;
-                const float p_lo0 = __shfl_sync(0xFFFFFFFFu, s[j][0], from), p_hi0 = __shfl_sync(0xFFFFFFFFu, s[j][2], from);
-                const float p_lo1 = __shfl_sync(0xFFFFFFFFu, s[j][1], from), p_hi1 = __shfl_sync(0xFFFFFFFFu, s[j][3], from);
-                const float p0 = r < 8 ? p_lo0 : p_hi0, p1 = r < 8 ? p_lo1 : p_hi1;
-                const bool sees0 = key + r < lim[2 * j], sees1 = key + r < lim[2 * j + 1];
-#pragma unroll
-                for (int d = 0; d < KS; ++d) {
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const uint32_t raw = *reinterpret_cast<const uint16_t*>(v_tile + swizzled(row, 2 * d + h, 128 * 128) + 2 * quad);
-                    const float v = unpack16<BF16>(raw).x;
-                    if (sees0) o_acc[d][j][2 * h] += p0 * v;
-                    if (sees1) o_acc[d][j][2 * h + 1] += p1 * v;
-                  }
-                }
+              uint4* v = reinterpret_cast<uint4*>(smem + slot * (2 * Cfg::kTile) + Cfg::kTile + swizzled(warp * 16 + (lane & 15), c, 128 * 128));
+              if (not_finite<BF16>(*v)) {
+                *v = finite_part<BF16>(*v);
+                bad = true;
               }
-              __syncwarp();
-              if (lane < Cfg::kChunks * 8) *reinterpret_cast<uint4*>(const_cast<uint8_t*>(v_tile) + swizzled(row, lane, 128 * 128)) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (__any_sync(0xFFFFFFFFu, bad)) {
+              taken_out = true;
               fence_async_smem();
               __syncwarp();
             }
@@ -462,6 +446,55 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           const int r = 8 * (j >> 1) + 2 * pos + (j & 1);
           s_m[warp * kNarrowRows + r] = m[j];
           s_l[warp * kNarrowRows + r] = l[j];
+        }
+      }
+      // Values that are not finite: some were taken out of the products, the others came in as p * inf with p in two parts, of
+      // which the second may be zero or negative. Either way an element is then what the values that its row sees add up to.
+      float odd = 0.f;   // NaN: an element is not finite though its row's sum is
+#pragma unroll
+      for (int j = 0; j < 2 * NT; ++j) {
+        float z = 0.f;
+#pragma unroll
+        for (int d = 0; d < KS; ++d) z = fmaf(o_acc[d][j >> 1][j & 1], 0.f, fmaf(o_acc[d][j >> 1][2 + (j & 1)], 0.f, z));
+        if (l[j] == l[j]) odd += z;
+      }
+      if (__any_sync(0xFFFFFFFFu, taken_out || odd != odd)) {
+        uint32_t met[2] = {0u, 0u};   // elements that met one
+#pragma unroll 1
+        for (int t = 0; t < n; ++t) {
+          const int key = key0 + t * kTileKeys;
+          if (key >= lim_max) break;
+          const int page = __ldg(p.page_table + in.table_of * p.table_stride + (key >> p.page_shift));   // a page has 16 keys at least
+          if (page < 0 || page >= p.num_pages) continue;
+          const uint16_t* v = static_cast<const uint16_t*>(p.v_pages) +
+                              (((static_cast<long long>(page) * p.Hkv + in.hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * d_real;
+          bool bad = false;
+#pragma unroll 1
+          for (int c = lane >> 4; c < d_real / 8; c += 2) bad |= not_finite<BF16>(__ldg(reinterpret_cast<const uint4*>(v + (lane & 15) * d_real) + c));
+          uint32_t keys = __ballot_sync(0xFFFFFFFFu, bad);
+          keys = (keys | keys >> 16) & 0xFFFFu;
+#pragma unroll 1
+          for (; keys != 0; keys &= keys - 1) {
+            const int r = __ffs(keys) - 1;
+#pragma unroll
+            for (int i = 0; i < 2 * KS; ++i) {   // columns 8 i + quad
+              const uint32_t raw = 8 * i < d_real ? __ldg(v + r * d_real + 8 * i + quad) : 0u;
+              if ((raw & kExponent<BF16>) == kExponent<BF16>) {
+                const float x = unpack16<BF16>(raw).x;
+#pragma unroll
+                for (int j = 0; j < 2 * NT; ++j) {
+                  if (key + r < lim[j]) {
+                    constexpr int per = 32 / (2 * NT);   // columns to a word
+                    float& o = o_acc[i >> 1][j >> 1][2 * (i & 1) + (j & 1)];
+                    uint32_t& word = met[i / per];
+                    const uint32_t bit = 1u << ((i % per) * 2 * NT + j);
+                    o = word & bit ? o + x : x;
+                    word |= bit;
+                  }
+                }
+              }
+            }
+          }
         }
       }
       const long long share = in.share;

@@ -240,15 +240,25 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm,
                : "memory");
 }
 
+template <bool BF16>
+constexpr uint32_t kExponent = BF16 ? 0x7F80u : 0x7C00u;   // all of its bits set: infinite or NaN
+
 // Whether one of the eight 16-bit values is infinite or NaN.
 template <bool BF16>
 __device__ __forceinline__ bool not_finite(const uint4& v) {
-  constexpr uint32_t m = BF16 ? 0x7F80u : 0x7C00u;
+  constexpr uint32_t m = kExponent<BF16>;
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) bad |= (w[i] & m) == m || (w[i] & (m << 16)) == m << 16;
   return bad;
+}
+// The eight values with zeros in the place of those.
+template <bool BF16>
+__device__ __forceinline__ uint4 finite_part(const uint4& v) {
+  constexpr uint32_t m = kExponent<BF16>;
+  auto word = [](uint32_t w) { return w & (((w & m) == m ? 0u : 0xFFFFu) | ((w & (m << 16)) == m << 16 ? 0u : 0xFFFF0000u)); };
+  return make_uint4(word(v.x), word(v.y), word(v.z), word(v.w));
 }
 
 // Programmatic dependent launch: a kernel so launched may start before its predecessor has ended; what that one wrote is

@@ -189,6 +189,64 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(cuda_device
         assert not torch.isfinite(got[:, :, T - 1]).any()
 
 
+def same_kinds(got, want, tol, what):
+    """Infinite with the sign, NaN and finite where the definition says so; the finite ones within tol."""
+    got = got.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan()), f"{what}: NaN"
+    for sign in (math.inf, -math.inf):
+        assert torch.equal(got == sign, want == sign), f"{what}: {sign}"
+    fin = want.isfinite()
+    worst = float(((got - want).abs() / tol)[fin].max())
+    assert worst <= 1.0, f"{what}: {worst:.3g} times the tolerance"
+
+
+def infinite_values(B, H, Hkv, T, D, page, lengths, dtype, seed, **kw):
+    """A call on keys whose values are infinite or NaN here and there: (out, 64-bit out, mean of |v|, vmax, scores' bound)."""
+    kp, vp, table, lens, g = make_cache(B, Hkv, D, page, lengths, T, dtype, seed=seed, shared=kw.get("shared_prefix", 0))
+    q = torch.randn(B, H, T, D, generator=g).to(dtype)
+    plain = vp.clone()
+    for b in range(B):
+        n = lengths[b] + T
+        # column 0: +inf everywhere; 1: -inf; 2: both; 3: NaN; 4..: +inf at one key of every sixteenth place
+        for i in torch.randint(0, n, (6,), generator=g).tolist():
+            p, row = int(table[b, i // page]), i % page
+            vp[p, :, row, 0], vp[p, :, row, 1], vp[p, :, row, 3] = math.inf, -math.inf, math.nan
+            vp[p, :, row, 2] = math.inf if i % 2 else -math.inf
+        for i in range(0, n, max(1, n // (D // 3))):
+            vp[int(table[b, i // page]), :, i % page, 4 + i % (D - 4)] = math.inf if i % 3 else -math.inf
+    gpu = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+    got = omni.omni_cache_attention(q.cuda(), on_gpu(kp, vp, table, lens), **gpu)
+    ref = {k: v for k, v in kw.items() if k != "shared_prefix"}
+    want = orc.attention(q, kp, vp, table, lens, **ref)[0]
+    fin = lambda t: torch.nan_to_num(t.double(), nan=0.0, posinf=0.0, neginf=0.0)
+    score = 2.0 ** -20 * D ** -0.5 * float((fin(q).abs().amax((0, 1, 2)) * fin(kp).abs().amax((0, 1, 2))).sum())
+    size = orc.attention(q, kp, plain, table, lens, **ref)[2]
+    return got, want, size, float(fin(plain).abs().max()), score
+
+
+# B, H, Hkv, T, D, page, lengths, dtype, more: up to 16 rows to a key/value head
+INFINITE_FEW = [
+    (1, 2, 2, 1, 64, 16, [40], torch.float16, {}),
+    (2, 8, 2, 1, 128, 64, [300, 17], torch.bfloat16, {}),
+    (2, 4, 1, 1, 32, 32, [63, 129], torch.float16, dict(softcap=20.0)),
+    (1, 16, 1, 1, 128, 16, [2000], torch.bfloat16, {}),                        # 16 rows, cut among CTAs
+    (3, 2, 1, 4, 64, 128, [5, 0, 700], torch.bfloat16, {}),                    # 8 rows that see different numbers of keys
+    (2, 3, 1, 5, 128, 16, [100, 40], torch.float16, dict(causal=False)),
+    (1, 1, 1, 1, 32, 16, [6000], torch.bfloat16, {}),
+    (4, 2, 2, 1, 64, 16, [100, 80, 90, 300], torch.float16, dict(shared_prefix=64)),
+]
+
+
+@pytest.mark.parametrize("B,H,Hkv,T,D,page,lengths,dtype,more", INFINITE_FEW)
+def test_infinite_values_with_few_rows(cuda_device, B, H, Hkv, T, D, page, lengths, dtype, more):
+    for seed in range(3):
+        got, want, size, vmax, score = infinite_values(B, H, Hkv, T, D, page, lengths, dtype, seed, **more)
+        assert want.isinf().any() and want.isnan().any() and want.isfinite().any()
+        # as in check(): the result's rounding, the weights' errors
+        tol = torch.finfo(dtype).eps / 2 * want.abs() + 2 * (score + 2.0 ** -21 + 2.0 ** -16) * vmax + 2.0 ** -25
+        same_kinds(got, want, tol, f"seed {seed}")
+
+
 @pytest.mark.parametrize("bad", [-1, 10 ** 6, -2 ** 31, 2 ** 31 - 1])
 @pytest.mark.parametrize("heads", [4, 48])
 def test_pages_that_are_not_there(cuda_device, bad, heads):
