@@ -18,8 +18,8 @@
 // over the first half of S), O of the two groups.
 //
 // A value that is infinite or NaN must not reach the rows that do not see its key (0 * NaN): where rows of a tile see
-// different numbers of keys such a key's V is zeroed too, and its share is added to the rows that see it when the piece is
-// written (add_not_finite).
+// different numbers of keys it is taken out of the product. What such values make of the rows that see them is found when
+// the piece is written (write_not_finite).
 //
 // Keys that are not there - behind the last token, in a page that does not exist - are never loaded; what the ring holds in
 // their places is zeroed in V (0 * NaN) and masked in S.
@@ -79,49 +79,86 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t addr, float (&f)[COLS]) {
   }
 }
 
+// Barrier of the eight softmax warps, and whether `yes` holds in any of their threads.
+__device__ __forceinline__ bool softmax_any(bool yes) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.or.pred p, 1, 256, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(yes))
+      : "memory");
+  return any != 0;
+}
+
 template <bool BF16>
 __device__ __forceinline__ float value16(uint16_t raw) {
   return BF16 ? __uint_as_float(static_cast<uint32_t>(raw) << 16) : __half2float(__ushort_as_half(raw));
 }
 
-// Whether a row of a V tile (chunks of 128 bytes, `pitch` apart) has a value that is not finite.
+// Takes what is infinite or NaN out of a row of a V tile (chunks of 128 bytes, `pitch` apart). Whether there was any.
 template <bool BF16, int CHUNKS>
-__device__ __noinline__ bool row_not_finite(uint32_t row, uint32_t pitch) {
+__device__ __noinline__ bool take_out_not_finite(uint8_t* row, int r, int pitch) {
   bool bad = false;
 #pragma unroll 4
-  for (int c = 0; c < CHUNKS * 8; ++c) bad |= not_finite<BF16>(lds_v4(row + (c >> 3) * pitch + (c & 7) * 16));
+  for (int c = 0; c < CHUNKS * 8; ++c) {
+    uint4* at = reinterpret_cast<uint4*>(row + (c >> 3) * pitch + r * 128 + (c & 7) * 16);
+    if (not_finite<BF16>(*at)) {
+      *at = finite_part<BF16>(*at);
+      bad = true;
+    }
+  }
   return bad;
 }
 
-// What the product left out for one query row: keys [key_lo, key_hi) whose V is not finite, as far as the row sees them and a
-// page has them, columns [c0, c1). Everything from memory; `out` (16 bit, divided by the row's sum) or `share` (32 bit).
+// By the eight softmax warps, when a piece is written: elements whose row sees infinite or NaN values in their column are what
+// these add up to (the product has them as zeros, as inf, or as NaN where an fp16 weight is below the type's smallest).
+// Keys key0 .. key1, a thread's row (keys below `lim`, columns c0 .. c1) in `out`, or in `share` (32 bit). `keys`: 8 words in
+// shared memory. From memory, a key to a thread; then the keys that have such values, row by row.
 template <bool BF16>
-__device__ __noinline__ void add_not_finite(const CacheAttnParams& p, const Piece& pc, const RowId& id, int key_lo, int key_hi, float top, float sum, int d,
-                                            int c0, int c1, float* share, uint16_t* out) {
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + id.b * p.qs_b + (static_cast<long long>(pc.hk) * p.G + id.g) * p.qs_h + id.t * p.qs_t;
-  for (int key = key_lo; key < key_hi; ++key) {
-    const int page = __ldg(p.page_table + pc.table_of * p.table_stride + (key >> p.page_shift));
-    if (page < 0 || page >= p.num_pages) continue;
-    const long long at = (((static_cast<long long>(page) * p.Hkv + pc.hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * d;
-    const uint16_t *k = static_cast<const uint16_t*>(p.k_pages) + at, *v = static_cast<const uint16_t*>(p.v_pages) + at;
+__device__ __noinline__ void write_not_finite(const CacheAttnParams& p, const Piece& pc, int key0, int key1, int lim, int d, int c0, int c1, float* share,
+                                              uint16_t* out, volatile uint32_t* keys) {
+  const int tid = threadIdx.x, mask = (1 << p.page_shift) - 1;
+  const int* table = p.page_table + pc.table_of * p.table_stride;
+  unsigned long long met = 0;   // columns that met one
+  auto values = [&](int key) -> const uint16_t* {
+    const int page = __ldg(table + (key >> p.page_shift));
+    if (page < 0 || page >= p.num_pages) return nullptr;
+    return static_cast<const uint16_t*>(p.v_pages) + (((static_cast<long long>(page) * p.Hkv + pc.hk) << p.page_shift) + (key & mask)) * d;
+  };
+  for (int base = key0; base < key1; base += 256) {
     bool bad = false;
-    for (int c = 0; c < d; c += 8) bad |= not_finite<BF16>(*reinterpret_cast<const uint4*>(v + c));
-    if (!bad) continue;
-    float s = 0.f;
-    for (int c = 0; c < d; ++c) s += value16<BF16>(q[c]) * value16<BF16>(k[c]);
-    s *= p.scale;
-    if (p.softcap > 0.f) s = tanhf(s / p.softcap) * p.softcap;
-    float w = ex2_approx(s * 1.4426950408889634f - (top == -INFINITY ? 0.f : top));
-    if (share == nullptr) w /= sum;
-    for (int c = c0; c < c1; ++c) {
-      const float x = w * value16<BF16>(v[c]);
-      if (share != nullptr) {
-        share[c] += x;
-      } else {
-        const uint32_t both = pack2<BF16>(value16<BF16>(out[c]) + x, 0.f);
-        out[c] = static_cast<uint16_t>(both);
+    if (base + tid < key1) {
+      const uint16_t* v = values(base + tid);
+      for (int c = 0; v != nullptr && c < d; c += 8) bad |= not_finite<BF16>(__ldg(reinterpret_cast<const uint4*>(v + c)));
+    }
+    const uint32_t word = __ballot_sync(0xFFFFFFFFu, bad);
+    if ((tid & 31) == 0) keys[tid >> 5] = word;
+    softmax_sync();
+    for (int w = 0; w < 8; ++w) {
+      for (uint32_t left = keys[w]; left != 0; left &= left - 1) {
+        const int key = base + 32 * w + __ffs(left) - 1;
+        if (key >= lim) break;
+        const uint16_t* v = values(key);
+        for (int c = c0; c < c1; ++c) {
+          const uint16_t raw = __ldg(v + c);
+          if ((raw & kExponent<BF16>) != kExponent<BF16>) continue;
+          const float x = value16<BF16>(raw);
+          const bool again = met >> (c - c0) & 1u;
+          met |= 1ull << (c - c0);
+          if (share != nullptr) {
+            share[c] = again ? share[c] + x : x;
+          } else {
+            out[c] = static_cast<uint16_t>(pack2<BF16>(again ? value16<BF16>(out[c]) + x : x, 0.f));
+          }
+        }
       }
     }
+    softmax_sync();   // the next words go over these
   }
 }
 
@@ -151,7 +188,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   int* s_lim = reinterpret_cast<int*>(tmem_slot + 2);                                    // [8] largest limit of a warp's rows, [8] smallest
   Piece* s_piece = reinterpret_cast<Piece*>(smem + Cfg::kBars + Cfg::kPiece);
   static_assert(sizeof(Piece) <= 64, "shared memory layout");
-  volatile int* s_bad = s_lim + 16;                                                       // a V that is not finite was left out
+  volatile int* s_bad = s_lim + 16;   // a value that is not finite was taken out
   uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + Cfg::kBars + Cfg::kValid);      // [kSlots] keys that are there
   float* s_m = reinterpret_cast<float*>(smem + Cfg::kBars + Cfg::kRows);                         // [2][128]
   float* s_l = s_m + 256;                                                                 // [2][128]
@@ -279,12 +316,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           for (int w = 0; w < 4; ++w) allow[w] = valid[w] & low_bits(lim - key - 32 * w);
           const int quarter = warp & 3;   // key r of the tile is in word r / 32
           const uint32_t word = quarter == 0 ? valid[0] : quarter == 1 ? valid[1] : quarter == 2 ? valid[2] : valid[3];
-          bool drop = !(word >> lane & 1u);   // not there, or no row sees it: zero its V
-          if (!drop && key + r >= lim_min) {  // not every row sees it
-            drop = row_not_finite<BF16, Cfg::kChunks>(sRing + Cfg::kTile * vs + r * 128, Cfg::kChunk);
-            if (drop) *s_bad = 1;
-          }
-          if (drop) {
+          if (!(word >> lane & 1u)) {   // not there, or no row sees it: zero its V
 #pragma unroll
             for (int c = 0; c < Cfg::kChunks; ++c) {
               uint4* at = reinterpret_cast<uint4*>(smem + Cfg::kTile * (1 + vs) + c * Cfg::kChunk + r * 128);
@@ -292,6 +324,11 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
               for (int j = 0; j < 8; ++j) at[j] = make_uint4(0u, 0u, 0u, 0u);
             }
             fence_async_smem();
+          } else if (key + r >= lim_min) {   // not every row sees it
+            if (take_out_not_finite<BF16, Cfg::kChunks>(smem + Cfg::kTile * (1 + vs), r, Cfg::kChunk)) {
+              *s_bad = 1;
+              fence_async_smem();
+            }
           }
         }
 
@@ -371,10 +408,17 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       const bool have = mine > 0 && any;
       constexpr int C = D / 4, Q4 = C / 4;   // columns of a round, 16-byte pieces of a row
       float4* xchg = reinterpret_cast<float4*>(smem);   // [2][128][Q4], pieces of a row spread over the banks
+      float odd = 0.f;   // NaN: an element is not finite though its row's sum is
 #pragma unroll 1   // code that runs once comes at about 7 cycles an instruction: little of it counts
       for (int round = 0; round * C < d_real; ++round) {
         float o[C];
-        if (mine > 0) tmem_ld_cols<C>(tO + round * C, o);
+        if (mine > 0) {
+          tmem_ld_cols<C>(tO + round * C, o);
+          if (sum == sum) {
+#pragma unroll
+            for (int j = 0; j < C; ++j) odd = fmaf(o[j], 0.f, odd);
+          }
+        }
 #pragma unroll
         for (int j = 0; j < Q4; ++j) {
           xchg[(128 * g + r) * Q4 + (j ^ (r & (Q4 - 1)))] =
@@ -398,16 +442,12 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         }
         softmax_sync();   // the next round, or the next piece's queries, go over what was read
       }
-      if (left_out) {   // what is written is there for all of the softmax threads behind the barrier above
+      if (softmax_any(left_out || odd != odd)) {
         const Piece whole = *s_piece;
-        const int key_lo = max(lim_min, key_first), key_hi = min(lim, whole.key0 + whole.tile1 * kTileKeys);
         const int half = d_real / 2;
-        if (r < rows_here) {
-          add_not_finite<BF16>(p, whole, row_of(p, whole.prefix, whole.seg, whole.rt * kWideRows + r), key_lo, key_hi, top, sum, d_real, g * half, (g + 1) * half,
+        write_not_finite<BF16>(p, whole, key_first, min(lim_max, whole.key0 + whole.tile1 * kTileKeys), r < rows_here ? lim : 0, d_real, g * half, (g + 1) * half,
                                share != nullptr ? share + r * d_real : nullptr,
-                               static_cast<uint16_t*>(p.out) + static_cast<long long>(s_out[r]) * d_real);
-        }
-        softmax_sync();
+                               static_cast<uint16_t*>(p.out) + static_cast<long long>(s_out[r]) * d_real, reinterpret_cast<volatile uint32_t*>(smem));
       }
       if (r < rows_here && g == 0) {
         if (share != nullptr) {

@@ -200,10 +200,10 @@ def same_kinds(got, want, tol, what):
     assert worst <= 1.0, f"{what}: {worst:.3g} times the tolerance"
 
 
-def infinite_values(B, H, Hkv, T, D, page, lengths, dtype, seed, **kw):
+def infinite_values(B, H, Hkv, T, D, page, lengths, dtype, seed, gain=1.0, **kw):
     """A call on keys whose values are infinite or NaN here and there: (out, 64-bit out, mean of |v|, vmax, scores' bound)."""
     kp, vp, table, lens, g = make_cache(B, Hkv, D, page, lengths, T, dtype, seed=seed, shared=kw.get("shared_prefix", 0))
-    q = torch.randn(B, H, T, D, generator=g).to(dtype)
+    q = (gain * torch.randn(B, H, T, D, generator=g)).to(dtype)
     plain = vp.clone()
     for b in range(B):
         n = lengths[b] + T
@@ -245,6 +245,50 @@ def test_infinite_values_with_few_rows(cuda_device, B, H, Hkv, T, D, page, lengt
         # as in check(): the result's rounding, the weights' errors
         tol = torch.finfo(dtype).eps / 2 * want.abs() + 2 * (score + 2.0 ** -21 + 2.0 ** -16) * vmax + 2.0 ** -25
         same_kinds(got, want, tol, f"seed {seed}")
+
+
+# more than 16 rows to a key/value head
+INFINITE_MANY = [
+    (1, 24, 1, 1, 128, 128, [257], torch.float16, {}),
+    (2, 2, 1, 33, 64, 64, [0, 90], torch.float16, {}),
+    (1, 4, 4, 70, 32, 16, [100], torch.bfloat16, dict(causal=False, softcap=30.0)),
+    (2, 2, 2, 130, 128, 32, [17, 300], torch.bfloat16, dict(causal=False)),
+    (1, 2, 1, 20, 64, 16, [3000], torch.bfloat16, {}),                         # cut among CTAs
+    (1, 2, 1, 20, 128, 64, [300], torch.float16, dict(causal=False, gain=8.0)),  # weights below fp16's smallest
+    (1, 20, 1, 1, 64, 64, [300], torch.float16, dict(gain=8.0)),
+    (12, 2, 1, 1, 64, 16, [100 + i for i in range(12)], torch.float16, dict(shared_prefix=64)),
+]
+
+
+@pytest.mark.parametrize("B,H,Hkv,T,D,page,lengths,dtype,more", INFINITE_MANY)
+def test_infinite_values_with_many_rows(cuda_device, B, H, Hkv, T, D, page, lengths, dtype, more):
+    for seed in range(2):
+        got, want, size, vmax, score = infinite_values(B, H, Hkv, T, D, page, lengths, dtype, seed, **more)
+        assert want.isinf().any() and want.isnan().any() and want.isfinite().any()
+        # as in check(), P rounded to 16 bits; the shared prefix of two rows a sequence has 24 rows
+        tol = torch.finfo(dtype).eps / 2 * (want.abs() + size) + 2 * (score + 2.0 ** -21 + 2.0 ** -16) * vmax + 2.0 ** -25
+        if dtype == torch.float16:
+            tol = tol + 2.0 ** -24 * (max(lengths) + T) * vmax
+        same_kinds(got, want, tol, f"seed {seed}")
+
+
+@pytest.mark.parametrize("B,H,Hkv,T,D,page,lengths,dtype,more", [
+    (1, 2, 1, 20, 128, 64, [300], torch.float16, {}),
+    (2, 4, 2, 30, 64, 16, [100, 40], torch.bfloat16, {}),
+])
+def test_finite_columns_beside_infinite_ones(cuda_device, B, H, Hkv, T, D, page, lengths, dtype, more):
+    """The columns of a key that are finite go through the product like any other's, although rows of the tile see different
+    numbers of keys: the same bits as without the infinite ones."""
+    kp, vp, table, lens, g = make_cache(B, Hkv, D, page, lengths, T, dtype, seed=9)
+    q = torch.randn(B, H, T, D, generator=g).to(dtype)
+    clean = omni.omni_cache_attention(q.cuda(), on_gpu(kp, vp, table, lens))
+    for b in range(B):
+        for t in range(T):
+            i = lengths[b] + t
+            vp[int(table[b, i // page]), :, i % page, t % 3] = math.inf
+    got = omni.omni_cache_attention(q.cuda(), on_gpu(kp, vp, table, lens))
+    assert torch.equal(got[..., 3:], clean[..., 3:])
+    assert (got[:, :, 3:, :3] == math.inf).all() and (got[:, :, 0, 0] == math.inf).all()
 
 
 @pytest.mark.parametrize("bad", [-1, 10 ** 6, -2 ** 31, 2 ** 31 - 1])
