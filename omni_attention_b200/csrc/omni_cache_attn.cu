@@ -109,6 +109,27 @@ __device__ __forceinline__ uint32_t swizzled(int r, int c, int pitch) {
   return static_cast<uint32_t>((c >> 3) * pitch + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// What the infinite and NaN values of column `col` in keys key0 .. key1 add up to, 0 without any: the result of a row that sees
+// these keys, whatever the products made of them. Everything from memory.
+template <bool BF16>
+__device__ __noinline__ float not_finite_sum(const CacheAttnParams& p, int table_of, int hk, int key0, int key1, int d, int col) {
+  const int in_page = (1 << p.page_shift) - 1;
+  const int* table = p.page_table + table_of * p.table_stride;
+  float sum = 0.f;
+  for (int key = key0; key < key1; key += 16) {   // 16 keys from a multiple of 16 on are in one page
+    const int page = __ldg(table + (key >> p.page_shift));
+    if (page < 0 || page >= p.num_pages) continue;
+    const uint16_t* v = static_cast<const uint16_t*>(p.v_pages) +
+                        (((static_cast<long long>(page) * p.Hkv + hk) << p.page_shift) + (key & in_page)) * d + col;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t raw = __ldg(v + i * d);
+      if ((raw & kExponent<BF16>) == kExponent<BF16> && key + i < key1) sum += unpack16<BF16>(raw).x;
+    }
+  }
+  return sum;
+}
+
 // Barrier of the eight computing warps.
 __device__ __forceinline__ void compute_sync() { named_barrier_sync(1, kWarps * 32); }
 
@@ -147,6 +168,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * Cfg::kSlots;
   const uint32_t bar_q = bar_empty + 8 * Cfg::kSlots;      // [2] a piece's description and queries are there
   const uint32_t bar_free = bar_q + 16;                    // [2] and not needed any more
+  volatile int* taken_out = reinterpret_cast<volatile int*>(rest + 240);   // [2] of a piece's V, something that is not finite
   volatile int* abort_flag = reinterpret_cast<volatile int*>(rest + 248);
   uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(rest + 256);   // [kSlots]
   PieceInfo* info = reinterpret_cast<PieceInfo*>(rest + 512);             // [2]
@@ -164,6 +186,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       mbar_init(bar_free + 8 * i, kWarps);
     }
     *abort_flag = 0;
+    taken_out[0] = taken_out[1] = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -288,7 +311,6 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         l[j] = 0.f;
       }
 
-      bool taken_out = false;   // of V, what is not finite
       for (int t = 0; t < n; ++t, ++fill) {
         const uint32_t slot = fill % Cfg::kSlots;
         const int key = key0 + t * kTileKeys;
@@ -417,7 +439,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
               }
             }
             if (__any_sync(0xFFFFFFFFu, bad)) {
-              taken_out = true;
+              if (lane == 0) taken_out[buf] = 1;
               fence_async_smem();
               __syncwarp();
             }
@@ -448,55 +470,6 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           s_l[warp * kNarrowRows + r] = l[j];
         }
       }
-      // Values that are not finite: some were taken out of the products, the others came in as p * inf with p in two parts, of
-      // which the second may be zero or negative. Either way an element is then what the values that its row sees add up to.
-      float odd = 0.f;   // NaN: an element is not finite though its row's sum is
-#pragma unroll
-      for (int j = 0; j < 2 * NT; ++j) {
-        float z = 0.f;
-#pragma unroll
-        for (int d = 0; d < KS; ++d) z = fmaf(o_acc[d][j >> 1][j & 1], 0.f, fmaf(o_acc[d][j >> 1][2 + (j & 1)], 0.f, z));
-        if (l[j] == l[j]) odd += z;
-      }
-      if (__any_sync(0xFFFFFFFFu, taken_out || odd != odd)) {
-        uint32_t met[2] = {0u, 0u};   // elements that met one
-#pragma unroll 1
-        for (int t = 0; t < n; ++t) {
-          const int key = key0 + t * kTileKeys;
-          if (key >= lim_max) break;
-          const int page = __ldg(p.page_table + in.table_of * p.table_stride + (key >> p.page_shift));   // a page has 16 keys at least
-          if (page < 0 || page >= p.num_pages) continue;
-          const uint16_t* v = static_cast<const uint16_t*>(p.v_pages) +
-                              (((static_cast<long long>(page) * p.Hkv + in.hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * d_real;
-          bool bad = false;
-#pragma unroll 1
-          for (int c = lane >> 4; c < d_real / 8; c += 2) bad |= not_finite<BF16>(__ldg(reinterpret_cast<const uint4*>(v + (lane & 15) * d_real) + c));
-          uint32_t keys = __ballot_sync(0xFFFFFFFFu, bad);
-          keys = (keys | keys >> 16) & 0xFFFFu;
-#pragma unroll 1
-          for (; keys != 0; keys &= keys - 1) {
-            const int r = __ffs(keys) - 1;
-#pragma unroll
-            for (int i = 0; i < 2 * KS; ++i) {   // columns 8 i + quad
-              const uint32_t raw = 8 * i < d_real ? __ldg(v + r * d_real + 8 * i + quad) : 0u;
-              if ((raw & kExponent<BF16>) == kExponent<BF16>) {
-                const float x = unpack16<BF16>(raw).x;
-#pragma unroll
-                for (int j = 0; j < 2 * NT; ++j) {
-                  if (key + r < lim[j]) {
-                    constexpr int per = 32 / (2 * NT);   // columns to a word
-                    float& o = o_acc[i >> 1][j >> 1][2 * (i & 1) + (j & 1)];
-                    uint32_t& word = met[i / per];
-                    const uint32_t bit = 1u << ((i % per) * 2 * NT + j);
-                    o = word & bit ? o + x : x;
-                    word |= bit;
-                  }
-                }
-              }
-            }
-          }
-        }
-      }
       const long long share = in.share;
       constexpr int C = Cfg::kRound / NT, TR = 256 / ROWS, V = C / TR;   // columns of a round, threads of a row, columns of a thread
       constexpr int P = C + 4;                                           // pitch of a row
@@ -504,6 +477,7 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       const long long at_row = in.out[r];
       const bool sees = in.lim[r] > 0;
       float f[kWarps], top = -INFINITY, sum = 0.f;
+      bool odd = false;   // values were taken out, or an element is not finite though its row's sum is
 #pragma unroll
       for (int round = 0; round < D / C; ++round) {
         if (round * C >= d_real) break;
@@ -520,6 +494,8 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         }
         compute_sync();
         if (round == 0) {
+          odd = taken_out[buf] != 0;
+          if (threadIdx.x == 0) taken_out[buf ^ 1] = 0;   // the piece before is done with it, the next one has not begun
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w * kNarrowRows + r]);
           const float at = top == -INFINITY ? 0.f : top;
@@ -543,6 +519,10 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] += f[w] * s_join[(w * ROWS + r) * P + in_round + i];
           }
+          float z = 0.f;
+#pragma unroll
+          for (int i = 0; i < V; ++i) z = fmaf(acc[i], 0.f, z);
+          odd |= z != z && sum == sum;
           if (share >= 0) {
             float* to = share_at(p, how, share, d_real) + r * d_real + col;
 #pragma unroll
@@ -559,6 +539,21 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           }
         }
         compute_sync();   // the next round goes over what was read
+      }
+      // Of values that are not finite some were taken out of the products, the others came in as p * inf with p in two parts, of
+      // which the second may be zero or negative: an element whose row sees such values in its column is what they add up to.
+      if (odd && r < rows) {
+#pragma unroll 1
+        for (int e = 0; e < d_real / TR; ++e) {
+          const int col = e / V * C + threadIdx.x % TR * V + e % V;   // what this thread wrote
+          const float x = not_finite_sum<BF16>(p, in.table_of, in.hk, in.key0, min(in.lim[r], in.key0 + n * kTileKeys), d_real, col);
+          if (x == 0.f) continue;
+          if (share >= 0) {
+            share_at(p, how, share, d_real)[r * d_real + col] = x;
+          } else {
+            static_cast<uint16_t*>(p.out)[at_row * d_real + col] = static_cast<uint16_t>(pack16<BF16>(x, 0.f));
+          }
+        }
       }
       if (r < rows && threadIdx.x % TR == 0) {
         if (share >= 0) {

@@ -79,22 +79,6 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t addr, float (&f)[COLS]) {
   }
 }
 
-// Barrier of the eight softmax warps, and whether `yes` holds in any of their threads.
-__device__ __forceinline__ bool softmax_any(bool yes) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %1, 0;\n\t"
-      "bar.red.or.pred p, 1, 256, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}\n"
-      : "=r"(any)
-      : "r"(static_cast<uint32_t>(yes))
-      : "memory");
-  return any != 0;
-}
-
 template <bool BF16>
 __device__ __forceinline__ float value16(uint16_t raw) {
   return BF16 ? __uint_as_float(static_cast<uint32_t>(raw) << 16) : __half2float(__ushort_as_half(raw));
@@ -188,7 +172,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
   int* s_lim = reinterpret_cast<int*>(tmem_slot + 2);                                    // [8] largest limit of a warp's rows, [8] smallest
   Piece* s_piece = reinterpret_cast<Piece*>(smem + Cfg::kBars + Cfg::kPiece);
   static_assert(sizeof(Piece) <= 64, "shared memory layout");
-  volatile int* s_bad = s_lim + 16;   // a value that is not finite was taken out
+  volatile int* s_bad = s_lim + 16;   // [0] a value that is not finite was taken out, [1] an element is not though its row's sum is
   uint32_t(*s_valid)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + Cfg::kBars + Cfg::kValid);      // [kSlots] keys that are there
   float* s_m = reinterpret_cast<float*>(smem + Cfg::kBars + Cfg::kRows);                         // [2][128]
   float* s_l = s_m + 256;                                                                 // [2][128]
@@ -211,7 +195,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     }
     mbar_init(bar_end, 1);
     *abort_flag = 0;
-    *s_bad = 0;
+    s_bad[0] = s_bad[1] = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -326,7 +310,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             fence_async_smem();
           } else if (key + r >= lim_min) {   // not every row sees it
             if (take_out_not_finite<BF16, Cfg::kChunks>(smem + Cfg::kTile * (1 + vs), r, Cfg::kChunk)) {
-              *s_bad = 1;
+              s_bad[0] = 1;
               fence_async_smem();
             }
           }
@@ -395,7 +379,7 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       s_m[128 * g + r] = st.M;
       s_l[128 * g + r] = st.l;
       softmax_sync();   // (also: every score of the piece is read, its queries are not needed any more)
-      const bool left_out = *s_bad != 0;
+      bool taken_out = s_bad[0] != 0;
       const float mo = s_m[128 * (1 - g) + r], lo = s_l[128 * (1 - g) + r];
       const float top = lim > 0 ? fmaxf(st.M, mo) : -INFINITY, at = top == -INFINITY ? 0.f : top;
       float f = ex2_approx(st.M - at);
@@ -408,16 +392,16 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       const bool have = mine > 0 && any;
       constexpr int C = D / 4, Q4 = C / 4;   // columns of a round, 16-byte pieces of a row
       float4* xchg = reinterpret_cast<float4*>(smem);   // [2][128][Q4], pieces of a row spread over the banks
-      float odd = 0.f;   // NaN: an element is not finite though its row's sum is
 #pragma unroll 1   // code that runs once comes at about 7 cycles an instruction: little of it counts
       for (int round = 0; round * C < d_real; ++round) {
         float o[C];
         if (mine > 0) {
           tmem_ld_cols<C>(tO + round * C, o);
-          if (sum == sum) {
+          float2 z[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int j = 0; j < C; ++j) odd = fmaf(o[j], 0.f, odd);
-          }
+          for (int j = 0; j < C / 2; ++j) z[j & 1] = __ffma2_rn(make_float2(o[2 * j], o[2 * j + 1]), make_float2(0.f, 0.f), z[j & 1]);
+          const float all = z[0].x + z[0].y + z[1].x + z[1].y;
+          if (all != all && sum == sum) s_bad[1] = 1;
         }
 #pragma unroll
         for (int j = 0; j < Q4; ++j) {
@@ -425,7 +409,8 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
               have ? make_float4(o[4 * j] * f, o[4 * j + 1] * f, o[4 * j + 2] * f, o[4 * j + 3] * f) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         softmax_sync();
-        if (tid == 0) *s_bad = 0;   // everyone has read it, nobody sets it before the next piece
+        if (tid == 0) s_bad[0] = 0;   // everyone has read it, nobody sets it before the next piece
+        taken_out |= s_bad[1] != 0;
 #pragma unroll
         for (int i = 0; i < 128 * Q4 / 256; ++i) {
           const int item = tid + 256 * i, rr = item / Q4, j = item % Q4;
@@ -442,7 +427,8 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         }
         softmax_sync();   // the next round, or the next piece's queries, go over what was read
       }
-      if (softmax_any(left_out || odd != odd)) {
+      if (tid == 0) s_bad[1] = 0;   // as above
+      if (taken_out) {
         const Piece whole = *s_piece;
         const int half = d_real / 2;
         write_not_finite<BF16>(p, whole, key_first, min(lim_max, whole.key0 + whole.tile1 * kTileKeys), r < rows_here ? lim : 0, d_real, g * half, (g + 1) * half,
