@@ -299,13 +299,29 @@ __device__ __forceinline__ void turn_of(const RotaryParams& p, const Place<D, HA
     (j & 1 ? r.s[j >> 1].y : r.s[j >> 1].x) = sn;
   }
 }
-__device__ __forceinline__ void rotate(Pairs& x, const Turn& r) {
+// Pairs behind the rotated part pass through as they are (a turn by cosine 1 and sine 0 would make the neighbour of an infinite
+// element NaN). With vector loads in the half layout all of a thread's pairs are rotated or none.
+template <bool VEC, int D, bool HALF>
+__device__ __forceinline__ void rotate(Pairs& x, const Turn& r, const Place<D, HALF>& at) {
+  const int n = at.rd2 - at.pair(0);   // how many are rotated
+  if (n <= 0) return;
+  Pairs y;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 minus = make_float2(-r.s[i].x, -r.s[i].y);
-    const float2 a = __ffma2_rn(x.b[i], minus, __fmul2_rn(x.a[i], r.c[i]));
-    x.b[i] = __ffma2_rn(x.b[i], r.c[i], __fmul2_rn(x.a[i], r.s[i]));
-    x.a[i] = a;
+    y.a[i] = __ffma2_rn(x.b[i], minus, __fmul2_rn(x.a[i], r.c[i]));
+    y.b[i] = __ffma2_rn(x.b[i], r.c[i], __fmul2_rn(x.a[i], r.s[i]));
+  }
+  if constexpr (VEC && HALF) {
+    x = y;
+  } else if (n >= 8) {
+    x = y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (2 * i < n) x.a[i].x = y.a[i].x, x.b[i].x = y.b[i].x;
+      if (2 * i + 1 < n) x.a[i].y = y.a[i].y, x.b[i].y = y.b[i].y;
+    }
   }
 }
 __device__ __forceinline__ void scale_by(Pairs& x, float f) {
@@ -452,11 +468,11 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_kernel(cons
         if (norm) {
           const float r = rsqrtf(row_sum<LPR>(dot(v, v)) * (1.f / D) + p.eps);
           times(v, w);
-          if (seg < 2) rotate(v, turn);
+          if (seg < 2) rotate<VEC>(v, turn, at);
           scale_by(v, r);
           if (p.w_per_head && h + 1 < min(h1, seg_end)) load_weight<T, D, HALF, VEC>(p.seg[seg].w, p.w_f32, ++hl, at, w);
         } else if (seg < 2) {
-          rotate(v, turn);
+          rotate<VEC>(v, turn, at);
         }
         if (zero) {
 #pragma unroll
@@ -578,7 +594,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_bwd_kernel(
       }
       read_ahead(i + kStages - 1);
       const float r = rsqrtf(row_sum<LPR>(dot(v, v)) * (1.f / D) + p.eps);
-      rotate(d, turn);
+      rotate<VEC>(d, turn, at);
       scale_by(v, r);   // x_hat
       if (inside) {
 #pragma unroll

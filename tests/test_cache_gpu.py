@@ -189,6 +189,22 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(cuda_device
         assert not torch.isfinite(got[:, :, T - 1]).any()
 
 
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16), (32, torch.bfloat16)])
+def test_append_without_rotation_stores_what_it_is_given(cuda_device, D, dtype):
+    g = torch.Generator().manual_seed(6)
+    k, v, q = (torch.randn(2, 3, 20, D, generator=g).to(dtype) for _ in range(3))
+    for t in (k, v, q):
+        where = torch.rand(t.shape, generator=g) < 0.2
+        t[where] = torch.tensor([math.inf, -math.inf, math.nan], dtype=dtype)[torch.arange(int(where.sum())) % 3]
+    cache = omni.OmniPagedCache.allocate(4, 3, 16, D, 2, 2, dtype)
+    cache.page_table.copy_(torch.arange(4).view(2, 2))
+    back = omni.omni_cache_append(cache, k.cuda(), v.cuda(), q=q.cuda())
+    stored = lambda pages: pages.view(2, 2, 3, 16, D).transpose(1, 2).reshape(2, 3, 32, D)[:, :, :20].cpu()
+    for got, given in ((stored(cache.k_pages), k), (stored(cache.v_pages), v), (back.cpu(), q)):
+        assert torch.equal(got.isnan(), given.isnan())
+        assert torch.equal(got.nan_to_num(nan=7.0), given.nan_to_num(nan=7.0))
+
+
 def same_kinds(got, want, tol, what):
     """Infinite with the sign, NaN and finite where the definition says so; the finite ones within tol."""
     got = got.double().cpu()

@@ -226,6 +226,40 @@ def test_infinite_and_zero_rows_stay_where_they_are(cuda_device):
     assert not out[0, 1, 6].any()
 
 
+@pytest.mark.parametrize("D,rd", [(64, 32), (64, 20), (64, 6), (128, 64), (128, 2), (32, 8), (32, 16)])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_what_is_not_rotated_passes_through(cuda_device, D, rd, layout, dtype):
+    """Every element behind rotary_dim comes out bit for bit, an infinite or NaN neighbour or not; the same in the gradients."""
+    q, g, _, _ = make(2, 3, 3, 19, D, dtype)
+    marks = torch.tensor([math.inf, -math.inf, math.nan], dtype=dtype)
+    at = torch.rand(q.shape, generator=torch.Generator().manual_seed(4))
+    at[..., :rd] = 1.0
+    for t in (q, g):
+        where = at < 0.3
+        t[where] = marks[torch.arange(int(where.sum())) % 3]
+    rot = omni.OmniRotary.from_base(rd, layout=layout, device="cuda")
+    x = q.cuda().requires_grad_()
+    y, _ = omni.omni_rotary(x, None, rot)
+    dx, = torch.autograd.grad(y, x, g.cuda())
+    same = lambda a, b: torch.equal(a.cpu().nan_to_num(nan=7.0), b.nan_to_num(nan=7.0)) and torch.equal(a.cpu().isnan(), b.isnan())
+    for got, given in ((y.detach(), q), (dx, g)):
+        assert torch.isfinite(got[..., :rd]).all() and same(got[..., rd:], given[..., rd:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_normed_rows_with_an_infinite_element(cuda_device, dtype):
+    """By the definition: the row's factor is 0, its finite elements come out 0 and the infinite one NaN; rotation mixes it with
+    the other member of its pair, and with nothing that is not rotated."""
+    q, _, w, _ = make(1, 2, 1, 4, 64, dtype, "shared")
+    q[0, 0, 1, 40], q[0, 1, 2, 4] = math.inf, -math.inf
+    rot = omni.OmniRotary.from_base(32, device="cuda")
+    got = omni.omni_rotary(q.cuda(), None, rot, None, w.cuda())[0].cpu()
+    want = orc.rotate(q, torch.arange(4)[None], rot.inv_freq.cpu(), weight=w)
+    assert torch.equal(got.isnan(), want.isnan()) and int(want.isnan().sum()) == 3
+    assert not got[0, 0, 1, :40].any() and not got[0, 0, 1, 41:].any()
+
+
 def test_no_second_derivative(cuda_device):
     q = torch.randn(1, 1, 4, 32, device="cuda", requires_grad=True)
     out, _ = omni.omni_rotary(q, None, omni.OmniRotary.from_base(32, device="cuda"))
