@@ -226,8 +226,10 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       const uint16_t* src = nullptr;
       if (lane < ROWS && row < pc.rows) {
         const RowId id = row_of(p, pc.prefix, pc.seg, row);
-        src = static_cast<const uint16_t*>(p.q) + id.b * p.qs_b + (static_cast<long long>(pc.hk) * p.G + id.g) * p.qs_h + id.t * p.qs_t;
         lim = min(limit_of(p, id.b, id.t), pc.total);
+        if (lim > 0) {   // a row that sees nothing may hold anything, and moves no other row's maximum
+          src = static_cast<const uint16_t*>(p.q) + id.b * p.qs_b + (static_cast<long long>(pc.hk) * p.G + id.g) * p.qs_h + id.t * p.qs_t;
+        }
         to.out[lane] = static_cast<int>(out_row(p, id, pc.hk));
       }
       constexpr int CH = D / 8;
@@ -363,10 +365,14 @@ omni_cache_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             for (int j = 0; j < NT; ++j) {
 #pragma unroll
               for (int e = 0; e < 4; e += 2) {
-                float2 y = make_float2(s[j][e], s[j][e + 1]);
-                y = small ? tanh_small2(y) : make_float2(tanh_exact(y.x), tanh_exact(y.y));
-                s[j][e] = y.x * cap_out;
-                s[j][e + 1] = y.y * cap_out;
+                const float2 y = make_float2(s[j][e], s[j][e + 1]);
+                float2 t = tanh_small2(y);
+                if (!small) {   // which form a score takes depends on nothing but itself: keys that are not there are among these
+                  t.x = fabsf(y.x) <= kTanhPolyLimit ? t.x : tanh_exact(y.x);
+                  t.y = fabsf(y.y) <= kTanhPolyLimit ? t.y : tanh_exact(y.y);
+                }
+                s[j][e] = t.x * cap_out;
+                s[j][e + 1] = t.y * cap_out;
               }
             }
           } else {

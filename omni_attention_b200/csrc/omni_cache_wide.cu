@@ -84,6 +84,14 @@ __device__ __forceinline__ float value16(uint16_t raw) {
   return BF16 ? __uint_as_float(static_cast<uint32_t>(raw) << 16) : __half2float(__ushort_as_half(raw));
 }
 
+// Zeros in the place of scores that are not allowed.
+__device__ __forceinline__ void zero_not_allowed64(uint32_t allow0, uint32_t allow1, float (&s)[64]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[j] = ((allow0 >> j) & 1u) ? s[j] : 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[32 + j] = ((allow1 >> j) & 1u) ? s[32 + j] : 0.f;
+}
+
 // Takes what is infinite or NaN out of a row of a V tile (chunks of 128 bytes, `pitch` apart). Whether there was any.
 template <bool BF16, int CHUNKS>
 __device__ __noinline__ bool take_out_not_finite(uint8_t* row, int r, int pitch) {
@@ -326,7 +334,12 @@ omni_cache_wide_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
           }
           float s[64];
           load_scores64(tS + 64 * h, s);
-          if constexpr (SOFTCAP) soft_cap_scores(s, cap_in, cap_out);
+          if constexpr (SOFTCAP) {
+            // The largest score decides the form of the row's soft-cap: not one that the row does not see, of a key that was never
+            // loaded even.
+            if (masked) zero_not_allowed64(allow[2 * h], allow[2 * h + 1], s);
+            soft_cap_scores(s, cap_in, cap_out);
+          }
           if (masked) apply_allow64(allow[2 * h], allow[2 * h + 1], s);
           if constexpr (SOFTCAP) {
             uint32_t w[32];

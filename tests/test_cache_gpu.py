@@ -205,6 +205,29 @@ def test_append_without_rotation_stores_what_it_is_given(cuda_device, D, dtype):
         assert torch.equal(got.nan_to_num(nan=7.0), given.nan_to_num(nan=7.0))
 
 
+@pytest.mark.parametrize("softcap", [50.0, None])
+@pytest.mark.parametrize("H,T,causal", [(2, 1, True), (4, 3, True), (16, 1, True), (24, 2, True), (4, 30, False), (3, 40, True)])
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16), (32, torch.float16)])
+def test_what_nobody_sees_changes_no_bit(cuda_device, D, dtype, H, T, causal, softcap):
+    """Pages behind the tokens, queries of padding, and what ran before: zeros, large numbers, infinities or NaN there, the same bits."""
+    B, page, lengths, counts = 3, 16, [37, 5, 300], torch.tensor([T, (T + 1) // 2, T], dtype=torch.int32)
+    results = []
+    big = make_cache(2, 1, D, page, [900, 700], T, dtype, seed=8, stale=0.0)
+    for stale in (0.0, 300.0, -1e4, math.nan, math.inf):
+        kp, vp, table, lens, g = make_cache(B, 1, D, page, lengths, T, dtype, seed=7, stale=stale)
+        q = torch.randn(B, H, T, D, generator=g).to(dtype)
+        for b, c in enumerate(counts.tolist()):
+            q[b, :, c:] = stale
+            for i in range(lengths[b] + c, lengths[b] + T):
+                kp[int(table[b, i // page]), :, i % page] = stale
+                vp[int(table[b, i // page]), :, i % page] = stale
+        if stale != 0.0:    # what shared memory holds
+            omni.omni_cache_attention(torch.full((2, H, T, D), 100.0, dtype=dtype, device="cuda"), on_gpu(big[0] * 100, big[1] * 100, *big[2:4]))
+        results.append(omni.omni_cache_attention(q.cuda(), on_gpu(kp, vp, table, lens), counts=counts.cuda(), causal=causal, softcap=softcap, return_lse=True))
+    for out, lse in results[1:]:
+        assert torch.equal(out, results[0][0]) and torch.equal(lse, results[0][1])
+
+
 def same_kinds(got, want, tol, what):
     """Infinite with the sign, NaN and finite where the definition says so; the finite ones within tol."""
     got = got.double().cpu()
