@@ -113,7 +113,7 @@ def _attention_forward_with_omni_core(module, original_forward):
             if dtype not in (torch.float16, torch.bfloat16):   # the kernels compute on 16-bit operands
                 q, k, v = (t.to(cache.k_pages.dtype if paged else torch.bfloat16) for t in (q, k, v))
             if paged:
-                omni_cache_append(cache, k, v)
+                omni_cache_append(cache, k.to(cache.k_pages.dtype), v.to(cache.k_pages.dtype))
             out = transfusion_attention_core(q.contiguous(), k.contiguous(), v.contiguous(), block_mask,
                                              softcap_value=float(module.softcap_value), scale=float(module.scale)).to(dtype)
         if getattr(module, "laser", False):

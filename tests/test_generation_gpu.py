@@ -77,6 +77,38 @@ def test_prompt_text_and_image(cuda_device, dim_head, layout, page):
     unpatch_attention(mod)
 
 
+def prompt_and_cache(module_dtype, cache_dtype, rot, weight=None, n=50, heads=2, dim_head=64):
+    """(module, x, mask, empty cache, the prompt's stored keys and values as [b, h, n, d])"""
+    torch.manual_seed(4)
+    mod = patch_attention(AttentionLike(96, dim_head, heads, learned_mix=False)).to("cuda").to(module_dtype)
+    x = torch.randn(2, n, 96, device="cuda").to(module_dtype)
+    mask = transfusion_block_mask(torch.tensor([[[1, 10, 20]], [[1, 0, 7]]], dtype=torch.int32).cuda(), heads, n)
+    cache = omni.OmniPagedCache.allocate(8, heads, 16, dim_head, 2, 4, cache_dtype)
+    cache.page_table.copy_(torch.arange(8, device="cuda").view(2, 4))
+    stored = lambda pages: pages.view(2, 4, heads, 16, dim_head).transpose(1, 2).reshape(2, heads, 64, dim_head)[:, :, :n]
+    return mod, x, mask, cache, stored
+
+
+DTYPES = [(m, c) for m in (torch.float16, torch.bfloat16, torch.float32) for c in (torch.float16, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("module_dtype,cache_dtype", DTYPES)
+def test_prompt_and_text_with_a_module_and_a_cache_of_any_dtype(cuda_device, module_dtype, cache_dtype):
+    rot = omni.OmniRotary.from_base(64, device="cuda")
+    mod, x, mask, cache, stored = prompt_and_cache(module_dtype, cache_dtype, rot)
+    with torch.no_grad():
+        want = mod(x, block_mask=mask, rotary_emb=rot.at())      # the same without a cache
+        got = mod(x, block_mask=mask, rotary_emb=rot.at(), cache=cache)
+        assert got.dtype == module_dtype
+        if module_dtype != torch.float32:     # (an fp32 module's core is computed in the cache's dtype)
+            assert torch.equal(got, want)
+        k = omni.omni_rotary(None, mod.to_qk(x)[1], rot)[1]
+        assert torch.equal(stored(cache.k_pages), k.to(cache_dtype)) and torch.equal(stored(cache.v_pages), mod.to_v(x).to(cache_dtype))
+        cache.lengths += 50
+        one = mod(x[:, :1], rotary_emb=rot.at(torch.full((2, 1), 50, device="cuda")), cache=cache, causal=True)
+        assert one.dtype == module_dtype and torch.isfinite(one).all()
+
+
 def test_training_through_norms_and_rotation(cuda_device):
     torch.manual_seed(2)
     b, n, dim, heads, dh = 1, 200, 64, 2, 64
