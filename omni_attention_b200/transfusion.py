@@ -72,7 +72,13 @@ def _attention_forward_with_omni_core(module, original_forward):
 
     def cached_core(q, k, v, rotary_emb, cache, causal):
         at = rotary_emb if isinstance(rotary_emb, RotaryAt) else None
-        if rotary_emb is not None and at is None:
+        if at is not None and q.dtype != cache.k_pages.dtype:
+            # normed and turned in the module's dtype and rounded after that, as the prompt's keys are
+            if at.positions is None:
+                at = at._replace(positions=cache.lengths.clamp(min=0)[:, None] + torch.arange(q.shape[2], dtype=torch.int32, device=q.device))
+            q, k = rotated(q, k, at)
+            at = None
+        elif rotary_emb is not None and at is None:
             q, k = rotated(q, k, rotary_emb)
         q, k, v = (t.to(cache.k_pages.dtype) for t in (q, k, v))
         if at is None:

@@ -109,6 +109,32 @@ def test_prompt_and_text_with_a_module_and_a_cache_of_any_dtype(cuda_device, mod
         assert one.dtype == module_dtype and torch.isfinite(one).all()
 
 
+@pytest.mark.parametrize("module_dtype,cache_dtype", DTYPES)
+@pytest.mark.parametrize("given", [True, False])
+def test_keys_are_the_same_from_a_prompt_and_from_tokens(cuda_device, module_dtype, cache_dtype, given):
+    """The same tokens through the block mask and through generation leave the same bits in the cache (norm, rotation, one
+    rounding to the cache's dtype), whether their positions are given or follow from the cache's lengths."""
+    rot = omni.OmniRotary.from_base(64, device="cuda")
+    w = 1 + 0.2 * torch.randn(64, device="cuda")
+    mod, x, mask, cache, stored = prompt_and_cache(module_dtype, cache_dtype, rot)
+    positions = torch.arange(50, device="cuda").expand(2, 50).contiguous()
+    at = lambda lo, hi: rot.at(positions[:, lo:hi] if given else None, w, w)
+    with torch.no_grad():
+        mod(x, block_mask=mask, rotary_emb=rot.at(positions, w, w), cache=cache)
+        k, v = stored(cache.k_pages).clone(), stored(cache.v_pages).clone()
+        cache.k_pages.zero_(), cache.v_pages.zero_()
+        for lo, hi in ((0, 20), (20, 50)):
+            mod(x[:, lo:hi], rotary_emb=at(lo, hi), cache=cache, causal=True)
+            cache.lengths += hi - lo
+        # the projections of 20 and 30 tokens may differ from those of 50 in their last bits: compared on the module's own k
+        own = torch.cat([mod.to_qk(x[:, lo:hi])[1] for lo, hi in ((0, 20), (20, 50))], 2)
+        own_v = torch.cat([mod.to_v(x[:, lo:hi]) for lo, hi in ((0, 20), (20, 50))], 2)
+        want = omni.omni_rotary(None, own, rot, positions, None, w)[1].to(cache_dtype)
+        assert torch.equal(stored(cache.k_pages), want) and torch.equal(stored(cache.v_pages), own_v.to(cache_dtype))
+        if torch.equal(own, mod.to_qk(x)[1]):
+            assert torch.equal(k, want)
+
+
 def test_training_through_norms_and_rotation(cuda_device):
     torch.manual_seed(2)
     b, n, dim, heads, dh = 1, 200, 64, 2, 64
