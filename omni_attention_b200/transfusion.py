@@ -24,7 +24,7 @@ from torch import Tensor
 
 from .block_mask import OmniBlockMask, create_omni_block_mask_from_modality_positions
 from .cache import OmniPagedCache, omni_cache_append, omni_cache_attention
-from .ops import omni_attention, omni_attention_autograd
+from .ops import OmniAttnError, omni_attention, omni_attention_autograd
 from .rotary import RotaryAt, omni_rotary
 
 
@@ -57,8 +57,9 @@ def _attention_forward_with_omni_core(module, original_forward):
 
     With an OmniPagedCache the x of the call are the sequences' new tokens: their keys and values are stored behind the
     cache's ``lengths`` (which the caller moves on after the last layer) and they attend to the cache and to each other,
-    ``causal`` or all of them (an image that is denoised). With a block mask as well it is the prompt, on an empty
-    cache: its tokens attend to each other by the mask and are stored."""
+    ``causal`` or all of them (an image that is denoised). With a block mask as well it is the prompt, which must find the
+    cache empty: its tokens attend to each other by the mask, to nothing before them, and are stored. Whether the cache is
+    empty, and whether all tokens found their pages, is looked at where ``patch_attention`` was told ``check_status``."""
 
     def rotated(q, k, rotary_emb):
         if isinstance(rotary_emb, RotaryAt):
@@ -82,11 +83,13 @@ def _attention_forward_with_omni_core(module, original_forward):
             q, k = rotated(q, k, rotary_emb)
         q, k, v = (t.to(cache.k_pages.dtype) for t in (q, k, v))
         if at is None:
-            omni_cache_append(cache, k, v)
+            omni_cache_append(cache, k, v, check_status=module._omni_check_status)
         else:
-            q = omni_cache_append(cache, k, v, q, at.rotary, at.positions, None, at.q_weight, at.k_weight, at.eps)
+            q = omni_cache_append(cache, k, v, q, at.rotary, at.positions, None, at.q_weight, at.k_weight, at.eps,
+                                  check_status=module._omni_check_status)
         cap = float(module.softcap_value)
-        return omni_cache_attention(q, cache, causal=causal, scale=float(module.scale), softcap=cap if cap > 0 else None)
+        return omni_cache_attention(q, cache, causal=causal, scale=float(module.scale), softcap=cap if cap > 0 else None,
+                                    check_status=module._omni_check_status)
 
     def forward(x, attn_mask=None, rotary_emb=None, cache=None, causal=False, block_mask=None,
                 return_kv_cache=False, return_values=False, value_residual=None):
@@ -99,6 +102,9 @@ def _attention_forward_with_omni_core(module, original_forward):
             return original_forward(x, attn_mask=attn_mask, rotary_emb=rotary_emb, cache=cache, causal=causal,
                                     block_mask=block_mask, return_kv_cache=return_kv_cache, return_values=return_values,
                                     value_residual=value_residual)
+        if masked and paged and module._omni_check_status and bool((cache.lengths > 0).any()):
+            raise OmniAttnError("a prompt (a call with an OmniBlockMask) attends to its own tokens only: the cache must be empty, but "
+                                f"its lengths are {cache.lengths.tolist()}")
         q, k = module.to_qk(x)
         v = module.to_v(x)
         orig_v = v
@@ -119,7 +125,7 @@ def _attention_forward_with_omni_core(module, original_forward):
             if dtype not in (torch.float16, torch.bfloat16):   # the kernels compute on 16-bit operands
                 q, k, v = (t.to(cache.k_pages.dtype if paged else torch.bfloat16) for t in (q, k, v))
             if paged:
-                omni_cache_append(cache, k.to(cache.k_pages.dtype), v.to(cache.k_pages.dtype))
+                omni_cache_append(cache, k.to(cache.k_pages.dtype), v.to(cache.k_pages.dtype), check_status=module._omni_check_status)
             out = transfusion_attention_core(q.contiguous(), k.contiguous(), v.contiguous(), block_mask,
                                              softcap_value=float(module.softcap_value), scale=float(module.scale)).to(dtype)
         if getattr(module, "laser", False):
@@ -136,7 +142,7 @@ def _attention_forward_with_omni_core(module, original_forward):
     return forward
 
 
-def patch_attention(module):
+def patch_attention(module, check_status: bool = False):
     """Swap the attention core of ``module`` for the kernels. ``module`` is the reference's
     ``transfusion_pytorch.transfusion.Attention`` or anything with the same attributes: ``to_qk`` (x ->
     q, k as [b, h, n, d]), ``to_v``, ``to_out``, ``scale``, ``softcap_value`` and, optionally,
@@ -144,6 +150,8 @@ def patch_attention(module):
     is not applied by the kernels: a module whose ``dropout.p`` is non-zero in training mode is refused.
     The mask arrives through the ``block_mask`` argument the reference's forward already has, as an
     OmniBlockMask (``transfusion_block_mask``), a paged cache through ``cache``, the positions through ``rotary_emb``.
+    ``check_status=True``: calls with a paged cache wait for the GPU and raise where a prompt meets a cache that is not empty
+    or a token's page is not there (not while a CUDA graph is captured). A second patch of the same module changes that only.
     Returns the module; ``unpatch_attention`` undoes it."""
     for name in ("to_qk", "to_v", "to_out", "scale", "softcap_value"):
         if not hasattr(module, name):
@@ -151,6 +159,7 @@ def patch_attention(module):
     drop = getattr(module, "dropout", None)
     if drop is not None and getattr(drop, "p", 0.0) > 0.0 and getattr(module, "training", False):
         raise ValueError("patch_attention: attention dropout is not supported by the kernels (set dropout to 0 or eval())")
+    module._omni_check_status = bool(check_status)
     if hasattr(module, "_omni_original_forward"):
         return module
     module._omni_original_forward = module.forward
@@ -161,5 +170,5 @@ def patch_attention(module):
 def unpatch_attention(module):
     if hasattr(module, "_omni_original_forward"):
         module.forward = module._omni_original_forward
-        del module._omni_original_forward
+        del module._omni_original_forward, module._omni_check_status
     return module

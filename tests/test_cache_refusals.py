@@ -265,3 +265,22 @@ def test_c_entries_return_codes():
     for name in ("OMNI_ERR_ROTARY", "OMNI_ERR_CACHE"):
         lib.omni_attn_error_string.restype = ctypes.c_char_p
         assert lib.omni_attn_error_string(E[name]) != b"unknown error code"
+
+
+def test_a_prompt_on_a_cache_that_is_not_empty():
+    """The slot's own check, where it was asked for: before anything is computed."""
+    from omni_attention_b200.transfusion import patch_attention, transfusion_block_mask, unpatch_attention
+    from test_transfusion_gpu import AttentionLike
+    mod = AttentionLike(32, 64, 2, learned_mix=False)
+    mask = transfusion_block_mask(torch.tensor([[[1, 2, 3]], [[1, 0, 5]]], dtype=i32), 2, 128)
+    c, x = cache(), torch.randn(2, 128, 32)
+    c.lengths[1] = 3
+    with torch.no_grad():
+        assert patch_attention(mod, check_status=True) is mod
+        refused("must be empty", mod, x, block_mask=mask, cache=c)
+        patch_attention(mod)                        # not asked for any more: the next complaint is that there is no GPU
+        refused("CUDA", mod, x, block_mask=mask, cache=c)
+        patch_attention(mod, check_status=True)
+        c.lengths.zero_()
+        refused("CUDA|cuda", mod, x, block_mask=mask, cache=c, error=(OmniAttnError, RuntimeError))
+    assert unpatch_attention(mod) is mod and not hasattr(mod, "_omni_check_status")

@@ -135,6 +135,25 @@ def test_keys_are_the_same_from_a_prompt_and_from_tokens(cuda_device, module_dty
             assert torch.equal(k, want)
 
 
+def test_a_checked_slot(cuda_device):
+    """check_status: the same results, and an error for a prompt on a cache that is not empty or a page that is not there."""
+    rot = omni.OmniRotary.from_base(64, device="cuda")
+    mod, x, mask, cache, stored = prompt_and_cache(torch.float16, torch.float16, rot)
+    with torch.no_grad():
+        want = mod(x, block_mask=mask, rotary_emb=rot.at(), cache=cache)
+        patch_attention(mod, check_status=True)
+        assert torch.equal(mod(x, block_mask=mask, rotary_emb=rot.at(), cache=cache), want)
+        cache.lengths += 50
+        mod(x[:, :1], rotary_emb=rot.at(), cache=cache, causal=True)
+        with pytest.raises(omni.OmniAttnError, match="must be empty"):
+            mod(x, block_mask=mask, rotary_emb=rot.at(), cache=cache)
+        cache.page_table[1, 3] = -1
+        with pytest.raises(omni.OmniAttnError, match="page_table"):
+            mod(x[:, :1], rotary_emb=rot.at(), cache=cache, causal=True)
+        patch_attention(mod)
+        mod(x[:, :1], rotary_emb=rot.at(), cache=cache, causal=True)
+
+
 def test_training_through_norms_and_rotation(cuda_device):
     torch.manual_seed(2)
     b, n, dim, heads, dh = 1, 200, 64, 2, 64
