@@ -260,6 +260,7 @@ pybind11::tuple rotary(const Optional& q_in, const Optional& k_in, const Optiona
               "q and k must share dtype, batch, length and head_dim: " + shape_of(q) + " and " + shape_of(k));
     }
     check_rotary_args(r, q, k);
+    OMNI_REQUIRE(!wants_grad({&r.inv_freq}), "omni_rotary has no gradient of inv_freq: detach it, or call it under torch.no_grad()");
     check_device(q.defined() ? q : k, {&q, &k, &r.inv_freq, &r.positions, &r.q_weight, &r.k_weight});
     if (q.defined()) q = with_rows(q);
     if (k.defined()) k = with_rows(k);
@@ -324,7 +325,7 @@ pybind11::object cache_append(const torch::Tensor& k_pages, const torch::Tensor&
     OMNI_REQUIRE(cache.heads == k.size(1), "the cache's heads are not those of k");
     const int32_t* counts_ptr = int32_or_null(counts, {B}, "counts must be contiguous int32 [B]");
     int32_t* status_ptr = const_cast<int32_t*>(int32_or_null(status, {1}, "status must be int32 [1]"));
-    OMNI_REQUIRE(!wants_grad({&q, &k, &v, &r.q_weight, &r.k_weight}),
+    OMNI_REQUIRE(!wants_grad({&q, &k, &v, &r.q_weight, &r.k_weight, &r.inv_freq}),
             "omni_cache_append has no backward: call it under torch.no_grad(), or on tensors that need no gradient");
     check_device(k, {&v, &q, &k_pages, &v_pages, &table, &lengths, &counts, &status, &r.inv_freq, &r.positions, &r.q_weight, &r.k_weight});
     at::AutoDispatchBelowADInplaceOrView below;

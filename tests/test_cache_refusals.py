@@ -267,6 +267,16 @@ def test_c_entries_return_codes():
         assert lib.omni_attn_error_string(E[name]) != b"unknown error code"
 
 
+def test_learned_frequencies():
+    """Nothing here has a gradient of inv_freq: refused where one is asked for."""
+    r = omni.OmniRotary(torch.ones(32, dtype=torch.float64).requires_grad_())
+    refused("inv_freq", omni.omni_rotary, t(1, 1, 3, 64), None, r)
+    refused("inv_freq", omni.omni_rotary, t(1, 1, 3, 64).requires_grad_(), None, r)
+    refused("no backward", omni.omni_cache_append, cache(), t(2, 2, 3, 64), t(2, 2, 3, 64), rotary=r)
+    with torch.no_grad():
+        refused("CUDA", omni.omni_rotary, t(1, 1, 3, 64), None, r)
+
+
 def test_a_prompt_on_a_cache_that_is_not_empty():
     """The slot's own check, where it was asked for: before anything is computed."""
     from omni_attention_b200.transfusion import patch_attention, transfusion_block_mask, unpatch_attention
