@@ -243,6 +243,13 @@ bool wants_grad(std::initializer_list<const torch::Tensor*> ts) {
   return false;
 }
 
+// A tangent of forward-mode differentiation would be dropped: the kernels' results have none.
+void check_no_tangent(const char* what, std::initializer_list<const torch::Tensor*> ts) {
+  for (const torch::Tensor* t : ts) {
+    OMNI_REQUIRE(!t->defined() || !t->_fw_grad(0).defined(), std::string(what) + " has no forward-mode derivative: an input carries a tangent");
+  }
+}
+
 pybind11::object result(const torch::Tensor& t) { return t.defined() ? pybind11::cast(t) : pybind11::object(pybind11::none()); }
 
 pybind11::tuple rotary(const Optional& q_in, const Optional& k_in, const Optional& inv_freq, bool half, double factor,
@@ -261,6 +268,7 @@ pybind11::tuple rotary(const Optional& q_in, const Optional& k_in, const Optiona
     }
     check_rotary_args(r, q, k);
     OMNI_REQUIRE(!wants_grad({&r.inv_freq}), "omni_rotary has no gradient of inv_freq: detach it, or call it under torch.no_grad()");
+    check_no_tangent("omni_rotary", {&q, &k, &r.q_weight, &r.k_weight, &r.inv_freq});
     check_device(q.defined() ? q : k, {&q, &k, &r.inv_freq, &r.positions, &r.q_weight, &r.k_weight});
     if (q.defined()) q = with_rows(q);
     if (k.defined()) k = with_rows(k);
@@ -327,6 +335,7 @@ pybind11::object cache_append(const torch::Tensor& k_pages, const torch::Tensor&
     int32_t* status_ptr = const_cast<int32_t*>(int32_or_null(status, {1}, "status must be int32 [1]"));
     OMNI_REQUIRE(!wants_grad({&q, &k, &v, &r.q_weight, &r.k_weight, &r.inv_freq}),
             "omni_cache_append has no backward: call it under torch.no_grad(), or on tensors that need no gradient");
+    check_no_tangent("omni_cache_append", {&q, &k, &v, &r.q_weight, &r.k_weight, &r.inv_freq, &k_pages, &v_pages});
     check_device(k, {&v, &q, &k_pages, &v_pages, &table, &lengths, &counts, &status, &r.inv_freq, &r.positions, &r.q_weight, &r.k_weight});
     at::AutoDispatchBelowADInplaceOrView below;
     c10::cuda::CUDAGuard guard(k.device());
@@ -370,6 +379,7 @@ pybind11::object cache_attention(torch::Tensor q, const torch::Tensor& k_pages, 
     OMNI_REQUIRE(shared_prefix >= 0 && shared_prefix <= table.size(1) * k_pages.size(2), "shared_prefix must be from 0 to the tokens that the page table holds");
     OMNI_REQUIRE(!wants_grad({&q, &k_pages, &v_pages}),
             "omni_cache_attention has no backward: call it under torch.no_grad(), or on tensors that need no gradient");
+    check_no_tangent("omni_cache_attention", {&q, &k_pages, &v_pages});
     check_device(q, {&k_pages, &v_pages, &table, &lengths, &counts, &limits, &status});
     at::AutoDispatchBelowADInplaceOrView below;
     c10::cuda::CUDAGuard guard(q.device());

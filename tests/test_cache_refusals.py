@@ -277,6 +277,27 @@ def test_learned_frequencies():
         refused("CUDA", omni.omni_rotary, t(1, 1, 3, 64), None, r)
 
 
+def test_forward_mode():
+    """A tangent is refused, whether something requires a gradient or not: it would be dropped."""
+    from torch.autograd import forward_ad as fw
+    r = omni.OmniRotary.from_base(64)
+    q, k, c = t(2, 4, 3, 64), t(2, 2, 3, 64), cache()
+    with fw.dual_level():
+        d = lambda x: fw.make_dual(x, torch.ones_like(x))
+        for grad in (False, True):
+            refused("forward-mode", omni.omni_rotary, d(q), k.clone().requires_grad_(grad), r)
+        refused("forward-mode", omni.omni_rotary, q, d(k), r)
+        refused("forward-mode", omni.omni_rotary, q, k, r, None, d(t(64)), t(64))
+        refused("forward-mode", omni.omni_rotary, q, k, omni.OmniRotary(d(r.inv_freq)))
+        for args in ((d(k), k, q), (k, d(k), q), (k, k, d(q))):
+            refused("forward-mode", omni.omni_cache_append, c, *args)
+        refused("forward-mode", omni.omni_cache_attention, d(q), c)
+        c2 = omni.OmniPagedCache(c.k_pages, d(c.v_pages), c.page_table, c.lengths)
+        refused("forward-mode", omni.omni_cache_attention, q, c2)
+        refused("CUDA", omni.omni_rotary, q, k, r)
+    refused("CUDA", omni.omni_cache_append, c, k, k, q)
+
+
 def test_a_prompt_on_a_cache_that_is_not_empty():
     """The slot's own check, where it was asked for: before anything is computed."""
     from omni_attention_b200.transfusion import patch_attention, transfusion_block_mask, unpatch_attention
