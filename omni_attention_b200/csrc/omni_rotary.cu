@@ -272,31 +272,60 @@ __device__ __forceinline__ void load_weight(const void* w, bool f32, int row, co
   }
 }
 
-// Cosines and sines of the thread's pairs at a position, with the factor; 1 and 0 for what is not rotated.
 struct Turn {
   float2 c[4], s[4];
 };
-// EXACT: sincospif (an ulp or two); else the special function unit's sine and cosine of an angle within half a turn, off by
-// 2^-21, which a 16-bit result does not show and takes a tenth of the instructions.
+// Cosines and sines of two angles given in turns, at most half a turn: Taylor's series about the nearest quarter turn, |x| <= pi / 4,
+// to x^9 and x^10 (what is left out is below 2^-28). The turns are off by 2^-26, which is 2^-23.4 of an angle; x by its product's
+// rounding and 2 pi's, 2^-25 each; the sums by 2^-24: together less than 2^-22 (on 8 million angles 2^-22.7).
+__device__ __forceinline__ void sincos_turns(float2 turns, float2& sn, float2& cs) {
+  auto both = [](float v) { return make_float2(v, v); };
+  constexpr float kBig = 12582912.f;   // 1.5 * 2^23: a sum with it is rounded to whole numbers
+  const float2 sum = __ffma2_rn(turns, both(4.f), both(kBig));
+  const float2 quarters = __fadd2_rn(sum, both(-kBig));
+  const float2 x = __fmul2_rn(__ffma2_rn(quarters, both(-0.25f), turns), both(6.2831853071795865f));
+  const float2 z = __fmul2_rn(x, x);
+  float2 s = __ffma2_rn(z, both(1.f / 362880.f), both(-1.f / 5040.f));
+  s = __ffma2_rn(s, z, both(1.f / 120.f));
+  s = __ffma2_rn(s, z, both(-1.f / 6.f));
+  s = __ffma2_rn(__fmul2_rn(s, z), x, x);
+  float2 c = __ffma2_rn(z, both(-1.f / 3628800.f), both(1.f / 40320.f));
+  c = __ffma2_rn(c, z, both(-1.f / 720.f));
+  c = __ffma2_rn(c, z, both(1.f / 24.f));
+  c = __ffma2_rn(c, z, both(-0.5f));
+  c = __ffma2_rn(c, z, both(1.f));
+  auto place = [](int k, float s1, float c1, float& sin_out, float& cos_out) {
+    const float a = k & 1 ? c1 : s1, b = k & 1 ? s1 : c1;
+    sin_out = k & 2 ? -a : a;
+    cos_out = (k + 1) & 2 ? -b : b;
+  };
+  place(__float_as_int(sum.x), s.x, c.x, sn.x, cs.x);
+  place(__float_as_int(sum.y), s.y, c.y, sn.y, cs.y);
+}
+// Cosines and sines of the thread's pairs at a position, with the factor. EXACT: as above, for results in 32 bits: fp32 data, and
+// gradients of weights, which may be fp32 whatever the data's type. Else the special function unit's sine and cosine, which take
+// fewer instructions: the unit's own 2^-21.2 for angles within half a turn, 2^-23.4 of the turns, 2^-23 of the product with 2 pi and
+// 2^-23.4 of 2 pi itself, less than 2^-20.4 together. Forward, bf16, head_dim 128: 64 heads of 8 192 tokens 47.3 us EXACT and 46.9,
+// 8 heads of 65 536 53.3 and 51.0, 2 heads of 262 144 92.6 and 84.4.
 template <bool EXACT, int D, bool HALF>
 __device__ __forceinline__ void turn_of(const RotaryParams& p, const Place<D, HALF>& at, long long pos, Turn& r) {
   const double t = static_cast<double>(pos) * 0.15915494309189533577;   // 1 / (2 pi)
+  auto turns_of = [&](int j) {
+    if (at.pair(j) >= at.rd2) return 0.f;   // (not used)
+    const double turns = t * __ldg(p.inv_freq + at.pair(j));
+    return static_cast<float>(turns - rint(turns));
+  };
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float sn = 0.f, cs = 1.f;
-    if (at.pair(j) < at.rd2) {
-      double turns = t * __ldg(p.inv_freq + at.pair(j));
-      turns -= rint(turns);
-      if constexpr (EXACT) {
-        sincospif(2.f * static_cast<float>(turns), &sn, &cs);
-      } else {
-        __sincosf(6.2831853071795865f * static_cast<float>(turns), &sn, &cs);
-      }
-      cs *= p.factor;
-      sn *= p.factor * p.sign;
+  for (int i = 0; i < 4; ++i) {
+    const float2 turns = make_float2(turns_of(2 * i), turns_of(2 * i + 1));
+    if constexpr (EXACT) {
+      sincos_turns(turns, r.s[i], r.c[i]);
+    } else {
+      __sincosf(6.2831853071795865f * turns.x, &r.s[i].x, &r.c[i].x);
+      __sincosf(6.2831853071795865f * turns.y, &r.s[i].y, &r.c[i].y);
     }
-    (j & 1 ? r.c[j >> 1].y : r.c[j >> 1].x) = cs;
-    (j & 1 ? r.s[j >> 1].y : r.s[j >> 1].x) = sn;
+    r.c[i] = __fmul2_rn(r.c[i], make_float2(p.factor, p.factor));
+    r.s[i] = __fmul2_rn(r.s[i], make_float2(p.factor * p.sign, p.factor * p.sign));
   }
 }
 // Pairs behind the rotated part pass through as they are (a turn by cosine 1 and sine 0 would make the neighbour of an infinite
@@ -458,7 +487,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_kernel(cons
           norm = sg.w != nullptr;
           if (norm) load_weight<T, D, HALF, VEC>(sg.w, p.w_f32, p.w_per_head ? hl : 0, at, w);
           if (seg < 2 && !turned) {
-            turn_of<sizeof(T) == 4, D, HALF>(p, at, position_of(p, b, n), turn);
+            turn_of<sizeof(T) == 4>(p, at, position_of(p, b, n), turn);
             turned = true;
           }
         }
@@ -575,7 +604,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_bwd_kernel(
     };
 #pragma unroll 1
     for (int i = 0; i < kStages - 1; ++i) read_ahead(i);
-    turn_of<sizeof(T) == 4, D, HALF>(p, at, position_of(p, b, n), turn);   // sign = -1: the rotation back
+    turn_of<true>(p, at, position_of(p, b, n), turn);   // sign = -1: the rotation back
 #pragma unroll 1
     for (int i = 0; i < n_rows; ++i) {
       Pairs v, d;

@@ -89,6 +89,29 @@ def test_forward_and_backward(cuda_device, B, H, Hkv, N, D, rd, layout, norm, dt
         check(grads[2 + i], rw.grad, w.dtype, 0.2 * full, f"d{name}_weight")
 
 
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_gradients_of_fp32_weights_have_exact_angles(cuda_device, dtype, layout):
+    """A row of ones without eps has the norm 1, and the gradient (1, 0) of each pair makes the weight's gradient the pair's cosine
+    and minus its sine, with no rounding beside theirs: in 32 bits, whatever the data's dtype. A cosine or sine is off by less
+    than 2^-22 (see above)."""
+    D, calls = 128, 200
+    rot = omni.OmniRotary.from_base(D, layout=layout, device="cuda")
+    first = (slice(0, D, 2), slice(1, D, 2)) if layout == "interleaved" else (slice(0, D // 2), slice(D // 2, D))
+    x = torch.ones(1, 1, 1, D, dtype=dtype, device="cuda")
+    g = torch.zeros_like(x)
+    g[..., first[0]] = 1
+    positions = torch.randint(0, 100000, (calls, 1), generator=torch.Generator().manual_seed(2))
+    worst = 0.0
+    for pos in positions:
+        w = torch.ones(D, device="cuda", requires_grad=True)
+        dw, = torch.autograd.grad(omni.omni_rotary(x, None, rot, pos.cuda(), w, eps=0.0)[0], w, g)
+        a = pos.double() * rot.inv_freq.cpu()
+        dw = dw.double().cpu()
+        worst = max(worst, float((dw[first[0]] - a.cos()).abs().max()), float((dw[first[1]] + a.sin()).abs().max()))
+    assert worst <= 2.0 ** -22, f"2^{math.log2(worst):.2f}"
+
+
 @pytest.mark.parametrize("where", [0, 1 << 20, 3_000_000_000])
 @pytest.mark.parametrize("layout", ["interleaved", "half"])
 def test_far_positions_are_as_exact_as_near_ones(cuda_device, where, layout):
