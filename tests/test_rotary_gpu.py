@@ -112,6 +112,29 @@ def test_gradients_of_fp32_weights_have_exact_angles(cuda_device, dtype, layout)
     assert worst <= 2.0 ** -22, f"2^{math.log2(worst):.2f}"
 
 
+@pytest.mark.parametrize("norm", [None, "shared", "head"])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_sixteen_bit_results(cuda_device, dtype, layout, norm):
+    """fp16 and bf16 results use the special function unit: a cosine or sine is off by 2^-21.2 (the unit's own error within half a
+    turn), 2^-23.4 (the turns in 32 bits), 2^-23 (their product with 2 pi) and 2^-23.4 (2 pi itself), less than 2^-20.4 together. The
+    norm's factor adds 2^-22, two products and a sum 3 * 2^-24: less than 2^-19.7 of |u| + |v| for the pair (u, v), then the rounding."""
+    D = 128
+    q, _, w, _ = make(2, 3, 1, 300, D, dtype, norm, torch.float32, seed=11)
+    pos = torch.randint(0, 200000, (2, 300), generator=torch.Generator().manual_seed(12))
+    rot = omni.OmniRotary.from_base(D, layout=layout, device="cuda")
+    got, _ = omni.omni_rotary(q.cuda(), None, rot, pos.cuda(), None if w is None else w.cuda())
+    want = orc.rotate(q, pos, rot.inv_freq.cpu(), layout, 1.0, w)
+    before = orc.rotate(q, pos, None, weight=w).abs()
+    if layout == "interleaved":
+        terms = (before[..., 0::2] + before[..., 1::2]).repeat_interleave(2, -1)
+    else:
+        terms = (before[..., :D // 2] + before[..., D // 2:]).repeat(1, 1, 1, 2)
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -19.7 * terms + (2.0 ** -25 if dtype == torch.float16 else 0)
+    worst = float(((got.double().cpu() - want).abs() / tol).max())
+    assert worst <= 1.0, f"{worst:.3g} times the tolerance"
+
+
 @pytest.mark.parametrize("where", [0, 1 << 20, 3_000_000_000])
 @pytest.mark.parametrize("layout", ["interleaved", "half"])
 def test_far_positions_are_as_exact_as_near_ones(cuda_device, where, layout):
