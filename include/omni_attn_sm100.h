@@ -53,7 +53,7 @@ extern "C" {
 #define OMNI_ERR_CUDA (-10)            /* a CUDA runtime/driver call failed; see omni_attn_last_cuda_error() */
 #define OMNI_ERR_NO_DRIVER_ENTRY (-11) /* cuTensorMapEncodeTiled is not available from the driver */
 #define OMNI_ERR_SCRATCH (-12)         /* scratch buffer smaller than OMNI_ATTN_SCRATCH_BYTES */
-#define OMNI_ERR_SOFTCAP (-14)         /* softcap negative or NaN */
+#define OMNI_ERR_SOFTCAP (-14)         /* softcap negative or NaN; over a paged cache also out of range */
 #define OMNI_ERR_WORKSPACE (-15)       /* omni_attn_bwd_sm100: workspace smaller than omni_attn_bwd_workspace_bytes() */
 #define OMNI_ERR_ROTARY (-16)          /* rotary_dim odd, negative or above head_dim, or no inv_freq for one that is not 0 */
 #define OMNI_ERR_CACHE (-17)           /* paged cache: sizes not positive, page_size no power of two from 16 to 1024, or heads that do not divide the queries' */
@@ -390,7 +390,8 @@ int omni_attn_cache_append_sm100(const omni_attn_heads* q, const omni_attn_heads
  * rows whose limit is not positive, are zero with LSE -inf.
  *  q              in  [B, H, T, head_dim] fp16 or bf16, rows 16-byte aligned
  *  out            out [B, H, T, head_dim] contiguous; lse [B, H, T] fp32, natural log, or NULL
- *  softcap        tanh soft-cap of the scaled scores, 0 = none; scale <= 0: head_dim ** -0.5
+ *  softcap        tanh soft-cap of the scaled scores, 0 = none, else from 1e-6 to 1e30 times the scale and at most 1e37;
+ *                 scale <= 0: head_dim ** -0.5
  *  shared_prefix  the first that many tokens of all sequences are in the same pages (rounded down to whole pages): they
  *                 are read once for the batch. 0 = nothing is known to be shared. With a status word, table entries that
  *                 break the promise are reported as OMNI_STATUS_BAD_INDEX.

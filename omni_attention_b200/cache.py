@@ -116,7 +116,7 @@ def omni_cache_attention(q: Tensor, cache: OmniPagedCache, counts: Optional[Tens
     b attends its first ``cache.lengths[b] + t + 1`` tokens, with ``causal=False`` all ``cache.lengths[b] + counts[b]`` of
     them, with ``limits`` (int32 [B, T]) its first ``limits[b, t]``. Rows behind a sequence's count (``counts`` int32 [B],
     None = T) and rows with no key are zero (LSE -inf). ``scale`` (positive) defaults to D ** -0.5, ``softcap`` > 0 caps the scaled
-    scores with tanh. ``shared_prefix``: that many first tokens of all sequences are in the same pages (a prompt with
+    scores with tanh (from 1e-6 to 1e30 times the scale; None, 0 or less: no cap). ``shared_prefix``: that many first tokens of all sequences are in the same pages (a prompt with
     several continuations): they are read once for the whole batch. Keys in pages that are not there are left out;
     ``check_status=True`` waits for the GPU and raises then, also when ``shared_prefix`` tokens are not in the same pages.
     Returns out [B, H, T, D] (and lse [B, H, T], natural log, with ``return_lse``). No gradients."""

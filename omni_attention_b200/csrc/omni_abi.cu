@@ -612,7 +612,7 @@ const char* omni_attn_error_string(int code) {
     case OMNI_ERR_CUDA: return "a CUDA call failed (see omni_attn_last_cuda_error)";
     case OMNI_ERR_NO_DRIVER_ENTRY: return "cuTensorMapEncodeTiled not available from the CUDA driver";
     case OMNI_ERR_SCRATCH: return "scratch buffer smaller than OMNI_ATTN_SCRATCH_BYTES";
-    case OMNI_ERR_SOFTCAP: return "softcap must be >= 0 (0 = none); the plain kernel has no soft-cap";
+    case OMNI_ERR_SOFTCAP: return "softcap must be >= 0 (0 = none), over a paged cache from 1e-6 to 1e30 times the scale and at most 1e37; the plain kernel has no soft-cap";
     case OMNI_ERR_WORKSPACE: return "workspace smaller than omni_attn_bwd_workspace_bytes()";
     case OMNI_ERR_ROTARY: return "rotary_dim must be even, 0 <= rotary_dim <= head_dim, with inv_freq unless it is 0";
     case OMNI_ERR_CACHE:

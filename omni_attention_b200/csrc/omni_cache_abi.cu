@@ -101,6 +101,9 @@ bool vectors(const omni_attn_rotary* r, std::initializer_list<const omni_attn_he
   return r == nullptr || (!misaligned(r->q_weight) && !misaligned(r->k_weight));
 }
 
+// The kernels form scale / softcap to the sixth power, its inverse, and softcap * log2(e), all in 32 bits.
+bool soft_cap_fits(float softcap, float scale) { return softcap <= 1e37f && softcap >= 1e-6 * scale && softcap <= 1e30 * scale; }
+
 int heads_of(const omni_attn_heads* t) { return t == nullptr ? 0 : t->heads; }
 
 }  // namespace
@@ -238,7 +241,8 @@ int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* 
   if ((rc = check_cache(cache)) != OMNI_OK) return rc;
   if (q->heads <= 0 || q->heads % cache->heads != 0) return OMNI_ERR_CACHE;
   if (static_cast<long long>(B) * q->heads * T >= (1LL << 31) - 64) return OMNI_ERR_SHAPE;
-  if (!(softcap >= 0.f) || std::isinf(softcap)) return OMNI_ERR_SOFTCAP;
+  const float scale_used = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(head_dim));
+  if (!(softcap >= 0.f) || (softcap > 0.f && !soft_cap_fits(softcap, scale_used))) return OMNI_ERR_SOFTCAP;
   if (!rows_aligned(*q, 2) || misaligned(out) || misaligned(workspace)) return OMNI_ERR_ALIGNMENT;
   if (shared_prefix < 0) return OMNI_ERR_SEQLEN;
   CacheAttnParams p{};
@@ -272,7 +276,7 @@ int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* 
   p.num_pages = cache->num_pages;
   p.page_shift = shift_of(cache->page_size);
   p.causal = causal;
-  p.scale = scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(head_dim));
+  p.scale = scale_used;
   p.softcap = softcap;
   p.wait_cycles = wait_cycle_budget();
   if (!cache_attn_fits(p)) return OMNI_ERR_TOO_LONG;

@@ -376,6 +376,9 @@ pybind11::object cache_attention(torch::Tensor q, const torch::Tensor& k_pages, 
     const int32_t* limits_ptr = int32_or_null(limits, {B, T}, "limits must be contiguous int32 [B, T]");
     int32_t* status_ptr = const_cast<int32_t*>(int32_or_null(status, {1}, "status must be int32 [1]"));
     OMNI_REQUIRE(std::isfinite(static_cast<float>(scale)) && std::isfinite(static_cast<float>(softcap)) && scale >= 0.0, "scale and softcap must be finite, scale not negative");
+    const double scale_used = scale > 0.0 ? scale : 1.0 / std::sqrt(static_cast<double>(D));
+    OMNI_REQUIRE(!(softcap > 0.0) || (softcap >= 1.1e-6 * scale_used && softcap <= 0.9e30 * scale_used && softcap <= 0.9e37),
+                 "softcap must be between 1e-6 and 1e30 times the scale, and below 1e37 (None or 0: no soft-cap)");
     OMNI_REQUIRE(shared_prefix >= 0 && shared_prefix <= table.size(1) * k_pages.size(2), "shared_prefix must be from 0 to the tokens that the page table holds");
     OMNI_REQUIRE(!wants_grad({&q, &k_pages, &v_pages}),
             "omni_cache_attention has no backward: call it under torch.no_grad(), or on tensors that need no gradient");

@@ -228,6 +228,16 @@ def test_what_nobody_sees_changes_no_bit(cuda_device, D, dtype, H, T, causal, so
         assert torch.equal(out, results[0][0]) and torch.equal(lse, results[0][1])
 
 
+@pytest.mark.parametrize("H", [4, 40])
+@pytest.mark.parametrize("cap", [1.5e-7, 1e-3, 1e5, 1e29])
+def test_caps_near_the_ends_of_their_range(cuda_device, cap, H):
+    """From a cap that leaves nothing of the scores to one that changes nothing, zero scores among them."""
+    kp, vp, table, lens, g = make_cache(2, 2, 64, 16, [300, 20], 2, torch.float16, seed=13)
+    q = torch.randn(2, H, 2, 64, generator=g).half()
+    q[0, 1] = 0
+    run(q, kp, vp, table, lens, f"cap {cap}", softcap=cap)
+
+
 def same_kinds(got, want, tol, what):
     """Infinite with the sign, NaN and finite where the definition says so; the finite ones within tol."""
     got = got.double().cpu()

@@ -267,6 +267,22 @@ def test_c_entries_return_codes():
         assert lib.omni_attn_error_string(E[name]) != b"unknown error code"
 
 
+def test_caps_out_of_range():
+    """Caps whose quotients with the scale leave 32 bits: they came out as no cap, or as NaN and infinities."""
+    q, c = t(2, 4, 1, 64), cache()
+    for cap in (1e-300, 1e-50, 1e-40, 1e-8, 1.2e-7, 1e30, 2e37, 3e38):
+        refused("softcap must be", omni.omni_cache_attention, q, c, softcap=cap)
+    refused("softcap must be", omni.omni_cache_attention, q, c, softcap=50.0, scale=1e8)
+    refused("softcap must be", omni.omni_cache_attention, q, c, softcap=50.0, scale=1e-29)
+    for cap in (None, 0.0, -3.0, 1.5e-7, 50.0, 1e29):
+        refused("CUDA", omni.omni_cache_attention, q, c, softcap=cap)
+    E, lib, A, F, P = codes(), ops.load_library(), 0x10000, ctypes.c_float, ctypes.c_void_p   # nothing is read
+    full = dict(k=A, v=A, table=A, stride=4, lengths=A, num_pages=4, max_pages=4, page=16, heads=2)
+    for scale, cap in ((0.0, 1e-8), (0.0, 3e38), (1.0, 1e-7), (1e8, 50.0), (1e-30, 50.0), (1e30, 1e38)):
+        assert lib.omni_attn_cache_attention_sm100(ctypes.byref(Heads(A, 64, 64, 64, 4)), P(A), None, ctypes.byref(Cache(**full)), None, None, 1, 1, 1, 64, 0,
+                                                   F(scale), F(cap), 0, P(A), ctypes.c_longlong(1 << 30), None, None) == E["OMNI_ERR_SOFTCAP"]
+
+
 def test_learned_frequencies():
     """Nothing here has a gradient of inv_freq: refused where one is asked for."""
     r = omni.OmniRotary(torch.ones(32, dtype=torch.float64).requires_grad_())
