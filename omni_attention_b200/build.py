@@ -48,10 +48,16 @@ def _nvcc() -> str:
 def build_library(force: bool = False, verbose: bool = False) -> str:
     srcs = [os.path.join(CSRC, s) for s in CUDA_SOURCES]
     deps = srcs + [os.path.join(CSRC, h) for h in CUDA_HEADERS]
+    # one object per source, several at a time; an object that is newer than its source and all headers and was made by the same
+    # command stays, unless the compiler is to say what it does (verbose)
+    stamp, command = os.path.join(OBJ_DIR, "command.txt"), " ".join([_nvcc(), *NVCC_FLAGS])
+    same = os.path.exists(stamp) and open(stamp).read() == command
+    force = force or verbose or not same
     if not force and _newer(LIB_PATH, deps):
         return LIB_PATH
-    # one object per source, several at a time; an object that is newer than its source and all headers stays
     os.makedirs(OBJ_DIR, exist_ok=True)
+    if not same and os.path.exists(stamp):
+        os.remove(stamp)   # until all objects are made by the new command
     headers = [os.path.join(CSRC, h) for h in CUDA_HEADERS]
     objs = [os.path.join(OBJ_DIR, os.path.basename(s)[:-3] + ".o") for s in srcs]
     flags = [*NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else [])]
@@ -64,6 +70,8 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 1)) as pool:
         list(pool.map(compile_one, zip(srcs, objs)))
     subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *objs], check=True, cwd=CSRC)
+    with open(stamp, "w") as f:
+        f.write(command)
     return LIB_PATH
 
 
