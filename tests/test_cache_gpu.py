@@ -321,6 +321,31 @@ def test_infinite_values_with_many_rows(cuda_device, B, H, Hkv, T, D, page, leng
         same_kinds(got, want, tol, f"seed {seed}")
 
 
+@pytest.mark.parametrize("B,T,most,dtype", [(100, 3, 200, torch.bfloat16), (44, 1, 1500, torch.float16), (60, 12, 150, torch.float16), (44, 10, 900, torch.bfloat16)])
+def test_infinite_values_of_some_sequences(cuda_device, B, T, most, dtype):
+    """More (sequence, head) pairs than CTAs: what one piece of a CTA's work finds stays out of its next ones."""
+    H, Hkv, D, page = 8, 4, 64, 16
+    g = torch.Generator().manual_seed(14)
+    lengths = torch.randint(0, most, (B,), generator=g).tolist()
+    kp, vp, table, lens, g = make_cache(B, Hkv, D, page, lengths, T, dtype, seed=15)
+    q = torch.randn(B, H, T, D, generator=g).to(dtype)
+    clean = omni.omni_cache_attention(q.cuda(), on_gpu(kp, vp, table, lens)).cpu()
+    for b in range(0, B, 3):
+        n = lengths[b] + T
+        for i, col, sign in ((n - 1, 3, 1), (0, 9, -1), (n // 2, 20, 1)):
+            vp[int(table[b, i // page]), b % Hkv, i % page, col] = sign * math.inf
+    got = omni.omni_cache_attention(q.cuda(), on_gpu(kp, vp, table, lens)).cpu()
+    want = clean.clone()
+    for b in range(0, B, 3):
+        heads = slice(2 * (b % Hkv), 2 * (b % Hkv) + 2)
+        n = lengths[b] + T
+        for i, col, sign in ((n - 1, 3, 1), (0, 9, -1), (n // 2, 20, 1)):
+            for t in range(T):
+                if i <= lengths[b] + t:
+                    want[b, heads, t, col] = sign * math.inf
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("B,H,Hkv,T,D,page,lengths,dtype,more", [
     (1, 2, 1, 20, 128, 64, [300], torch.float16, {}),
     (2, 4, 2, 30, 64, 16, [100, 40], torch.bfloat16, {}),
