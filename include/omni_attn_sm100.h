@@ -397,7 +397,8 @@ int omni_attn_cache_append_sm100(const omni_attn_heads* q, const omni_attn_heads
  *                 break the promise are reported as OMNI_STATUS_BAD_INDEX.
  *  workspace      omni_attn_cache_attention_workspace_bytes(..., max_pages * page_size) bytes, 16-byte aligned; no state
  *                 between calls, calls that overlap in time need two. May be NULL where that is 0 (a small cache).
- * What a page holds behind a sequence's last token is never used. */
+ * What a page holds behind a sequence's last token is never used. The weights go into the product with 16 + 16 bits up to 16 query
+ * rows to a key/value head (H / heads * T, with a shared prefix times B), with 16 bits where there are more. */
 long long omni_attn_cache_attention_workspace_bytes(int B, int H, int kv_heads, int T, int head_dim, int shared_prefix,
                                                     long long capacity);
 int omni_attn_cache_attention_sm100(const omni_attn_heads* q, void* out, float* lse_or_null,

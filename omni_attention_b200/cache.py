@@ -119,6 +119,8 @@ def omni_cache_attention(q: Tensor, cache: OmniPagedCache, counts: Optional[Tens
     scores with tanh (from 1e-6 to 1e30 times the scale; None, 0 or less: no cap). ``shared_prefix``: that many first tokens of all sequences are in the same pages (a prompt with
     several continuations): they are read once for the whole batch. Keys in pages that are not there are left out;
     ``check_status=True`` waits for the GPU and raises then, also when ``shared_prefix`` tokens are not in the same pages.
+    Up to 16 query rows to a key/value head (H / Hkv * T, with ``shared_prefix`` times B) the result is off by its own rounding only,
+    with more the weights are rounded to 16 bits, as in ``omni_attention``.
     Returns out [B, H, T, D] (and lse [B, H, T], natural log, with ``return_lse``). No gradients."""
     if scale is not None and not scale >= torch.finfo(torch.float32).tiny:
         raise OmniAttnError(f"scale must be finite and positive (not zero, negative or NaN), got {scale}")

@@ -5,7 +5,7 @@
 // byte: with 16 rows that is a twentieth of what the card computes in the time of the read. So the query rows of a
 // key/value head go through the tensor cores together, as one tile of 8 or 16 rows (mma.sync: 16 rows would fill an eighth of
 // a tcgen05 tile), and all that matters is that enough reads are in flight on every SM. (More rows: omni_cache_wide.cu.)
-// Measured, 8 key/value heads of 128, bf16: 2 sequences of 131 072 tokens 159 us = 6.8 TB/s; 16 of up to 8 192 62 us = 5.8 TB/s,
+// Measured, 8 key/value heads of 128, bf16: 2 sequences of 131 072 tokens 159 us = 6.8 TB/s; 16 of up to 8 192 61-65 us by card = 5.5-5.9 TB/s,
 // 7 us of it before the first and after the last tile; 16 heads of 64, one sequence of 513 tokens 7.7 us, all of it latency.
 //
 // Split: the keys of all (sequence, key/value head, row tile) triples, in tiles of kTileKeys, form one line of units that is

@@ -6,8 +6,10 @@
 // (2 800 cycles), its two products 1 024; from 256 rows on the second row tile finds the keys in L2 and the chain scores ->
 // softmax -> P -> product bounds it. So the tiles of keys go to two softmax groups in turn, each with its own scores,
 // maximum, sum and O, and one group's chain runs under the other's products; at the end of a piece the groups' halves are
-// joined through shared memory. Measured, head_dim 128, bf16: 2 x 32 heads of 256 rows on 4 352 keys 53 us = 690 TFLOP/s (67 with
-// the soft-cap), 1 900 cycles a tile; the 16 384 shared tokens of 64 sequences, 8 key/value heads, 31 us.
+// joined through shared memory. Measured, head_dim 128, bf16: 2 x 32 heads of 256 rows on 4 352 keys 53 us = 690 TFLOP/s (69 with
+// the soft-cap): 34 tiles of 1 965 cycles, 20 500 cycles before the first and after the last (start 6 400, queries 4 800, first
+// scores 1 100, end 8 200), at 1.74 GHz in a loop (power cap) and up to 1.9 in a short run; the 16 384 shared tokens of 64 sequences,
+// 8 key/value heads, 31 us.
 //
 // Roles of a CTA (one per SM, 384 threads):
 //   warps 0-3, 4-7  softmax groups: thread = query row = TMEM lane. They also gather the rows' queries into shared memory
@@ -15,7 +17,9 @@
 //   warp 8          TMA: K and V of each tile of keys page by page into a ring (lane = page of the tile)
 //   warp 9          one elected thread issues every tcgen05.mma (warps 10 and 11 only give their registers up)
 // Hand-overs go through mbarriers; every wait is bounded as in the forward kernels. TMEM: S of the two groups (P, 16 bit,
-// over the first half of S), O of the two groups.
+// over the first half of S), O of the two groups. P is one 16-bit value, as in the block-mask forward (with its rest as a second
+// operand, as in omni_cache_attn.cu, the products would take half as long again, and the rest's columns in TMEM are the next
+// scores'): the error against 64 bits is 2.3e-3 of the result's norm where its own rounding to bf16 is 1.7e-3.
 //
 // A value that is infinite or NaN must not reach the rows that do not see its key (0 * NaN): where rows of a tile see
 // different numbers of keys it is taken out of the product. What such values make of the rows that see them is found when
@@ -45,8 +49,8 @@ struct WideCfg {
   static constexpr int kSlots = D == 128 ? 6 : 10;   // K and V tiles in flight
   // Scores of a tile in two halves of 64 keys: the second half is computed as soon as the group has read the scores before for
   // the last time, under their exponentials, and its maximum is looked for under the first half's product. 2 x 16 heads of 256
-  // rows on 4 352 keys: head_dim 64 33.9 -> 31.2 us; head_dim 128 (32 heads) 53.2 -> 55.9, because a product 64 keys wide
-  // reads the queries twice as often and shared memory is what bounds it.
+  // rows on 4 352 keys: head_dim 64 33.9 -> 31.2 us; head_dim 128 (32 heads) 53.2 -> 55.9 (a product 64 keys wide
+  // reads the queries from shared memory twice as often; no counter shows whether that is the reason).
   static constexpr bool kHalves = D == 64;
   static constexpr int kBars = (1 + kSlots) * kTile;
   // Behind the tiles: barriers, flags and limits, which keys are there, row states, the piece's description.

@@ -15,8 +15,9 @@
 // Bound: memory - each element is read once and written once, about ten operations between. A thread owns 8 pairs (16
 // elements) of a token and keeps their cosines and sines in registers while it walks over the heads, so that these are
 // computed once per token and group of heads, not once per row; D / 16 threads are a row, and the norm's sums go through
-// that many lanes' shuffles. Measured, 64 heads of 128, 8 192 tokens, bf16: forward 46 us for 268 MB, backward with norms 67 us
-// for 402 MB (5.8 and 6.0 TB/s) and 5 us for the weights' sums.
+// that many lanes' shuffles. Measured, 64 heads of 128, 8 192 tokens, bf16: forward 47 us for 268 MB, backward with norms 67 us
+// for 402 MB (5.7 and 6.0 TB/s) and 5 to 7 us for the weights' sums; fp32: 106 us for 537 MB, with norms 155 us in all for 805 MB
+// (5.1 and 5.2), without 97 us for 537 MB.
 #include "omni_cache_line.cuh"
 #include "omni_launch.h"
 #include "omni_rotary.cuh"

@@ -121,7 +121,7 @@ def omni_rotary(q: Optional[Tensor], k: Optional[Tensor], rotary: Optional[OmniR
                 positions: Optional[Tensor] = None, q_weight: Optional[Tensor] = None, k_weight: Optional[Tensor] = None,
                 eps: float = 1e-6) -> Tuple[Optional[Tensor], Optional[Tensor]]:
     """Queries and keys, normed per head (where a weight is given) and turned by their positions; differentiable with
-    respect to q, k and the weights.
+    respect to q, k and the weights (not to ``inv_freq``, not twice, not in forward mode: refused).
 
     q [B, H, N, D], k [B, Hkv, N, D]: CUDA tensors of one dtype (fp16, bf16, fp32), D 32, 64 or 128, any strides (rows that
     are contiguous along D and start on 16-byte boundaries are read where they lie; others are read element by element,
