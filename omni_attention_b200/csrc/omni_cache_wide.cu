@@ -83,11 +83,6 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t addr, float (&f)[COLS]) {
   }
 }
 
-template <bool BF16>
-__device__ __forceinline__ float value16(uint16_t raw) {
-  return BF16 ? __uint_as_float(static_cast<uint32_t>(raw) << 16) : __half2float(__ushort_as_half(raw));
-}
-
 // Zeros in the place of scores that are not allowed.
 __device__ __forceinline__ void zero_not_allowed64(uint32_t allow0, uint32_t allow1, float (&s)[64]) {
 #pragma unroll
@@ -113,14 +108,15 @@ __device__ __noinline__ bool take_out_not_finite(uint8_t* row, int r, int pitch)
 
 // By the eight softmax warps, when a piece is written: elements whose row sees infinite or NaN values in their column are what
 // these add up to (the product has them as zeros, as inf, or as NaN where an fp16 weight is below the type's smallest).
-// Keys key0 .. key1, a thread's row (keys below `lim`, columns c0 .. c1) in `out`, or in `share` (32 bit). `keys`: 8 words in
-// shared memory. From memory, a key to a thread; then the keys that have such values, row by row.
+// Keys key0 .. key1, a thread's row (keys below `lim`, columns c0 .. c1, 64 at most) in `out`, or in `share` (32 bit). `keys`: 8
+// words in shared memory. From memory, a key to a thread; then the keys that have such values, row by row.
 template <bool BF16>
 __device__ __noinline__ void write_not_finite(const CacheAttnParams& p, const Piece& pc, int key0, int key1, int lim, int d, int c0, int c1, float* share,
                                               uint16_t* out, volatile uint32_t* keys) {
   const int tid = threadIdx.x, mask = (1 << p.page_shift) - 1;
   const int* table = p.page_table + pc.table_of * p.table_stride;
-  unsigned long long met = 0;   // columns that met one
+  unsigned long long plus = 0, minus = 0;   // columns that met +inf or NaN, -inf or NaN: both is NaN
+  const unsigned long long all = c1 - c0 == 64 ? ~0ull : (1ull << (c1 - c0)) - 1;
   auto values = [&](int key) -> const uint16_t* {
     const int page = __ldg(table + (key >> p.page_shift));
     if (page < 0 || page >= p.num_pages) return nullptr;
@@ -138,23 +134,35 @@ __device__ __noinline__ void write_not_finite(const CacheAttnParams& p, const Pi
     for (int w = 0; w < 8; ++w) {
       for (uint32_t left = keys[w]; left != 0; left &= left - 1) {
         const int key = base + 32 * w + __ffs(left) - 1;
-        if (key >= lim) break;
+        if (key >= lim || (plus & minus) == all) break;
         const uint16_t* v = values(key);
-        for (int c = c0; c < c1; ++c) {
-          const uint16_t raw = __ldg(v + c);
-          if ((raw & kExponent<BF16>) != kExponent<BF16>) continue;
-          const float x = value16<BF16>(raw);
-          const bool again = met >> (c - c0) & 1u;
-          met |= 1ull << (c - c0);
-          if (share != nullptr) {
-            share[c] = again ? share[c] + x : x;
-          } else {
-            out[c] = static_cast<uint16_t>(pack2<BF16>(again ? value16<BF16>(out[c]) + x : x, 0.f));
+        for (int c = c0; c < c1; c += 8) {
+          const uint4 eight = __ldg(reinterpret_cast<const uint4*>(v + c));
+          if (!not_finite<BF16>(eight)) continue;
+          const uint32_t words[4] = {eight.x, eight.y, eight.z, eight.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t raw = words[i >> 1] >> (16 * (i & 1)) & 0xFFFFu;
+            if ((raw & kExponent<BF16>) != kExponent<BF16>) continue;
+            const bool nan = (raw & 0x7FFFu) != kExponent<BF16>;
+            const unsigned long long bit = 1ull << (c - c0 + i);
+            if (nan || !(raw >> 15)) plus |= bit;
+            if (nan || raw >> 15) minus |= bit;
           }
         }
       }
     }
     softmax_sync();   // the next words go over these
+  }
+  for (unsigned long long left = plus | minus; left != 0; left &= left - 1) {
+    const int i = __ffsll(left) - 1;
+    const bool up = plus >> i & 1u, down = minus >> i & 1u;
+    const float x = up && down ? __int_as_float(0x7FFFFFFF) : up ? INFINITY : -INFINITY;
+    if (share != nullptr) {
+      share[c0 + i] = x;
+    } else {
+      out[c0 + i] = static_cast<uint16_t>(pack2<BF16>(x, 0.f));
+    }
   }
 }
 
