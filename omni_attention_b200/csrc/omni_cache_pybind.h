@@ -333,7 +333,7 @@ pybind11::object cache_append(const torch::Tensor& k_pages, const torch::Tensor&
     OMNI_REQUIRE(cache.heads == k.size(1), "the cache's heads are not those of k");
     const int32_t* counts_ptr = int32_or_null(counts, {B}, "counts must be contiguous int32 [B]");
     int32_t* status_ptr = const_cast<int32_t*>(int32_or_null(status, {1}, "status must be int32 [1]"));
-    OMNI_REQUIRE(!wants_grad({&q, &k, &v, &r.q_weight, &r.k_weight, &r.inv_freq}),
+    OMNI_REQUIRE(!wants_grad({&q, &k, &v, &r.q_weight, &r.k_weight, &r.inv_freq, &k_pages, &v_pages}),
             "omni_cache_append has no backward: call it under torch.no_grad(), or on tensors that need no gradient");
     check_no_tangent("omni_cache_append", {&q, &k, &v, &r.q_weight, &r.k_weight, &r.inv_freq, &k_pages, &v_pages});
     check_device(k, {&v, &q, &k_pages, &v_pages, &table, &lengths, &counts, &status, &r.inv_freq, &r.positions, &r.q_weight, &r.k_weight});

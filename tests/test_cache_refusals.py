@@ -293,6 +293,19 @@ def test_learned_frequencies():
         refused("CUDA", omni.omni_rotary, t(1, 1, 3, 64), None, r)
 
 
+def test_pages_that_require_a_gradient():
+    """Writing into them would cut their graph without a word, as an operation in place on such a leaf would: refused, but not
+    under no_grad."""
+    k = t(2, 2, 3, 64)
+    for which in ("k_pages", "v_pages"):
+        c = cache()
+        getattr(c, which).requires_grad_()
+        refused("no backward", omni.omni_cache_append, c, k, k)
+        refused("no backward", omni.omni_cache_attention, k, c)
+        with torch.no_grad():
+            refused("CUDA", omni.omni_cache_append, c, k, k)
+
+
 def test_forward_mode():
     """A tangent is refused, whether something requires a gradient or not: it would be dropped."""
     from torch.autograd import forward_ad as fw
