@@ -683,7 +683,9 @@ __global__ void __launch_bounds__(256) omni_cache_join_kernel(const __grid_const
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xFFFFFFFFu, to, o));
       const float ref = to == -INFINITY ? 0.f : to;
-      const float f1 = ex2_approx(top - ref), f2 = ex2_approx(m2 - ref);
+      // A share's weight is not 0 while it has keys: 0 * inf. (2^-126 of the largest shows in nothing else.)
+      constexpr float kLeast = 1.17549435e-38f;
+      const float f1 = top == -INFINITY ? 0.f : fmaxf(ex2_approx(top - ref), kLeast), f2 = m2 == -INFINITY ? 0.f : fmaxf(ex2_approx(m2 - ref), kLeast);
       float part = l2 * f2;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xFFFFFFFFu, part, o);

@@ -321,6 +321,31 @@ def test_infinite_values_with_many_rows(cuda_device, B, H, Hkv, T, D, page, leng
         same_kinds(got, want, tol, f"seed {seed}")
 
 
+@pytest.mark.parametrize("H", [1, 12, 40])
+@pytest.mark.parametrize("length", [60, 700, 5000])
+@pytest.mark.parametrize("late", [True, False])
+def test_an_infinite_value_of_a_key_that_weighs_next_to_nothing(cuda_device, H, length, late):
+    """Its weight is exp(-110) of the largest, nothing in 32 bits: by the definition the result is infinite all the same, wherever
+    the keys are cut."""
+    D, page = 64, 16
+    kp, vp, table, lens, g = make_cache(1, 1, D, page, [length], 1, torch.bfloat16, seed=16)
+    n = length + 1
+    heavy = range(n // 2, n) if late else range(0, n // 2)
+    for i in range(n):
+        p, row = int(table[0, i // page]), i % page
+        kp[p, 0, row] = 0.0
+        kp[p, 0, row, 0] = 110.0 if i in heavy else 0.0      # the scores: 110 and 0
+    light = 0 if late else n - 1
+    vp[int(table[0, light // page]), 0, light % page, 3] = math.inf
+    q = torch.zeros(1, H, 1, D, dtype=torch.bfloat16)
+    q[..., 0] = 8.0
+    got = omni.omni_cache_attention(q.cuda(), on_gpu(kp, vp, table, lens)).cpu()
+    want = orc.attention(q, kp, vp, table, lens)[0]
+    assert (want[..., 3] == math.inf).all() and (got[..., 3] == math.inf).all()
+    rest = [c for c in range(D) if c != 3]
+    assert torch.isfinite(got[..., rest]).all() and float((got.double() - want)[..., rest].abs().max()) <= 2.0 ** -8 * 5
+
+
 @pytest.mark.parametrize("B,T,most,dtype", [(100, 3, 200, torch.bfloat16), (44, 1, 1500, torch.float16), (60, 12, 150, torch.float16), (44, 10, 900, torch.bfloat16)])
 def test_infinite_values_of_some_sequences(cuda_device, B, T, most, dtype):
     """More (sequence, head) pairs than CTAs: what one piece of a CTA's work finds stays out of its next ones."""
