@@ -304,7 +304,7 @@ __device__ __forceinline__ void sincos_turns(float2 turns, float2& sn, float2& c
   place(__float_as_int(sum.y), s.y, c.y, sn.y, cs.y);
 }
 // Cosines and sines of the thread's pairs at a position, with the factor. EXACT: as above, for results in 32 bits: fp32 data, and
-// gradients of weights, which may be fp32 whatever the data's type. Else the special function unit's sine and cosine, which take
+// gradients of fp32 weights whatever the data's type. Else the special function unit's sine and cosine, which take
 // fewer instructions: the unit's own 2^-21.2 for angles within half a turn, 2^-23.4 of the turns, 2^-23 of the product with 2 pi and
 // 2^-23.4 of 2 pi itself, less than 2^-20.4 together. Forward, bf16, head_dim 128: 64 heads of 8 192 tokens 47.3 us EXACT and 46.9,
 // 8 heads of 65 536 53.3 and 51.0, 2 heads of 262 144 92.6 and 84.4.
@@ -334,23 +334,31 @@ __device__ __forceinline__ void turn_of(const RotaryParams& p, const Place<D, HA
 template <bool VEC, int D, bool HALF>
 __device__ __forceinline__ void rotate(Pairs& x, const Turn& r, const Place<D, HALF>& at) {
   const int n = at.rd2 - at.pair(0);   // how many are rotated
-  if (n <= 0) return;
+  if constexpr (VEC) {
+    if (n <= 0) return;
+  }
   Pairs y;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 minus = make_float2(-r.s[i].x, -r.s[i].y);
     y.a[i] = __ffma2_rn(x.b[i], minus, __fmul2_rn(x.a[i], r.c[i]));
     y.b[i] = __ffma2_rn(x.b[i], r.c[i], __fmul2_rn(x.a[i], r.s[i]));
+    if constexpr (!VEC) {   // fewer registers: fp32, a weight for each head, half layout, rows off their boundaries 342 us with the branches, 315 so
+      x.a[i] = make_float2(2 * i < n ? y.a[i].x : x.a[i].x, 2 * i + 1 < n ? y.a[i].y : x.a[i].y);
+      x.b[i] = make_float2(2 * i < n ? y.b[i].x : x.b[i].x, 2 * i + 1 < n ? y.b[i].y : x.b[i].y);
+    }
   }
   if constexpr (VEC && HALF) {
     x = y;
-  } else if (n >= 8) {
-    x = y;
-  } else {
+  } else if constexpr (VEC) {
+    if (n >= 8) {
+      x = y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (2 * i < n) x.a[i].x = y.a[i].x, x.b[i].x = y.b[i].x;
-      if (2 * i + 1 < n) x.a[i].y = y.a[i].y, x.b[i].y = y.b[i].y;
+      for (int i = 0; i < 4; ++i) {
+        if (2 * i < n) x.a[i].x = y.a[i].x, x.b[i].x = y.b[i].x;
+        if (2 * i + 1 < n) x.a[i].y = y.a[i].y, x.b[i].y = y.b[i].y;
+      }
     }
   }
 }
@@ -605,7 +613,13 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) omni_rotary_bwd_kernel(
     };
 #pragma unroll 1
     for (int i = 0; i < kStages - 1; ++i) read_ahead(i);
-    turn_of<true>(p, at, position_of(p, b, n), turn);   // sign = -1: the rotation back
+    // sign = -1: the rotation back. A weight for each head means angles for each row: 106 us with the unit's sines, 117 EXACT (64 heads
+    // of 8 192 tokens, bf16, half layout).
+    if (sizeof(T) == 4 || p.w_f32) {
+      turn_of<true>(p, at, position_of(p, b, n), turn);
+    } else {
+      turn_of<false>(p, at, position_of(p, b, n), turn);
+    }
 #pragma unroll 1
     for (int i = 0; i < n_rows; ++i) {
       Pairs v, d;
